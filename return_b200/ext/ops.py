@@ -121,6 +121,9 @@ def core() -> ctypes.CDLL:
     return _core
 
 
+_TREE_SOURCES = ["attention_tree.cu"]
+_BRANCH_SOURCES = ["branch.cu", "beam.cu"]
+
 # head sizes compiled ahead of time by build_all(); any other multiple of 16 compiles on first use
 PREBUILT_HEAD_DIMS = (16, 32, 48, 64, 128)
 
@@ -136,6 +139,8 @@ def build_all():
     paths.append(build.library_path("return_latent", _LATENT_SOURCES, {"RB_PDL_MODE": PDL_MODE}))
     paths.append(build.library_path("return_moe", _MOE_SOURCES, {"RB_PDL_MODE": PDL_MODE}))
     paths.append(build.library_path("return_moe_tc5", _MOE_TC5_SOURCES, {"RB_PDL_MODE": PDL_MODE}))
+    paths.append(build.library_path("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE}))
+    paths.append(build.library_path("return_branch", _BRANCH_SOURCES, {"RB_PDL_MODE": PDL_MODE}))
     for d in TC5_ATTENTION_HEAD_DIMS:
         paths.append(build.library_path(f"return_attn_tc5_d{d}", ["attention_tc5.cu"], _attn_tc5_defines(d)))
     for d in PREBUILT_HEAD_DIMS:
@@ -2228,3 +2233,282 @@ def argmax(logits, tokens_out) -> None:
     n, V = logits.shape
     assert logits.dtype == torch.float32 and logits.stride(1) == 1 and tokens_out.dtype == torch.int32
     _check(core().rb_argmax(_ptr(logits), logits.stride(0), n, V, _ptr(tokens_out), _stream()), "argmax")
+
+
+# ------------------------------------------------------------------------------- several continuations of a request
+
+_tree = _branch = None
+
+TREE_MAX_NODES = 256               # drafted nodes of a segment
+TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
+TREE_MIN_SHARE = 4                 # a CTA of split keys walks at least so many tiles
+TREE_MAX_SPLITS = 64
+TREE_SCRATCH_BYTES = 256 << 20
+
+
+def tree_lib() -> ctypes.CDLL:
+    """The attention kernels for drafted trees."""
+    global _tree
+    if _tree is None:
+        lib = build.load("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE})
+        P, I, F = c_void_p, c_int, c_float
+        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, P]
+        lib.rb_tree_attention.restype = c_int
+        _tree = build.native_calls(lib)
+    return _tree
+
+
+def branch_lib() -> ctypes.CDLL:
+    """The kernels that commit a drafted tree, copy pages and state slots, and select beams."""
+    global _branch
+    if _branch is None:
+        lib = build.load("return_branch", _BRANCH_SOURCES, {"RB_PDL_MODE": PDL_MODE})
+        P, I, L = c_void_p, c_int, ctypes.c_longlong
+        lib.rb_tree_commit.argtypes = [P, P, P, P, P, I, P, I, I, P, I, I, I, I, P, P, P, I, P]
+        lib.rb_copy_pages.argtypes = [P, P, P, P, I, I, I, I, I, I, P]
+        lib.rb_copy_slots.argtypes = [P, I, P, P, I, I, P]
+        lib.rb_beam_select.argtypes = [P, L, P, I, I, I, I, P, P, P, P, P]
+        lib.rb_beam_scratch.argtypes = [I, I, I]
+        lib.rb_beam_scratch.restype = L
+        for name in ("rb_tree_commit", "rb_copy_pages", "rb_copy_slots", "rb_beam_select"):
+            getattr(lib, name).restype = c_int
+        _branch = build.native_calls(lib)
+    return _branch
+
+
+def _same_device(device, *tensors) -> None:
+    """Every tensor of a call lies on one CUDA device, the current one: kernels are launched there."""
+    for t in tensors:
+        if t is not None:
+            if not (t.is_cuda):
+                raise KernelError("the engine's kernels run on a CUDA device only; got a CPU tensor")
+            if not (t.device == device):
+                raise KernelError(f"tensors on {t.device} and {device} in one call")
+    if not (device.index == _device_index()):
+        raise KernelError(f"tensors on {device}, but the current device is cuda:{_device_index()}")
+
+
+def _ints(what: str, t: torch.Tensor, *shape) -> None:
+    if not (t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape):
+        raise KernelError(f"{what}: contiguous int32 of shape {shape} wanted, got {t.dtype} {tuple(t.shape)}")
+
+
+def _tree_lengths(batch, page_size: int, blocks: int):
+    """(longest tree, longest tree's end in slots) of a step of drafted trees, checked once per step and block table size."""
+    key = ("tree.lengths", page_size, blocks)
+    held = batch.scratch.get(key)
+    if held is None:
+        cu, first = batch.host.cu_q, batch.host.seg_pos0
+        n = len(first)
+        nodes = [int(cu[i + 1]) - int(cu[i]) for i in range(n)]
+        if not (len(cu) == n + 1 and n > 0 and min(nodes) >= 1):
+            raise KernelError("every segment of a tree step brings at least one node")
+        if not (max(nodes) <= TREE_MAX_NODES):
+            raise KernelError(f"a drafted tree of {max(nodes)} nodes; the kernels take {TREE_MAX_NODES}")
+        ends = [int(p) + k for p, k in zip(first, nodes)]
+        if not (min(int(p) for p in first) >= 0 and max(ends) <= page_size * blocks):
+            raise KernelError(f"the block table holds {page_size * blocks} slots of a segment, a tree ends at {max(ends)}")
+        T = int(cu[-1])
+        _ints("cu_q", batch.cu_q, n + 1)
+        _ints("seg_pos0", batch.seg_pos0, n)
+        _ints("tree_parent", batch.tree_parent, T)
+        held = batch.scratch[key] = (n, T, max(nodes), nodes, ends)
+    return held
+
+
+def tree_shares(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int):
+    """(splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; (1, 0): no split.  The
+    shares are as long as they can be while the launch's CTAs fill the GPU once."""
+    tiles = [(e - 1) // TREE_KEY_TILE - (max(0, e - k - window + 1) if window else 0) // TREE_KEY_TILE + 1 for k, e in zip(nodes, ends)]
+    blocks = [-(-k * rows_per_node // cta_rows) * kv_heads for k in nodes]
+    slots, longest = num_sms() * ctas_per_sm, max(tiles)
+    if sum(blocks) >= slots or longest < 2 * TREE_MIN_SHARE:
+        return 1, 0
+    most = max(1, min(TREE_MAX_SPLITS, TREE_SCRATCH_BYTES // max(1, rows * (head_dim + 2) * 4)))
+    lo, hi = max(TREE_MIN_SHARE, -(-longest // most)), longest
+    while lo < hi:                                     # the smallest share whose CTAs fit at once
+        mid = (lo + hi) // 2
+        if sum([b * -(-t // mid) for b, t in zip(blocks, tiles)]) <= slots:
+            hi = mid
+        else:
+            lo = mid + 1
+    splits = -(-longest // lo)
+    return (splits, lo) if splits > 1 else (1, 0)
+
+
+def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window=None,
+                   sink=None, softcap=None) -> None:
+    """Attention of a step whose segments are drafted trees; out [T, Hq*D].  Node i of a segment (``batch.tree_parent[i]`` is the
+    index in the segment of the node before it, below i, -1 for the root) has its key and value in slot ``seg_pos0 + i`` already and
+    stands at position ``seg_pos0 + depth(i)``; it sees the segment's cached keys, its ancestors and itself, with a window those
+    less than ``window`` positions back.  ``qkv``: rows that begin with the rotated queries (row stride any).  ``softcap``,
+    ``sink``: as in ``paged_attention``.  A segment has up to TREE_MAX_NODES nodes."""
+    T = qkv.shape[0]
+    n, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
+    if not (num_heads % num_kv_heads == 0 and 0 < head_dim <= 256):
+        raise KernelError("query heads: a multiple of the kv heads; head size: up to 256")
+    if not (qkv.dim() == 2 and qkv.stride(1) == 1 and T == rows and qkv.shape[1] >= num_heads * head_dim):
+        raise KernelError("qkv: a row per node, unit stride")
+    if not (k_pool.dtype == v_pool.dtype == qkv.dtype == out.dtype):
+        raise KernelError("queries, keys, values and output are of one type")
+    if not (tuple(k_pool.shape[1:]) == (num_kv_heads, page_size, head_dim) and k_pool.shape == v_pool.shape and k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise KernelError("pools: contiguous [pages, kv heads, page size, head size]")
+    if not (tuple(out.shape) == (T, num_heads * head_dim) and out.is_contiguous()):
+        raise KernelError("out: contiguous [nodes, heads * head size]")
+    if not (block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n and block_table.stride(1) == 1):
+        raise KernelError("block_table: int32 [segments, blocks]")
+    if not (window is None or window >= 0):
+        raise KernelError("window: not negative")
+    if not (softcap is None or softcap >= 0):
+        raise KernelError("softcap: not negative")
+    _same_device(qkv.device, qkv, k_pool, v_pool, block_table, out, batch.cu_q, batch.tree_parent, sink)
+    window = int(window or 0)
+    lib = tree_lib()
+    key = ("tree.shares", num_heads, num_kv_heads, head_dim, window, qkv.dtype)
+    shares = batch.scratch.get(key)
+    if shares is None:
+        shares = batch.scratch[key] = tree_shares(nodes, ends, window, num_heads // num_kv_heads, num_kv_heads, rows * num_heads, head_dim,
+                                                  32, 2 if head_dim <= 128 else 1)
+    splits, share = shares
+    # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
+    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
+    _check(lib.rb_tree_attention(_ptr(qkv), qkv.stride(0), _ptr(k_pool), _ptr(v_pool), _ptr(batch.cu_q), _ptr(batch.seg_pos0),
+                                 _ptr(batch.tree_parent), _ptr(block_table), block_table.stride(0), page_size, _ptr(out),
+                                 dtype_code(qkv.dtype), n, longest, T, num_heads, num_kv_heads, head_dim, float(scale), window,
+                                 float(softcap or 0.0), _sink_ptr(sink, num_heads), splits, share, _ptr(scratch), _stream()),
+           "tree_attention", 2 if splits > 1 else 1)
+
+
+def _pool_shape(pool):
+    """(planes, pages, heads, page size, bytes of a row) of a group's pool: [layers, 2, pages, heads, page size, n] or, for a cache of
+    latents, [layers, pages, page size, n]."""
+    if not (pool.dim() in (4, 6) and pool.is_contiguous() and pool.numel() > 0 and pool.element_size() >= 2):
+        raise KernelError("a pool: contiguous [layers, 2, pages, heads, page size, n] or [layers, pages, page size, n], 16-bit elements or wider")
+    s = pool.shape
+    heads = s[3] if pool.dim() == 6 else 1
+    return s[0] * s[1] if pool.dim() == 6 else s[0], s[-4] if pool.dim() == 6 else s[1], heads, s[-2], s[-1] * pool.element_size()
+
+
+def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
+    """Which nodes of the step's drafted trees hold, and their keys and values moved up.  ``sampled`` (int32 [T]): the token that follows
+    each node.  From a segment's root (node 0) on, a node's child holds if its token (``batch.tokens``) is the one sampled behind the
+    node; the lowest such child where there are several.  ``path`` (int32 [n, w], w at least the longest tree): the nodes that hold, in
+    order, then -1; ``count`` (int32 [n]) how many; ``emitted`` (int32 [n, w]): the token sampled behind each of them, then -1.
+    ``caches``: (pool, block_table) of every group of layers; the row of slot ``seg_pos0 + path[i]`` goes to slot ``seg_pos0 + i``.  The
+    request then holds ``seg_pos0 + count`` tokens.  Other rows stay as they are; a move from or to a page that the table marks as
+    gone is left out."""
+    n, T = len(batch.host.seg_pos0), int(batch.host.cu_q[-1])
+    width = path.shape[1] if path.dim() == 2 else 0
+    pools = [(pool, table, _pool_shape(pool)) for pool, table in caches]
+    lengths = None
+    for _, table, shape in pools:
+        if not (table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == n and table.stride(1) == 1):
+            raise KernelError("block_table: int32 [segments, blocks]")
+        lengths = _tree_lengths(batch, shape[3], table.shape[1])
+    if lengths is None:                                # a model without paged layers: the walk alone
+        lengths = _tree_lengths(batch, 1 << 30, 1)
+    _ints("sampled", sampled, T)
+    _ints("tokens", batch.tokens, T)
+    if not (width >= lengths[2]):
+        raise KernelError(f"path: {lengths[2]} columns at least")
+    _ints("path", path, n, width)
+    _ints("emitted", emitted, n, width)
+    _ints("count", count, n)
+    _same_device(sampled.device, sampled, batch.tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted,
+                 *[t for pool, table, _ in pools for t in (pool, table)])
+    lib = branch_lib()
+    args = (_ptr(batch.tokens), _ptr(batch.tree_parent), _ptr(sampled), _ptr(batch.cu_q), _ptr(batch.seg_pos0), n)
+    outs = (_ptr(path), _ptr(count), _ptr(emitted), width)
+    if not pools:
+        _check(lib.rb_tree_commit(*args, None, 0, 1, None, 0, 0, 0, 0, *outs, _stream()), "tree_commit")
+    for pool, table, (planes, pages, heads, page_size, row_bytes) in pools:
+        _check(lib.rb_tree_commit(*args, _ptr(table), table.stride(0), page_size, _ptr(pool), planes, pages, heads, row_bytes, *outs, _stream()),
+               "tree_commit")
+        outs = (None, None, None, 0)
+
+
+def copy_pages(pool, src, dst, rows) -> None:
+    """The first ``rows[i]`` token rows of page ``src[i]`` copied to page ``dst[i]`` (int32 [n] each), in all layers, keys and values and
+    heads of a group's pool.  A destination appears once and is no source.  A copy from or to a page that the pool does not have
+    (-1) is left out; ``rows`` beyond the page end with it."""
+    n = src.numel()
+    planes, pages, heads, page_size, row_bytes = _pool_shape(pool)
+    for name, t in (("src", src), ("dst", dst), ("rows", rows)):
+        _ints(name, t, n)
+    _same_device(pool.device, pool, src, dst, rows)
+    if n:
+        _check(branch_lib().rb_copy_pages(_ptr(pool), _ptr(src), _ptr(dst), _ptr(rows), n, planes, pages, heads, page_size, row_bytes,
+                                          _stream()), "copy_pages")
+
+
+class SlotTable:
+    """The state tensors of a model, [slots, ...] each, all of one device: what ``copy_slots`` works on.  Made once (``slot_table``); it
+    holds the tensors."""
+
+    def __init__(self, states):
+        self.states = list(states)
+        if not (len(self.states) > 0):
+            raise KernelError("a slot table needs at least one tensor")
+        self.device, self.slots = self.states[0].device, self.states[0].shape[0] if self.states[0].dim() else 0
+        rows = []
+        for t in self.states:
+            if not (t.is_cuda and t.device == self.device):
+                raise KernelError("the states lie on one CUDA device")
+            if not (t.dim() >= 1 and t.shape[0] == self.slots and self.slots > 0 and t.is_contiguous() and t.numel() > 0):
+                raise KernelError("states: contiguous [slots, ...], as many slots each")
+            rows.append(t.numel() // self.slots * t.element_size())
+        self._host = (ctypes.c_longlong * (2 * len(rows)))(*[t.data_ptr() for t in self.states], *rows)
+        self.address, self.launches = ctypes.addressof(self._host), -(-len(rows) // SLOT_TENSORS)
+
+
+SLOT_TENSORS = 64                  # tensors that one launch takes
+
+
+def slot_table(states) -> SlotTable:
+    return SlotTable(states)
+
+
+def copy_slots(table: SlotTable, src, dst) -> None:
+    """Row ``dst[i]`` of every state tensor <- row ``src[i]`` (int32 [n] each).  A destination appears once and is no source.  A copy
+    from or to a slot that does not exist is left out."""
+    n = src.numel()
+    _ints("src", src, n)
+    _ints("dst", dst, n)
+    _same_device(table.device, src, dst)
+    if n:
+        _check(branch_lib().rb_copy_slots(table.address, len(table.states), _ptr(src), _ptr(dst), n, table.slots, _stream()), "copy_slots",
+               table.launches)
+
+
+BEAM_MAX_KEEP, BEAM_MAX_BEAMS = 128, 64
+
+
+def beam_select(logits, scores, beams: int, scores_out, beams_out, tokens_out) -> None:
+    """The ``scores_out.shape[1]`` best continuations of every request, best first.  ``logits`` float32 [requests * beams, V];
+    ``scores`` float32 [requests * beams], the beams' sums of log-probabilities.  A continuation (b, v) has the total
+    scores[b] + log_softmax(logits[b])[v]; ties go to the lowest (b, v).  A total that is no number, and every one of a beam whose
+    score is not finite, counts as -inf.  Out: totals (float32), beams and tokens (int32), [requests, keep] each."""
+    if not (logits.dim() == 2 and scores_out.dim() == 2):
+        raise KernelError("logits [requests * beams, V], scores_out [requests, keep]")
+    (rows, V), (requests, keep) = logits.shape, scores_out.shape
+    if not (1 <= beams <= BEAM_MAX_BEAMS and rows == requests * beams):
+        raise KernelError(f"logits: a row per request and beam, up to {BEAM_MAX_BEAMS} beams")
+    if not (1 <= keep <= min(BEAM_MAX_KEEP, beams * V)):
+        raise KernelError(f"{keep} continuations asked for: 1 to {BEAM_MAX_KEEP}, and no more than there are")
+    if not (rows <= 65535 and beams * V < 2 ** 31 - 1):
+        raise KernelError("at most 65,535 rows, and beams * V within 31 bits")
+    if not (logits.dtype == torch.float32 and logits.stride(1) == 1):
+        raise KernelError("logits: float32, unit stride along a row")
+    if not (scores.dtype == torch.float32 and scores.is_contiguous() and scores.numel() == rows):
+        raise KernelError("scores: float32, one per row of logits")
+    if not (scores_out.dtype == torch.float32 and scores_out.is_contiguous()):
+        raise KernelError("scores_out: contiguous float32")
+    _ints("beams_out", beams_out, requests, keep)
+    _ints("tokens_out", tokens_out, requests, keep)
+    _same_device(logits.device, logits, scores, scores_out, beams_out, tokens_out)
+    if requests == 0:
+        return
+    lib = branch_lib()
+    scratch = torch.empty(lib.rb_beam_scratch(rows, V, keep), dtype=torch.float32, device=logits.device)
+    _check(lib.rb_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), requests, beams, V, keep, _ptr(scores_out), _ptr(beams_out),
+                              _ptr(tokens_out), _ptr(scratch), _stream()), "beam_select", 2)
