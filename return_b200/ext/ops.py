@@ -2240,6 +2240,7 @@ def argmax(logits, tokens_out) -> None:
 _tree = _branch = None
 
 TREE_MAX_NODES = 256               # drafted nodes of a segment
+TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
 TREE_MIN_SHARE = 4                 # a CTA of split keys walks at least so many tiles
 TREE_MAX_SPLITS = 64
@@ -2252,7 +2253,7 @@ def tree_lib() -> ctypes.CDLL:
     if _tree is None:
         lib = build.load("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE})
         P, I, F = c_void_p, c_int, c_float
-        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, P]
+        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, I, P, P]
         lib.rb_tree_attention.restype = c_int
         _tree = build.native_calls(lib)
     return _tree
@@ -2359,23 +2360,29 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
         raise KernelError("block_table: int32 [segments, blocks]")
     if not (window is None or window >= 0):
         raise KernelError("window: not negative")
-    if not (softcap is None or softcap >= 0):
-        raise KernelError("softcap: not negative")
+    if not (scale > 0 and (softcap is None or softcap >= 0)):
+        raise KernelError("scale: positive; softcap: not negative")
     _same_device(qkv.device, qkv, k_pool, v_pool, block_table, out, batch.cu_q, batch.tree_parent, sink)
     window = int(window or 0)
     lib = tree_lib()
-    key = ("tree.shares", num_heads, num_kv_heads, head_dim, window, qkv.dtype)
+    group = num_heads // num_kv_heads
+    q_at, ld = _ptr(qkv), qkv.stride(0)
+    tiles = 0                                          # the tensor cores take up to two tiles of TREE_TILE_ROWS rows a CTA
+    if qkv.dtype == torch.bfloat16 and head_dim in TC5_ATTENTION_HEAD_DIMS and not ((q_at | _ptr(k_pool) | _ptr(v_pool) | _ptr(out)) & 15 or ld & 7):
+        tiles = 1 if longest * group <= TREE_TILE_ROWS else 2
+    key = ("tree.shares", num_heads, num_kv_heads, head_dim, window, tiles)
     shares = batch.scratch.get(key)
     if shares is None:
-        shares = batch.scratch[key] = tree_shares(nodes, ends, window, num_heads // num_kv_heads, num_kv_heads, rows * num_heads, head_dim,
-                                                  32, 2 if head_dim <= 128 else 1)
+        shares = batch.scratch[key] = tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim,
+                                                  tiles * TREE_TILE_ROWS or 32, 1 if tiles or head_dim > 128 else 2)
     splits, share = shares
     # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
     scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
-    _check(lib.rb_tree_attention(_ptr(qkv), qkv.stride(0), _ptr(k_pool), _ptr(v_pool), _ptr(batch.cu_q), _ptr(batch.seg_pos0),
+    _check(lib.rb_tree_attention(q_at, ld, _ptr(k_pool), _ptr(v_pool), _ptr(batch.cu_q), _ptr(batch.seg_pos0),
                                  _ptr(batch.tree_parent), _ptr(block_table), block_table.stride(0), page_size, _ptr(out),
                                  dtype_code(qkv.dtype), n, longest, T, num_heads, num_kv_heads, head_dim, float(scale), window,
-                                 float(softcap or 0.0), _sink_ptr(sink, num_heads), splits, share, _ptr(scratch), _stream()),
+                                 float(softcap or 0.0), _sink_ptr(sink, num_heads), splits, share, _ptr(scratch), tiles,
+                                 _status_word(qkv.device) if tiles else None, _stream()),
            "tree_attention", 2 if splits > 1 else 1)
 
 

@@ -48,7 +48,7 @@ def test_tree_attention_refuses():
                           (dict(v_pool=good["v_pool"].float()), "one type"), (dict(v_pool=good["v_pool"][:5]), "pools"),
                           (dict(k_pool=good["k_pool"].transpose(1, 2)), "pools"), (dict(out=good["out"].float()), "one type"),
                           (dict(out=torch.zeros((4, 128), dtype=torch.bfloat16)[:, ::2]), "out"),
-                          (dict(block_table=good["block_table"].long()), "block_table"), (dict(window=-1), "window"), (dict(softcap=-1.0), "softcap")):
+                          (dict(block_table=good["block_table"].long()), "block_table"), (dict(window=-1), "window"), (dict(softcap=-1.0), "softcap"), (dict(scale=0.0), "scale")):
         refuse(match, ops.tree_attention, **{**attention_args(), **change})
     bad = attention_args()
     bad["batch"].tree_parent = bad["batch"].tree_parent.long()
