@@ -16,11 +16,14 @@ for other architectures, ``LinearStateCache`` slots of fixed size per resident s
 * Only the last page of a request is partly filled, so a block table is a list of page ids
   indexed by ``position // page_size``; ``-1`` marks a block that the window has passed (and that
   holds no kept first key) and whose page went back to the pool.
+* A request can be **forked** (beams of one prompt): both then hold its full pages, and a page goes back to the pool when the
+  last of them gives it back.  Only a last, partly filled page is ever written, and that one each has for itself.
 * Every request holds one **slot** (0 .. max_requests-1) for its fixed-size state and as its
   row in device-side tables, whether or not the architecture has such state.
 """
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 from typing import Callable, Dict, Hashable, List, Optional, Sequence
 
@@ -54,7 +57,7 @@ class PagePool:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))     # page 0 is handed out first
-        self._held = [False] * num_pages
+        self._held = [0] * num_pages             # by how many block tables
 
     @property
     def num_free(self) -> int:
@@ -66,18 +69,37 @@ class PagePool:
         out = [self._free.pop() for _ in range(n)]
         for p in out:
             assert not self._held[p], f"page {p} handed out twice"
-            self._held[p] = True
+            self._held[p] = 1
         return out
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more block table holds these pages."""
+        for p in pages:
+            assert self._held[p], f"page {p} shared but not held"
+            self._held[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def give_back(self, pages: Sequence[int]) -> None:
         for p in pages:
             if not (0 <= p < self.num_pages) or not self._held[p]:
                 raise AssertionError(f"page {p} freed but not held")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
     def held_pages(self) -> List[int]:
         return [p for p, h in enumerate(self._held) if h]
+
+
+@dataclass
+class Fork:
+    """What the device has to copy for a request that was forked: its slot's states, and in each group the first ``rows`` rows of a
+    partly filled last page, (group, page, new page, rows)."""
+    src_slot: int
+    dst_slot: int
+    pages: List[tuple] = field(default_factory=list)
 
 
 @dataclass
@@ -165,13 +187,14 @@ class CacheManager:
         return [b for b in range(g.kept_blocks, min(self._first_needed_block(g, length), len(blocks))) if blocks[b] >= 0]
 
     def pages_needed(self, rid, n_tokens: int) -> List[int]:
-        """Per group: pages that ``append(rid, n_tokens)`` would take beyond those it gives back."""
+        """Per group: pages that ``append(rid, n_tokens)`` would take beyond those it gives back to the pool (a page that
+        another request holds too does not go back)."""
         st = self._req[rid]
         out = []
-        for g, blocks in zip(self.groups, st.blocks):
+        for g, pool, blocks in zip(self.groups, self.pools, st.blocks):
             end_blocks = (st.length + n_tokens + g.page_size - 1) // g.page_size
             new = max(0, end_blocks - len(blocks))
-            out.append(new - len(self._passed_blocks(g, blocks, st.length)))
+            out.append(new - sum([pool.holders(blocks[b]) == 1 for b in self._passed_blocks(g, blocks, st.length)]))
         return out
 
     def fits(self, rid, n_tokens: int) -> bool:
@@ -212,6 +235,52 @@ class CacheManager:
         st.length += n_tokens
         return old
 
+    def fits_each(self, wants: Sequence[tuple]) -> bool:
+        """``fits_all`` for (request, tokens) pairs that append different numbers of tokens."""
+        total = [0] * len(self.groups)
+        for rid, n_tokens in wants:
+            for g, need in enumerate(self.pages_needed(rid, n_tokens)):
+                total[g] += max(need, 0)
+        return all(need <= pool.num_free for need, pool in zip(total, self.pools))
+
+    # ------------------------------------------------------------------ requests that part ways
+    def fork_all(self, pairs: Sequence[tuple]) -> List[Fork]:
+        """Every (request, new request) of ``pairs``: the new one gets a slot and the other's length and block tables.  Full
+        pages are held by both; of a partly filled last page, which each will go on writing, it gets one of its own.  No hook on
+        ``on_slot_taken`` runs: the caller copies states and pages as the ``Fork`` says, before either request's next step.
+        Raises KVCapacityError and changes nothing if slots or pages do not suffice."""
+        new = [dst for _, dst in pairs]
+        taken = [rid for rid in new if rid in self._req]
+        if taken or len(set(new)) != len(new):
+            raise KeyError(f"requests {taken or new!r} are already live, or named twice")
+        partial = [sum(1 for src, _ in pairs if self._req[src].length % g.page_size) for g in self.groups]
+        short = [(g.name, need, pool.num_free) for g, need, pool in zip(self.groups, partial, self.pools) if need > pool.num_free]
+        if short or len(pairs) > len(self._free_slots):
+            raise KVCapacityError(f"{len(pairs)} forks: {len(self._free_slots)} slots free, pages (group, needed, free) {short}")
+        out = []
+        for src, dst in pairs:
+            st = self._req[src]
+            fork = Fork(st.slot, self._free_slots.pop())
+            blocks: List[List[int]] = []
+            for gi, (g, pool, mine) in enumerate(zip(self.groups, self.pools, st.blocks)):
+                rows = st.length % g.page_size
+                whole = mine[:-1] if rows else list(mine)
+                pool.share([p for p in whole if p >= 0])
+                if rows:
+                    page = pool.take(1)[0]
+                    fork.pages.append((gi, mine[-1], page, rows))
+                    whole = whole + [page]
+                blocks.append(whole)
+            self._req[dst] = _RequestState(slot=fork.dst_slot, length=st.length, blocks=blocks)
+            out.append(fork)
+        return out
+
+    def rename(self, rid, new) -> None:
+        """The request goes on under another name."""
+        if new in self._req:
+            raise KeyError(f"request {new!r} is already live")
+        self._req[new] = self._req.pop(rid)
+
     def truncate(self, rid, length: int) -> None:
         """Takes the last tokens of a request back: its length becomes ``length`` (not more than it is) and the
         pages behind it return to their pools.  What lies in the kept pages beyond ``length`` is overwritten by
@@ -221,6 +290,11 @@ class CacheManager:
             raise ValueError(f"request {rid!r} holds {st.length} tokens; cannot truncate to {length}")
         if length < st.length and not self.truncatable:
             raise ValueError("per-request state depends on the tokens that were run: nothing can be taken back")
+        for g, pool, blocks in zip(self.groups, self.pools, st.blocks):
+            if length < st.length and length % g.page_size:
+                last = blocks[length // g.page_size]
+                if last >= 0 and pool.holders(last) > 1:
+                    raise ValueError(f"request {rid!r} shares the page that its token {length} would be written to")
         for g, pool, blocks in zip(self.groups, self.pools, st.blocks):
             keep = (length + g.page_size - 1) // g.page_size
             gone = [p for p in blocks[keep:] if p >= 0]
@@ -239,7 +313,12 @@ class CacheManager:
             owned: List[int] = []
             for st in self._req.values():
                 owned.extend(p for p in st.blocks[gi] if p >= 0)
-            assert len(owned) == len(set(owned)), f"group {gi}: a page is held by two block tables"
+            for st in self._req.values():
+                mine = [p for p in st.blocks[gi] if p >= 0]
+                assert len(mine) == len(set(mine)), f"group {gi}: a page is twice in one block table"
+            counts = Counter(owned)
+            assert all(pool.holders(p) == k for p, k in counts.items()), f"group {gi}: a page is held by more or fewer block tables than it counts"
+            owned = list(counts)
             assert sorted(owned) == pool.held_pages(), f"group {gi}: held pages and block tables disagree"
             free = list(pool._free)
             assert len(free) == len(set(free)), f"group {gi}: a page is on the free list twice"

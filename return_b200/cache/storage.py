@@ -19,6 +19,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..ext import ops
 from ..parts.base import BuildEnv, CompositeNeed, KVCacheNeed, KVView, LatentCacheNeed, LayerContext, StateNeed
 from .manager import CacheManager, GroupSpec
 
@@ -88,6 +89,7 @@ class CacheStorage:
         self.pools: List[Optional[torch.Tensor]] = []
         self._layer_views: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
         self.states: Dict[Tuple, torch.Tensor] = {}
+        self._slot_table = None              # of the states, for copies from slot to slot
 
     def make_manager(self) -> CacheManager:
         manager = CacheManager(self.group_specs, self.max_reside)
@@ -107,6 +109,7 @@ class CacheStorage:
                 self.pools.append(torch.zeros((layers, spec.num_pages, spec.page_size, d), dtype=dt, device=dev))
                 continue
             self.pools.append(torch.zeros((layers, 2, spec.num_pages, hkv, spec.page_size, d), dtype=dt, device=dev))
+        self._slot_table = None
         self.states = {i: torch.zeros((self.max_reside + 1,) + tuple(n.shape), dtype=n.dtype, device=dev)
                        for i, n in self._state_needs.items()}
 
@@ -126,6 +129,33 @@ class CacheStorage:
         """A request that takes a slot starts from zero state."""
         for t in self.states.values():
             t[slot].zero_()                  # in stream order: after the last step of whoever held the slot before
+
+    def copy_forks(self, forks) -> None:
+        """What ``CacheManager.fork_all`` asks for, in stream order: a launch a group that has partly filled pages, and one for the
+        states.  The forked requests' pages and slots are new, so no destination is a source."""
+        columns: Dict[object, List[Tuple[int, ...]]] = {}
+        for f in forks:
+            if self.states:
+                columns.setdefault("slots", []).append((f.src_slot, f.dst_slot))
+            for g, src, dst, rows in f.pages:
+                if self.pools[g] is not None and src >= 0:
+                    columns.setdefault(g, []).append((src, dst, rows))
+        if not columns:
+            return
+        flat = [v for moves in columns.values() for column in zip(*moves) for v in column]
+        with torch.cuda.device(self.env.device):
+            dev = torch.tensor(flat, dtype=torch.int32).pin_memory().to(self.env.device, non_blocking=True)
+            at = 0
+            for key, moves in columns.items():
+                n, width = len(moves), len(moves[0])
+                args = [dev[at + i * n:at + (i + 1) * n] for i in range(width)]
+                at += n * width
+                if key == "slots":
+                    if self._slot_table is None:
+                        self._slot_table = ops.slot_table(list(self.states.values()))
+                    ops.copy_slots(self._slot_table, *args)
+                else:
+                    ops.copy_pages(self.pools[key], *args)
 
     def layer_context(self, owner_index: int, batch, write: bool) -> LayerContext:
         return self._context((owner_index,), batch, write)

@@ -40,7 +40,7 @@ def _make_engine(args):
     from .engine.engine import Engine
     cfg = EngineConfig(max_token=args.max_token, max_reside=args.max_reside, page_size=args.page_size,
                        prefill_chunk=args.chunk, dtype=args.dtype, use_cuda_graph=args.graph, capture_at_start=args.capture_at_start, seed=args.seed,
-                       device=args.device)
+                       device=args.device, draft_tokens=getattr(args, "draft_tokens", 0))
     return Engine(args.model, cfg)
 
 
@@ -60,6 +60,12 @@ def cmd_generate(args) -> int:
         print("give --prompt-ids or --prompt-len", file=sys.stderr)
         return 2
     stops = [_ids(s) for s in (args.stop_ids or [])]
+    if args.beams:
+        found = engine.beam_search(prompts, beams=args.beams, max_new_tokens=args.new, length_penalty=args.length_penalty,
+                                   eos_token_id=args.eos_token_id)
+        for results in found:
+            print(json.dumps({"beams": [r.as_dict() for r in results]}))
+        return 0
     results = engine.generate(prompts, max_new_tokens=args.new, temperature=args.temperature, top_p=args.top_p,
                               top_k=args.top_k, stop_ids=stops, seed=args.seed, eos_token_id=args.eos_token_id)
     for r in results:
@@ -154,6 +160,9 @@ def main(argv=None) -> int:
     g.add_argument("--top-k", type=int, default=0)
     g.add_argument("--stop-ids", action="append", help="a stop sequence of token ids (repeatable)")
     g.add_argument("--eos-token-id", type=int, default=None, help="a stop sequence of one token")
+    g.add_argument("--draft-tokens", type=int, default=0, help="most tokens drafted for a request beside its next one (0: none)")
+    g.add_argument("--beams", type=int, default=0, help="beam search with so many beams a prompt, in the place of sampling (0: sample)")
+    g.add_argument("--length-penalty", type=float, default=1.0, help="the power of a continuation's length that its score is divided by")
     g.set_defaults(fn=cmd_generate)
 
     r = sub.add_parser("random-weights", help="write a random model folder")

@@ -17,7 +17,8 @@
 // v <- (1 - share) v + share v_first, in float32 before the store.
 //
 // Cache layout of one layer: [num_pages, Hkv, P, D]; the page of a token is
-// block_table[segment][pos / P], its row in the page pos % P.
+// block_table[segment][pos / P], its row in the page pos % P; with `slots` the token goes to slots[t] in the place of pos[t] (the
+// nodes of a drafted tree: several stand at one position, each has a slot of its own).
 #include "common.cuh"
 
 // Two neighbouring elements at a time.
@@ -55,7 +56,7 @@ __global__ void qk_norm_rope_write_kernel(
         TA* __restrict__ qkv, int ld,
         const void* __restrict__ qw, const void* __restrict__ kw, int w_dtype, float eps, float offset,
         const float* __restrict__ cos_t, const float* __restrict__ sin_t, int rot_dim,
-        const int* __restrict__ pos, const int* __restrict__ tok_seg,
+        const int* __restrict__ pos, const int* __restrict__ slots, const int* __restrict__ tok_seg,
         const int* __restrict__ block_table, int bt_stride, int page_size,
         TA* __restrict__ kpool, TA* __restrict__ vpool,
         int Hq, int Hkv, int D, int write_kv, int norm_n, const ValueMix vm) {
@@ -70,8 +71,9 @@ __global__ void qk_norm_rope_write_kernel(
     const int half = rot_dim >> 1;
     long long slot_base = -1;     // element offset of (page, kv head 0, row) in a pool
     if (write_kv && hh0 + HPW > Hq) {
-        const int page = block_table[(size_t)tok_seg[t] * bt_stride + p / page_size];
-        if (page >= 0) slot_base = ((long long)page * Hkv * page_size + (p % page_size)) * D;
+        const int at = slots != nullptr ? slots[t] : p;
+        const int page = block_table[(size_t)tok_seg[t] * bt_stride + at / page_size];
+        if (page >= 0) slot_base = ((long long)page * Hkv * page_size + (at % page_size)) * D;
     }
     TA* row = qkv + (size_t)t * ld;
     // ---- every load first
@@ -217,7 +219,7 @@ qk_norm_rope_write_vec_kernel(
         bf16* __restrict__ qkv, int ld,
         const void* __restrict__ qw, const void* __restrict__ kw, int w_dtype, float eps, float offset,
         const float* __restrict__ cos_t, const float* __restrict__ sin_t, int rot_dim,
-        const int* __restrict__ pos, const int* __restrict__ tok_seg,
+        const int* __restrict__ pos, const int* __restrict__ slots, const int* __restrict__ tok_seg,
         const int* __restrict__ block_table, int bt_stride, int page_size,
         bf16* __restrict__ kpool, bf16* __restrict__ vpool,
         int T, int Hq, int Hkv, int write_kv, int groups_per_token, int norm_n, const ValueMix vm) {
@@ -236,8 +238,9 @@ qk_norm_rope_write_vec_kernel(
     const int p = pos[t];
     long long slot_base = -1;     // element offset of (page, kv head 0, row) in a pool
     if (write_kv && (hg + 1) * HEADS_PER_WARP > Hq) {
-        const int page = block_table[(size_t)tok_seg[t] * bt_stride + p / page_size];
-        if (page >= 0) slot_base = ((long long)page * Hkv * page_size + (p % page_size)) * D;
+        const int at = slots != nullptr ? slots[t] : p;
+        const int page = block_table[(size_t)tok_seg[t] * bt_stride + at / page_size];
+        if (page >= 0) slot_base = ((long long)page * Hkv * page_size + (at % page_size)) * D;
     }
     bf16* row = qkv + (size_t)t * ld;
     uint4 a[ROPE_VEC_ROUNDS], b[ROPE_VEC_ROUNDS];
@@ -330,7 +333,7 @@ qk_norm_rope_write_vec_kernel(
 
 template <int LPH>
 static int launch_rope_vec(void* qkv, int ld, const void* qw, const void* kw, int w_dtype, float eps, float offset,
-                           const float* cos_t, const float* sin_t, int rot_dim, const int* pos, const int* tok_seg,
+                           const float* cos_t, const float* sin_t, int rot_dim, const int* pos, const int* slots, const int* tok_seg,
                            const int* block_table, int bt_stride, int page_size, void* kpool, void* vpool,
                            int T, int Hq, int Hkv, int write_kv, int norm_n, const ValueMix& vm, cudaStream_t st) {
     const int heads = write_kv ? Hq + 2 * Hkv : Hq + Hkv;
@@ -339,7 +342,7 @@ static int launch_rope_vec(void* qkv, int ld, const void* qw, const void* kw, in
     const long long items = (long long)T * groups;
     const dim3 grid((unsigned)((items + 3) / 4));
     return rb_launch_pdl(qk_norm_rope_write_vec_kernel<LPH>, grid, dim3(128), 0, st,
-        (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg, block_table, bt_stride,
+        (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg, block_table, bt_stride,
         page_size, (bf16*)kpool, (bf16*)vpool, T, Hq, Hkv, write_kv, groups, norm_n, vm);
 }
 
@@ -348,7 +351,7 @@ static int launch_rope_vec(void* qkv, int ld, const void* qw, const void* kw, in
 RB_EXPORT int rb_qk_norm_rope_write(
         void* qkv, int ld, const void* qw, const void* kw, int w_dtype, float eps, float offset,
         const float* cos_t, const float* sin_t, int rot_dim,
-        const int* pos, const int* tok_seg, const int* block_table, int bt_stride, int page_size,
+        const int* pos, const int* slots, const int* tok_seg, const int* block_table, int bt_stride, int page_size,
         void* kpool, void* vpool, int act_dtype, int T, int Hq, int Hkv, int D, int write_kv, int norm_n,
         const void* v_first, int v_first_ld, int v_first_head_stride, int v_first_n, const void* v_share, int v_share_dtype,
         cudaStream_t st) {
@@ -369,7 +372,7 @@ RB_EXPORT int rb_qk_norm_rope_write(
     if ((long long)T * heads >= 8192 && act_dtype != RB_F32 && rot_dim % 16 == 0 && aligned) {
         // many tokens of bfloat16: 16-byte pieces
 #define RB_ROPE_VEC(LPH_)                                                                                                       \
-        return launch_rope_vec<LPH_>(qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg, block_table,   \
+        return launch_rope_vec<LPH_>(qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg, block_table,   \
                                      bt_stride, page_size, kpool, vpool, T, Hq, Hkv, write_kv, norm_n, vm, st)
         if (D == 32) RB_ROPE_VEC(2);
         if (D == 64) RB_ROPE_VEC(4);
@@ -382,18 +385,18 @@ RB_EXPORT int rb_qk_norm_rope_write(
         const dim3 grid(T, (heads + 4 * HPW - 1) / (4 * HPW));
         if (act_dtype == RB_F32)
             return rb_launch_pdl(qk_norm_rope_write_kernel<float, HPW>, grid, dim3(threads), 0, st,
-                (float*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg,
+                (float*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg,
                 block_table, bt_stride, page_size, (float*)kpool, (float*)vpool, Hq, Hkv, D, write_kv, norm_n, vm);
         return rb_launch_pdl(qk_norm_rope_write_kernel<bf16, HPW>, grid, dim3(threads), 0, st,
-                (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg,
+                (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg,
                 block_table, bt_stride, page_size, (bf16*)kpool, (bf16*)vpool, Hq, Hkv, D, write_kv, norm_n, vm);
     }
     const dim3 grid(T, (heads + 3) / 4);
     if (act_dtype == RB_F32)
         return rb_launch_pdl(qk_norm_rope_write_kernel<float, 1>, grid, dim3(threads), 0, st,
-            (float*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg,
+            (float*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg,
             block_table, bt_stride, page_size, (float*)kpool, (float*)vpool, Hq, Hkv, D, write_kv, norm_n, vm);
     return rb_launch_pdl(qk_norm_rope_write_kernel<bf16, 1>, grid, dim3(threads), 0, st,
-            (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, tok_seg,
+            (bf16*)qkv, ld, qw, kw, w_dtype, eps, offset, cos_t, sin_t, rot_dim, pos, slots, tok_seg,
             block_table, bt_stride, page_size, (bf16*)kpool, (bf16*)vpool, Hq, Hkv, D, write_kv, norm_n, vm);
 }

@@ -17,7 +17,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..ext import build
+from ..ext import build, ops
 
 
 @dataclass
@@ -26,6 +26,8 @@ class StepEntry:
     tokens: Sequence[int]
     want: Sequence[int] = ()          # indices into ``tokens`` whose logits are wanted
     start: int = -1                   # position of tokens[0]; filled when the cache makes room
+    # tokens that are a drafted tree: the index in ``tokens`` of the token before each, below its own; -1 for tokens[0], the root
+    parents: Optional[Sequence[int]] = None
 
 
 @dataclass
@@ -49,6 +51,20 @@ class HostBatch:
     tiles: Dict[str, np.ndarray] = field(default_factory=dict)
     block_tables: List[np.ndarray] = field(default_factory=list)   # per group [n, blocks]
     rids: List[Hashable] = field(default_factory=list)
+    # a step of drafted trees (None: no such step): each token's parent within its segment, and its slot in the request's pages;
+    # ``pos`` then is the first token's position plus the depth in the tree
+    tree_parent: Optional[np.ndarray] = None     # [T]
+    slots: Optional[np.ndarray] = None           # [T]
+
+
+def tree_depths(parents: Sequence[int]) -> List[int]:
+    """The depth of every node of a tree whose node 0 is the root; raises ValueError for what is no such tree."""
+    depth: List[int] = []
+    for i, p in enumerate(parents):
+        if (p != -1) if i == 0 else not (0 <= p < i):
+            raise ValueError(f"parents of a drafted tree: -1 for the root, an earlier node for every other; got {p} at {i}")
+        depth.append(0 if i == 0 else depth[p] + 1)
+    return depth
 
 
 def build_host_batch(entries: Sequence[StepEntry], manager, vocab_size: Optional[int] = None,
@@ -100,6 +116,20 @@ def build_host_batch(entries: Sequence[StepEntry], manager, vocab_size: Optional
         tok_seg = np.repeat(tok_seg, seg_len)
         pos = np.arange(T, dtype=np.int32) + np.repeat(seg_pos0 - cu_q[:-1], seg_len)
     longest = int(seg_kv_len.max())
+    tree_parent = slots = None
+    if T > n and any(e.parents is not None for e in entries):
+        slots, parents, depths = pos, [], []
+        for i, e in enumerate(entries):
+            line = [-1] if e.parents is None and lens[i] == 1 else e.parents
+            if line is None or len(line) != lens[i]:
+                raise ValueError(f"entry of request {e.rid!r}: a step of drafted trees holds trees, a parent per token, and single tokens")
+            if lens[i] > ops.TREE_MAX_NODES:
+                raise ValueError(f"entry of request {e.rid!r}: a drafted tree of {lens[i]} tokens; at most {ops.TREE_MAX_NODES}")
+            parents += line
+            depths += tree_depths(line)
+        tree_parent = np.array(parents, np.int32)
+        pos = np.array(depths, np.int32) + np.repeat(seg_pos0, seg_len)
+        multi = []                               # no part's blocks of rows: their order is not that of the positions
     if vocab_size is not None and (tokens.min() < 0 or tokens.max() >= vocab_size):
         raise ValueError(f"token ids must lie in [0, {vocab_size})")
     if max_positions is not None and longest > max_positions:
@@ -124,7 +154,7 @@ def build_host_batch(entries: Sequence[StepEntry], manager, vocab_size: Optional
         num_tokens=T, num_segments=n, num_want=len(want_rows), tokens=tokens, pos=pos, tok_seg=tok_seg,
         seg_slot=seg_slot, cu_q=cu_q, seg_pos0=seg_pos0, seg_kv_len=seg_kv_len,
         want_rows=np.asarray(want_rows, np.int32), decode_segs=np.asarray(decode_segs, np.int32),
-        num_multi=len(multi), tiles=tiles, block_tables=tables, rids=rids)
+        num_multi=len(multi), tiles=tiles, block_tables=tables, rids=rids, tree_parent=tree_parent, slots=slots)
 
 
 class StepBatch:
@@ -140,7 +170,9 @@ class StepBatch:
         self.num_want = host.num_want
         self.variant = {}                    # nothing is fixed beforehand: every part works its launches out from the host tables
         tile_names = list(host.tiles)
-        arrays = ([getattr(host, f).reshape(-1) for f in self._FIELDS] + [host.tiles[n].reshape(-1) for n in tile_names]
+        self.tree_parent = self.slots = None
+        fields = self._FIELDS if host.tree_parent is None else self._FIELDS + ("tree_parent", "slots")
+        arrays = ([getattr(host, f).reshape(-1) for f in fields] + [host.tiles[n].reshape(-1) for n in tile_names]
                   + [bt.reshape(-1) for bt in host.block_tables])
         sizes, total = [], 0
         for a in arrays:
@@ -155,9 +187,9 @@ class StepBatch:
         dev.copy_(pinned[:total], non_blocking=True)
         staging.mark()
         views = dev.split_with_sizes(sizes)[::2]
-        for f, v in zip(self._FIELDS, views):
+        for f, v in zip(fields, views):
             setattr(self, f, v)
-        k = len(self._FIELDS)
+        k = len(fields)
         self.tiles = {n: v.view(-1, 2) for n, v in zip(tile_names, views[k:k + len(tile_names)])}
         self.block_tables = [v.view(bt.shape) for v, bt in zip(views[k + len(tile_names):], host.block_tables)]
 

@@ -8,7 +8,9 @@
 ``capture_at_start`` capture them all when the engine is built, as the reference does
 (rollout/model.py:346-407), instead of each on its first use;
 ``keep_sessions`` a request that ends keeps its cache for a follow-up request with the same id, until
-``release`` or until the pages are needed (the reference always keeps, rollout/engine.py:286-306).
+``release`` or until the pages are needed (the reference always keeps, rollout/engine.py:286-306);
+``draft_tokens`` most tokens that are drafted for a request beside its next one while it decodes, as a tree that one step checks
+(engine/draft.py; 0: none; the reference drafts none).  Models with per-request states take none.
 """
 from __future__ import annotations
 
@@ -16,6 +18,8 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+
+from ..ext.ops import TREE_MAX_NODES
 
 
 @dataclass(frozen=True)
@@ -29,6 +33,7 @@ class EngineConfig:
     use_cuda_graph: bool = True
     capture_at_start: bool = False
     keep_sessions: bool = False
+    draft_tokens: int = 0
     seed: int = 0
     device: str = "cuda:0"
 
@@ -39,6 +44,8 @@ class EngineConfig:
             raise ValueError("max_token must hold at least one page")
         if self.max_reside <= 0 or self.prefill_chunk <= 0:
             raise ValueError("max_reside and prefill_chunk must be positive")
+        if not 0 <= self.draft_tokens < TREE_MAX_NODES:
+            raise ValueError(f"draft_tokens: 0 to {TREE_MAX_NODES - 1}")
 
     @property
     def act_dtype(self) -> torch.dtype:

@@ -18,7 +18,9 @@ import torch
 from ..cache.manager import KVCapacityError
 from ..ext import ops
 from ..sampling.sampler import Sampler, uniform_draw
+from .beams import BeamResult, BeamSearch
 from .config import EngineConfig
+from .draft import PromptLookup
 from .request import GenerationResult, Request
 from .runner import ModelRunner
 from .scheduler import Scheduler, StepPlan
@@ -39,12 +41,16 @@ class Engine:
         self.scheduler = Scheduler(self.runner.manager, self.config.prefill_chunk, self.runner.max_positions,
                                    keep_sessions=self.config.keep_sessions)
         self.sampler = Sampler(self.runner.env.device, max(16, self.config.max_reside))
+        self.drafter = PromptLookup(self.config.draft_tokens) if self.config.draft_tokens else None
+        if self.drafter is not None and not self.runner.takes_trees():
+            raise ValueError("draft_tokens: this model keeps per-request state, or has mixers that take no drafted trees")
         if self.config.capture_at_start and self.runner.runs_ahead():
             self.runner.capture_decode_graphs()
         self._t_start = time.perf_counter()
         self._acc_decode = self._acc_prefill = 0.0
         self._dc_tok = self._pf_tok = 0
         self._steps = self._preemptions = 0
+        self._drafted = self._drafts_held = 0
         self._auto_id = 0
 
     # ------------------------------------------------------------------ step-wise interface
@@ -104,12 +110,68 @@ class Engine:
         """Every running request is decoding, none waits for a slot that is free, and decode steps go
         through captured graphs: the next step can then start before the host has read the last
         step's tokens, because its tokens can come straight from the sampler's device buffer."""
+        return self.runner.runs_ahead() and self._only_decodes()
+
+    def _only_decodes(self) -> bool:
         sch = self.scheduler
-        if not sch.running or not self.runner.runs_ahead():
-            return False
-        if sch.waiting and self.runner.manager.free_slots > 0:
+        if not sch.running or (sch.waiting and self.runner.manager.free_slots > 0):
             return False
         return all(r.output and r.num_computed == r.num_tokens - 1 for r in sch.running)
+
+    # ------------------------------------------------------------------ drafted trees
+    def _draft_step(self) -> Optional[List[Request]]:
+        """One step that checks a drafted tree of every running request, all of which decode: a node's logits give the token
+        behind it, drawn as ever from (seed, index of the output token), and the drafted tokens that agree hold.  So the output is that
+        of steps of single tokens, up to the rounding of logits that were computed in another shape of step.  Returns the requests that
+        ended; None where nothing was drafted, or pages or the token budget do not suffice: the ordinary step then runs."""
+        from .batch import StepEntry, tree_depths
+        sch, mgr, runner = self.scheduler, self.runner.manager, self.runner
+        reqs = list(sch.running)
+        budget = sch.prefill_chunk - len(reqs)
+        if budget < 0 or not mgr.fits_all([r.id for r in reqs], 1):
+            return None
+        t0 = time.perf_counter()
+        trees = []
+        for r in reqs:
+            # a node's token is the output token behind it: no deeper than what the request still wants, no slot beyond the limit
+            room = min(budget, r.max_new_tokens - len(r.output) - 1, sch.max_model_len - r.num_tokens)
+            tree = self.drafter.propose(r, room)
+            budget -= len(tree[0]) - 1
+            trees.append(tree)
+        if all(len(tokens) == 1 for tokens, _ in trees) or not mgr.fits_each([(r.id, len(t[0])) for r, t in zip(reqs, trees)]):
+            return None
+        entries, params, first = [], [], [0]
+        for r, (tokens, parents) in zip(reqs, trees):
+            entries.append(StepEntry(r.id, tokens, (), mgr.append(r.id, len(tokens)), parents))
+            depths = tree_depths(parents)
+            draws = [uniform_draw(r.seed, len(r.output) + d) for d in range(max(depths) + 1)]
+            params += [(r.temperature, r.top_k, r.top_p, draws[d]) for d in depths]
+            first.append(first[-1] + len(tokens))
+        logits, batch = runner.step_trees(entries)
+        sampled = self.sampler.launch(logits, params, 0, status=True)
+        path, count, _ = runner.commit_trees(batch, sampled)
+        toks, lps = self.sampler.fetch(0)                     # raises where a kernel's bounded wait gave up
+        paths, counts = path.tolist(), count.tolist()
+        ended: List[Request] = []
+        for i, r in enumerate(reqs):
+            kept = 0
+            for x in paths[i][:counts[i]]:
+                r.num_computed += 1
+                r.push(toks[first[i] + x], lps[first[i] + x])
+                kept += 1
+                if r.finished or r.num_tokens >= sch.max_model_len:
+                    r.finish_reason = r.reason() if r.finished else "length"
+                    ended.append(r)
+                    break
+            mgr.truncate(r.id, r.num_computed)
+            self._dc_tok += kept
+            self._drafts_held += kept - 1
+            self._drafted += len(trees[i][0]) - 1
+        for r in ended:
+            sch.finish(r)
+        self._steps += 1
+        self._acc_decode += time.perf_counter() - t0
+        return ended
 
     def _decode_ahead(self, max_steps: Optional[int] = None) -> List[Request]:
         """Consecutive steps of one decoded token per running request, each launched while the step
@@ -170,7 +232,13 @@ class Engine:
         ended: List[Request] = []
         left = max_steps
         while self.has_unfinished() and (left is None or left > 0):
-            if self._can_run_ahead():
+            if self.drafter is not None and self._only_decodes():
+                got = self._draft_step()
+                if got is not None:
+                    ended += got
+                    left = None if left is None else left - 1
+                    continue
+            elif self._can_run_ahead():
                 before = self._steps
                 ended += self._decode_ahead(left)
                 if left is not None:
@@ -214,6 +282,16 @@ class Engine:
         return [GenerationResult(r.id, list(r.output), list(r.output_logprobs), len(r.output), r.finish_reason)
                 for r in reqs]
 
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_new_tokens: int = 32, length_penalty: float = 1.0,
+                    eos_token_id: Optional[int] = None) -> List[List[BeamResult]]:
+        """For every prompt the ``beams`` continuations of highest score that a beam search finds, best first: the sum of a
+        continuation's log-probabilities over its length to the power ``length_penalty``.  Runs while no request does."""
+        if self.has_unfinished():
+            raise RuntimeError("beam search runs while no request does")
+        while self.scheduler._evict_kept():                   # its pages and slots are the search's
+            pass
+        return BeamSearch(self.runner, beams, max_new_tokens, length_penalty, eos_token_id).run(prompts)
+
     # ------------------------------------------------------------------ counters (rollout/engine.py:84-125,308-315)
     @property
     def run_time(self) -> float:
@@ -236,7 +314,7 @@ class Engine:
             "decode_tps": self.decode_tps, "prefill_tps": self.prefill_tps,
             "decode_duty": self._acc_decode / rt if rt > 0 else 0.0,
             "prefill_duty": self._acc_prefill / rt if rt > 0 else 0.0,
-            "preemptions": self._preemptions, "kept_sessions": len(self.scheduler.kept),
+            "preemptions": self._preemptions, "drafted": self._drafted, "drafts_held": self._drafts_held, "kept_sessions": len(self.scheduler.kept),
             # the pages of every group of layers (a model with full and window layers has two pools)
             "page_used": sum(m.pages_used()), "page_total": sum(g.num_pages for g in m.groups),
             "page_groups": [{"name": g.name, "used": u, "total": g.num_pages, "window": g.window}

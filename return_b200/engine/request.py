@@ -34,6 +34,7 @@ class Request:
     # scheduler state
     num_computed: int = 0                        # tokens of prompt + output whose keys are cached
     num_preemptions: int = 0
+    draft_state: Optional[dict] = field(default=None, repr=False, compare=False)      # what engine/draft.py keeps per request
     arrival: int = 0
 
     def push(self, tok: int, logprob: float = 0.0) -> None:

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 from typing import Hashable, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ..cache.manager import CacheManager, KVCapacityError
@@ -114,6 +115,44 @@ class ModelRunner:
         start = self.manager.append(rid, n)
         return StepEntry(rid=rid, tokens=tokens, want=want, start=start)
 
+    def fork_requests(self, pairs: Sequence[tuple]) -> None:
+        """Every (request, new request) of ``pairs``: the new one starts as a copy of the other.  Full pages are shared, the
+        rows of a partly filled last page and per-request states are copied.  Raises KVCapacityError, changing nothing, if slots or
+        pages do not suffice."""
+        self.storage.copy_forks(self.manager.fork_all(pairs))
+
+    # ------------------------------------------------------------------ drafted trees
+    def takes_trees(self) -> bool:
+        """Whether a step may bring drafted trees: the model's parts take them, and a request's length can be taken back."""
+        return bool(self.model.tree_safe and self.manager.truncatable)
+
+    @torch.no_grad()
+    def step_trees(self, entries: Sequence[StepEntry]):
+        """Runs entries that bring drafted trees (``StepEntry.parents``) as one step; returns (float32 logits [all their tokens,
+        vocab], what ``commit_trees`` wants).  Nothing is taken back here: each request is as long as its whole tree."""
+        if not self.takes_trees():
+            raise ValueError("this model keeps per-request state, or has mixers that take no drafted trees")
+        entries = [StepEntry(e.rid, e.tokens, range(len(e.tokens)), e.start, e.parents) for e in entries]
+        host = build_host_batch(entries, self.manager, self.vocab_size, self.max_positions, self.tilings)
+        if host.tree_parent is None:             # single tokens alone, or no tree at all
+            raise ValueError("step_trees runs steps that bring a tree of several tokens")
+        with torch.cuda.device(self.env.device):
+            batch = StepBatch(host, self.env.device, self.staging)
+            return self.model.forward(batch, self.storage), batch
+
+    @torch.no_grad()
+    def commit_trees(self, batch: StepBatch, sampled: torch.Tensor):
+        """After ``step_trees``: ``sampled`` (int32 [tokens of the step], on the device) follows each token.  The cached rows of the
+        nodes that hold move up behind each request's root, in stream order.  Returns device tensors (path, count, emitted) as
+        ``ops.tree_commit`` fills them; whoever asked then takes the requests back to their lengths (``manager.truncate``)."""
+        n, width = batch.num_segments, int(np.diff(batch.host.cu_q).max())
+        with torch.cuda.device(self.env.device):
+            path, emitted = (torch.empty((n, width), dtype=torch.int32, device=self.env.device) for _ in range(2))
+            count = torch.empty((n,), dtype=torch.int32, device=self.env.device)
+            caches = [(pool, table) for pool, table in zip(self.storage.pools, batch.block_tables) if pool is not None]
+            ops.tree_commit(sampled, batch, caches, path, count, emitted)
+        return path, count, emitted
+
     # ------------------------------------------------------------------ the step
     @torch.no_grad()
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -124,6 +163,8 @@ class ModelRunner:
         how a step starts before the host has seen the tokens the step before it sampled."""
         host = build_host_batch(entries, self.manager, self.vocab_size, self.max_positions, self.tilings)
         with torch.cuda.device(self.env.device):
+            if host.tree_parent is not None:
+                raise ValueError("drafted trees are run by step_trees")
             if self.config.use_cuda_graph and host.num_tokens == host.num_segments and self.model.graph_safe:
                 return self._graphed_decode(host, device_tokens)
             if device_tokens is not None:

@@ -101,7 +101,7 @@ def core() -> ctypes.CDLL:
         lib.rb_gemm_skinny_fused.restype = c_int
         lib.rb_gemm_skinny_ctas.argtypes = [I]
         lib.rb_gemm_skinny_ctas.restype = c_int
-        lib.rb_qk_norm_rope_write.argtypes = [P, I, P, P, I, F, F, P, P, I, P, P, P, I, I, P, P, I, I, I, I, I, I, I, P, I, I, I, P, I, P]
+        lib.rb_qk_norm_rope_write.argtypes = [P, I, P, P, I, F, F, P, P, I, P, P, P, P, I, I, P, P, I, I, I, I, I, I, I, P, I, I, I, P, I, P]
         lib.rb_attention_simt.argtypes = [P, I, P, P, P, P, P, I, I, P, I, I, I, I, I, F, I, P]
         lib.rb_attention_simt_mod.argtypes = [P, I, P, P, P, P, P, I, I, P, I, I, I, I, I, F, I, I, F, P, P, P, I, I, P]
         lib.rb_attn_prep.argtypes = [P, I, I, I, I, P, P, P, I, P, P, I, F, P, P, I, P, P, P, I, I, P, P, P, I, I, I, I, I, I, I, I, P]
@@ -847,14 +847,16 @@ def linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, act: Optional[st
 
 def qk_norm_rope_write(qkv, q_weight, k_weight, eps, cos, sin, rot_dim, pos, tok_seg, block_table,
                        page_size, k_pool, v_pool, num_heads, num_kv_heads, head_dim, write_kv=True,
-                       offset=0.0, norm_size=None, blend=None) -> None:
+                       offset=0.0, norm_size=None, blend=None, slots=None) -> None:
     """In place on qkv [T, (Hq+2Hkv)*D]: q heads normed and rotated; k heads normed, rotated and
     written to ``k_pool``; v heads written to ``v_pool``.  Pools: [pages, Hkv, P, D].  ``norm_size``: the elements of a
     head that the norm's mean runs over, where heads are padded with zeros (None: all).  ``blend`` = (first, head_stride, n,
     share): what is cached of a value v is (1 - share) v + share first, ``first`` [T, ...] the values of an earlier layer
-    (kv head g from column g * head_stride, n of them; what lies behind is zero in both), ``share`` one number."""
+    (kv head g from column g * head_stride, n of them; what lies behind is zero in both), ``share`` one number.  ``slots``
+    (int32 [T]): where keys and values go in a request's pages, in the place of ``pos`` (the nodes of a drafted tree)."""
     T = qkv.shape[0]
     assert qkv.stride(1) == 1
+    assert slots is None or (slots.dtype == torch.int32 and slots.numel() == T and slots.is_contiguous())
     assert pos.dtype == tok_seg.dtype == block_table.dtype == torch.int32
     assert k_pool.dtype == qkv.dtype and v_pool.dtype == qkv.dtype
     if rot_dim:
@@ -868,7 +870,7 @@ def qk_norm_rope_write(qkv, q_weight, k_weight, eps, cos, sin, rot_dim, pos, tok
         assert k_weight is not None and k_weight.dtype == q_weight.dtype
     _check(core().rb_qk_norm_rope_write(
         _ptr(qkv), qkv.stride(0), _ptr(q_weight), _ptr(k_weight), wd, eps, offset, _ptr(cos), _ptr(sin),
-        rot_dim, _ptr(pos), _ptr(tok_seg), _ptr(block_table), block_table.stride(0), page_size,
+        rot_dim, _ptr(pos), _ptr(slots), _ptr(tok_seg), _ptr(block_table), block_table.stride(0), page_size,
         _ptr(k_pool), _ptr(v_pool), dtype_code(qkv.dtype), T, num_heads, num_kv_heads, head_dim,
         1 if write_kv else 0, int(norm_size or 0), *_blend_args(blend, qkv), _stream()), "qk_norm_rope_write")
 

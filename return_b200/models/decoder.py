@@ -77,6 +77,11 @@ class DecoderModel:
             self._graph_safe = all(b.graph_safe for b in self.blocks) and self.final_norm.graph_safe
         return self._graph_safe
 
+    @property
+    def tree_safe(self) -> bool:
+        """Whether a step may bring drafted trees: every mixer takes them, and nothing looks at the token before."""
+        return self.spec.embedding_pairs is None and all(b.tree_safe for b in self.blocks)
+
     def batch_tilings(self):
         """Every table of query-row blocks that some part of the model reads (``Part.batch_tilings``)."""
         out = {}

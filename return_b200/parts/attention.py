@@ -41,6 +41,7 @@ class PagedAttention(Mixer):
         self.q_size = spec.num_heads * spec.head_dim
         self.kv_size = spec.num_kv_heads * spec.head_dim
         self._sink = None
+        self.tree_safe = not spec.keep_first      # the kernels for drafted trees know a window, not first keys kept beside it
 
     # ------------------------------------------------------------------ parameters and cache
     def params(self):
@@ -126,7 +127,8 @@ class PagedAttention(Mixer):
         offset = s.qk_norm.offset if s.qk_norm is not None else 0.0
         tables = self.position.rotary_tables() if self.position is not None else None
         o = ctx.buffer("attention.o", (T, self.q_size), qkv.dtype, qkv.device)
-        if (tables is not None or self.position is None) and ops.decode_only(b, qkv.dtype, s.num_heads, s.num_kv_heads, seen):
+        slots = getattr(b, "slots", None)          # of a step of drafted trees: several nodes stand at one position
+        if slots is None and (tables is not None or self.position is None) and ops.decode_only(b, qkv.dtype, s.num_heads, s.num_kv_heads, seen):
             # single decoded tokens only: norm, rotation, cache write and attention are one kernel
             cos, sin, rot = tables if tables is not None else (None, None, 0)
             ops.attention_decode_fused(qkv, qw, kw, eps, offset, cos, sin, rot, kv.k, kv.v, b, kv.block_table,
@@ -138,7 +140,7 @@ class PagedAttention(Mixer):
             cos, sin, rot = tables if tables is not None else (None, None, 0)
             ops.qk_norm_rope_write(qkv, qw, kw, eps, cos, sin, rot, b.pos, b.tok_seg, kv.block_table,
                                    kv.page_size, kv.k, kv.v, s.num_heads, s.num_kv_heads, s.head_dim,
-                                   write_kv=ctx.write_cache, offset=offset, norm_size=norm_size, blend=blend)
+                                   write_kv=ctx.write_cache, offset=offset, norm_size=norm_size, blend=blend, slots=slots)
         else:
             # an encoding that is not a rotation of pairs: norm, then the encoding's own in-place
             # step on q and k, then the cache write
@@ -149,7 +151,11 @@ class PagedAttention(Mixer):
             if ctx.write_cache:
                 ops.qk_norm_rope_write(qkv, None, None, 0.0, None, None, 0, b.pos, b.tok_seg, kv.block_table,
                                        kv.page_size, kv.k, kv.v, s.num_heads, s.num_kv_heads, s.head_dim,
-                                       write_kv=True, blend=blend)
+                                       write_kv=True, blend=blend, slots=slots)
+        if slots is not None:
+            ops.tree_attention(qkv, kv.k, kv.v, b, kv.block_table, kv.page_size, o, s.num_heads, s.num_kv_heads, s.head_dim,
+                               s.scale, s.window, self._sink, s.softcap)
+            return o
         ops.paged_attention(qkv, kv.k, kv.v, b, kv.block_table, kv.page_size, o, s.num_heads,
                             s.num_kv_heads, s.head_dim, s.scale, s.window, self._sink, None, s.softcap, keep=s.keep_first)
         return o

@@ -173,6 +173,8 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    tree_safe = False
+
     def cache_need(self):
         return None
 
@@ -191,6 +193,11 @@ class FeedForward(Part):
 
 
 class Block(Part):
+    @property
+    def tree_safe(self):
+        mixer = getattr(self, "mixer", None)
+        return mixer is not None and mixer.tree_safe
+
     def cache_need(self):
         return None
 

@@ -119,3 +119,127 @@ def test_tree_shares_cover_the_keys(monkeypatch):
         assert share >= ops.TREE_MIN_SHARE and splits * share >= max(tiles) > (splits - 1) * share
         blocks = sum(-(-k * 4 // 128) * 8 * -(-t // share) for k, t in zip(nodes, tiles))
         assert blocks <= 148
+
+
+# ---------------------------------------------------------------------------------------- drafted trees on the host
+
+def test_batch_of_drafted_trees():
+    from return_b200.cache.manager import CacheManager, GroupSpec
+    from return_b200.engine.batch import StepEntry, build_host_batch
+    from return_b200.parts.base import Tiling
+    m = CacheManager([GroupSpec("full", 4, 20)], max_requests=3)
+    for rid, cached in (("a", 5), ("b", 2)):
+        m.add(rid)
+        m.append(rid, cached)
+    entries = [StepEntry("a", [7, 8, 9, 8], [0, 3], m.append("a", 4), [-1, 0, 0, 2]), StepEntry("b", [6], [0], m.append("b", 1))]
+    b = build_host_batch(entries, m, 100, 50, {"x": Tiling(2)})
+    assert b.tree_parent.tolist() == [-1, 0, 0, 2, -1] and b.slots.tolist() == [5, 6, 7, 8, 2]
+    assert b.pos.tolist() == [5, 6, 6, 7, 2] and b.tiles["x"].shape == (0, 2) and b.num_multi == 0
+    assert b.seg_pos0.tolist() == [5, 2] and b.seg_kv_len.tolist() == [9, 3] and b.want_rows.tolist() == [0, 3, 4]
+    for parents in ([-1, 0, 3, 0], [0, 0, 0, 0], [-1, 0, -1, 0], [-1, 1, 0, 0], [-1, 0, 0], None):
+        entries[0].parents = parents
+        if parents is None:             # a prompt's portion is no tree, and no tree step has one
+            entries[1].parents = [-1]
+        with pytest.raises(ValueError, match="parent"):
+            build_host_batch(entries, m)
+    entries[0].parents = entries[1].parents = None
+    plain = build_host_batch(entries, m)
+    assert plain.tree_parent is None and plain.slots is None and plain.pos.tolist() == [5, 6, 7, 8, 2]
+    alone = [StepEntry("b", [1], [0], m.append("b", 1), [-1])]
+    assert build_host_batch(alone, m).tree_parent is None                       # single tokens: an ordinary decode step
+
+
+def test_forked_requests_share_full_pages():
+    from return_b200.cache.manager import CacheManager, GroupSpec, KVCapacityError
+    m = CacheManager([GroupSpec("full", 4, 9), GroupSpec("win", 4, 12, window=6)], max_requests=4)
+    m.add("a")
+    m.append("a", 10)
+    m.append("a", 1)
+    fork = m.fork_all([("a", "b"), ("a", "c")])
+    m.check()
+    full = m.block_table("a", 0)
+    assert m.length("b") == m.length("c") == 11 and m.block_table("b", 0)[:2] == full[:2] and m.block_table("b", 0)[2] != full[2]
+    assert fork[0].src_slot == m.slot("a") and fork[0].dst_slot == m.slot("b") != m.slot("c")
+    assert [x[::3] for x in fork[1].pages] == [(0, 3), (1, 3)] and fork[1].pages[0][1:3] == (full[2], m.block_table("c", 0)[2])
+    assert m.block_table("b", 1)[0] == m.block_table("a", 1)[0] == -1           # what the window has passed
+    assert m.pages_used()[0] == 5 and m.pools[0].holders(full[0]) == 3
+    for rid in "abc":
+        m.append(rid, 5)
+        m.check()
+    assert m.pages_used()[0] == 8
+    with pytest.raises(KVCapacityError):                                        # three copies, one free page
+        m.append("a", 1), m.append("b", 1)
+        m.fork_all([("a", "d")])
+    m.check()
+    m.free("a")
+    m.check()
+    assert m.pools[0].holders(full[0]) == 2
+    m.free("b"), m.free("c")
+    assert m.pages_used() == [0, 0]
+    m.check()
+
+
+def test_forks_refuse():
+    from return_b200.cache.manager import CacheManager, GroupSpec, KVCapacityError
+    m = CacheManager([GroupSpec("full", 4, 4)], max_requests=3)
+    m.add("a")
+    m.append("a", 9)
+    before = (m.pages_used(), m.free_slots)
+    for pairs, error in (([("a", "a")], KeyError), ([("a", "b"), ("a", "b")], KeyError), ([("x", "b")], KeyError),
+                         ([("a", "b"), ("a", "c")], KVCapacityError), ([("a", "b")] * 0 + [("a", "b"), ("a", "c"), ("a", "d")], KVCapacityError)):
+        with pytest.raises(error):
+            m.fork_all(pairs)
+        assert (m.pages_used(), m.free_slots) == before
+        m.check()
+    m.fork_all([("a", "b")])
+    m.truncate("a", 8)
+    with pytest.raises(ValueError, match="shares the page"):                    # position 6 lies in a page that b holds too
+        m.truncate("a", 6)
+    m.free("b")
+    m.truncate("a", 6)
+    m.check()
+
+
+def test_pages_that_another_holds_do_not_come_back():
+    from return_b200.cache.manager import CacheManager, GroupSpec
+    m = CacheManager([GroupSpec("win", 4, 6, window=4)], max_requests=2)
+    m.add("a")
+    m.append("a", 8)
+    m.fork_all([("a", "b")])
+    m.append("a", 4)                                                            # passes block 0, which b still holds
+    assert m.pages_needed("b", 4) == [0] and m.pools[0].num_free == 3
+    m.append("b", 4)
+    m.check()
+    assert m.pools[0].num_free == 3
+
+
+def test_prompt_lookup():
+    from return_b200.engine.draft import PromptLookup
+    from return_b200.engine.request import Request
+    d = PromptLookup(6, longest=3, shortest=2, places=2)
+    r = Request("x", [1, 2, 3, 4, 9, 1, 2, 3, 5, 9, 7, 1, 2, 3])
+    tokens, parents = d.propose(r, 100)
+    assert tokens[0] == 3 and parents[0] == -1 and len(tokens) <= 7
+    # the latest place first: 5 9 7 ..., then 4 9 1 ... as a second branch where there is room
+    assert tokens[1:4] == [5, 9, 7] and parents[1:4] == [0, 1, 2]
+    wide = PromptLookup(9, longest=3, shortest=2, places=2).propose(Request("y", r.prompt_ids), 3)
+    assert wide == ([3, 5, 9, 7], [-1, 0, 1, 2])
+    tokens, parents = PromptLookup(20, longest=3, shortest=2, places=2).propose(Request("z", r.prompt_ids), 100)
+    branch = [t for t, p in zip(tokens, parents) if p == 0]
+    assert branch == [5, 4] and len(set(zip(parents, tokens))) == len(tokens)
+    r.push(4)
+    assert d.propose(r, 100)[0][:3] == [4, 9, 1]                                # 2 3 4 stood once before: 9 1 2 ...
+    r.push(77)
+    assert d.propose(r, 100) == ([77], [-1]) and d.propose(r, 0) == ([77], [-1])
+    assert PromptLookup(4).propose(Request("w", [5]), 9) == ([5], [-1])
+    again = Request("v", list(r.prompt_ids) + r.output)
+    assert d.propose(again, 5) == d.propose(r, 5)
+    with pytest.raises(ValueError):
+        PromptLookup(4, longest=1, shortest=2)
+
+
+def test_draft_settings_refuse():
+    from return_b200.engine.config import EngineConfig
+    for bad in (-1, ops.TREE_MAX_NODES):
+        with pytest.raises(ValueError, match="draft_tokens"):
+            EngineConfig(draft_tokens=bad)
