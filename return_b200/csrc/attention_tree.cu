@@ -17,6 +17,7 @@
 // output, maximum and sum in float32, and tree_merge_kernel joins them in the order of the shares.  So the result depends
 // on `share`, which the host works out from the step's lengths, and on nothing else of the launch.
 #include "tc5.cuh"
+#include "tma.cuh"
 
 #define TREE_MAX_NODES 256
 #define TREE_WORDS (TREE_MAX_NODES / 32)
@@ -262,15 +263,20 @@ tree_simt_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool,
 }
 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
-// bfloat16, head sizes 64 and 128.  A CTA (one an SM) owns NQ tiles of 128 rows of one segment and key/value head and walks its share of
-// the keys in tiles of 64.  Per key tile and query tile:
-//   S = Q K^T     tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a query tile;
-//   softmax       a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into shared memory.  The reference maximum moves only
-//                 when the true one has outrun it by 2^8, so O is rescaled in tensor memory a few times at most;
-//   O += P V      tcgen05.mma, M = 128, N = head size, V as it lies in the cache.
-// Warps: 4 NQ of rows (those without rows have nothing to do, and nobody waits for them), one that issues S and one that issues P V for
-// each query tile (an issuing thread pays some 230 cycles a wait and 60 to 90 an instruction, so two threads share that), one that
-// gathers K and one that gathers V page by page with cp.async into the 128-byte swizzle, through rings of STAGES tiles.
+// bfloat16, head sizes 64 and 128.  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
+// tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
+//   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn, each with a maximum, sum and output of its own,
+//                  joined at the end;
+//   else           up to 256 rows: a query tile of 128 rows a group, both go through every key tile.
+// Per key tile and group:
+//   S = Q K^T      tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a group;
+//   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into shared memory.  The reference maximum moves only
+//                  when the true one has outrun it by 2^8, so O is rescaled in tensor memory a few times at most;
+//   O += P V       tcgen05.mma, M = 128, N = head size, V as it lies in the cache.
+// Warps: 8 of rows (those without rows have nothing to do, and nobody waits for them), for each group one that issues S and one that issues
+// P V (an issuing thread pays some 230 cycles a wait and 60 to 90 an instruction, so two threads share that), one that gathers K and one
+// that gathers V into the 128-byte swizzle, through rings of STAGES tiles: page by page with TMA where pages are 8, 16, 32 or a multiple of 64
+// rows, else row by row with cp.async.
 // Barriers: each ring stage has a full and an empty one; S, P and P V have one for each of two buffers.  A barrier's next phase always needs
 // all of its waiters to have passed the current one, so no parity wait can fall two phases behind.
 // A key tile that some row does not see in full is looked through for values that are no numbers before the products take it: they are
@@ -281,20 +287,21 @@ constexpr int QM = 128;                       // rows of a query tile
 constexpr int KN = KEY_TILE;
 constexpr float RESCALE_STEP = 8.0f;          // log2 units the true maximum may run ahead of the reference
 
-template <int D, int NQ> struct Shape {
+template <int D, bool STREAMS> struct Shape {
+    static constexpr int NQ = STREAMS ? 1 : 2;               // query tiles
     static constexpr int DS = D / 64;         // 64-wide slabs of the head size
     static constexpr unsigned Q_BYTES = DS * QM * 128, K_BYTES = DS * KN * 128, P_BYTES = QM * 128;
-    static constexpr int STAGES = D == 128 ? (NQ == 1 ? 5 : 3) : (NQ == 1 ? 8 : 6);
-    static constexpr int LAG = STAGES >= 5 ? 2 : 1;           // a tile is announced when this many later ones have been asked for
-    static constexpr int THREADS = 32 * (6 * NQ + 2);
-    static constexpr unsigned TMEM_COLS = NQ == 1 ? 256 : 512;
-    static constexpr unsigned O_COL = NQ * 2 * KN;
-    static constexpr int B_K_FULL = 0, B_V_FULL = STAGES, B_K_EMPTY = 2 * STAGES, B_V_EMPTY = 3 * STAGES, B_S = 4 * STAGES, B_P = B_S + 2 * NQ,
-                         B_PV = B_P + 2 * NQ, B_Q = B_PV + 2 * NQ, N_BARS = B_Q + NQ;
+    static constexpr int STAGES = D == 128 ? (STREAMS ? 4 : 3) : (STREAMS ? 8 : 6);
+    static constexpr int LAG = STAGES >= 4 ? 2 : 1;           // a tile is announced when this many later ones have been asked for
+    static constexpr int THREADS = 32 * 14;
+    static constexpr unsigned TMEM_COLS = 512, O_COL = 4 * KN;
+    static constexpr int B_K_FULL = 0, B_V_FULL = STAGES, B_K_EMPTY = 2 * STAGES, B_V_EMPTY = 3 * STAGES, B_S = 4 * STAGES, B_P = B_S + 4,
+                         B_PV = B_P + 4, B_Q = B_PV + 4, B_V_LAND = B_Q + 2, N_BARS = B_V_LAND + STAGES;
     static constexpr unsigned TAIL = N_BARS * 8 + 16 + TREE_MAX_NODES * 4;
-    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 2 * NQ * P_BYTES + TAIL;
-    static constexpr unsigned SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;       // one CTA an SM: it takes half or all of the tensor memory
-    static_assert(SMEM <= 227 * 1024 && O_COL + NQ * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
+    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 4 * P_BYTES + TAIL;
+    static constexpr unsigned SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;       // one CTA an SM: it takes all of the tensor memory
+    static_assert(SMEM <= 227 * 1024 && O_COL + 2 * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
+    static_assert(!STREAMS || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -349,15 +356,16 @@ struct Paging {
 };
 
 // grid: (row blocks x kv heads, segments, splits).
-template <int D, int NQ>
-__global__ void __launch_bounds__(Shape<D, NQ>::THREADS, 1)
+template <int D, bool STREAMS>
+__global__ void __launch_bounds__(Shape<D, STREAMS>::THREADS, 1)
 tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpool, const bf16* __restrict__ vpool,
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
                 const int* __restrict__ block_table, int bt_stride, int page_size, bf16* __restrict__ out,
                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, float scale, int window,
-                float softcap, const float* __restrict__ sink, int share, int* __restrict__ status) {
-    typedef Shape<D, NQ> S;
-    constexpr int STAGES = S::STAGES;
+                float softcap, const float* __restrict__ sink, int share, int* __restrict__ status, int by_tma,
+                const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    typedef Shape<D, STREAMS> S;
+    constexpr int STAGES = S::STAGES, NQ = S::NQ;
     // The swizzled tiles need 1024-byte alignment: the kernel has no static shared memory, so its window starts at the CTA's base.
     extern __shared__ __align__(1024) unsigned char tc5_smem[];
     if ((smem_u32(tc5_smem) & 1023u) != 0u) {
@@ -367,8 +375,8 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     unsigned char* sQ = tc5_smem;                             // [query tile]
     unsigned char* sK = sQ + NQ * S::Q_BYTES;                 // [stage]
     unsigned char* sV = sK + STAGES * S::K_BYTES;             // [stage]
-    unsigned char* sP = sV + STAGES * S::K_BYTES;             // [query tile][buffer]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sP + 2 * NQ * S::P_BYTES);
+    unsigned char* sP = sV + STAGES * S::K_BYTES;             // [group][buffer]
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sP + 4 * S::P_BYTES);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + S::N_BARS);
     volatile int* odd_values = reinterpret_cast<int*>(tmem_slot + 1);
     int* parent = reinterpret_cast<int*>(tmem_slot + 4);
@@ -379,24 +387,26 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const Segment sg(cu_q, seg_pos0, seg, window, share, gridDim.z);
     const int rows = min(NQ * QM, sg.n * G - row0);
     if (rows <= 0 || split >= sg.n_split) return;
-    const int nq = rows > QM ? 2 : 1;                         // query tiles that have rows
     const int t0 = share > 0 ? split * share : 0, t1 = share > 0 && split + 1 < sg.n_split ? t0 + share : sg.tiles;
     const int jt_begin = sg.jt0 + t0, n_tiles = t1 - t0;      // one tile at least
     const int* bt_row = block_table + (size_t)seg * bt_stride;
     const Paging pg(page_size);
     const unsigned bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
-    auto active_warps = [&](int qt) { return min(4, (rows - qt * QM + 31) >> 5); };
+    // a group's rows (as warps), its key tiles, and the number of its i-th among the CTA's
+    auto active_warps = [&](int g) { return max(0, min(4, (rows - (STREAMS ? 0 : g * QM) + 31) >> 5)); };
+    auto tiles_of = [&](int g) { return STREAMS ? (n_tiles - g + 1) >> 1 : active_warps(g) > 0 ? n_tiles : 0; };
+    auto tile_no = [&](int g, int i) { return STREAMS ? 2 * i + g : i; };
     // whether every row sees every key of a tile
     auto whole = [&](int j_base) { return j_base + KN - 1 < sg.c && (window <= 0 || j_base > sg.c + sg.n - 1 - window); };
 
-    if (warp == 4 * NQ) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
+    if (warp == 8) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
     if (tid == 0) {
         for (int i = 0; i < S::N_BARS; ++i) {
             int count = 1;
-            if (i >= S::B_K_EMPTY && i < S::B_S) count = nq;
+            if (i >= S::B_K_EMPTY && i < S::B_S) count = !STREAMS && rows > QM ? 2 : 1;       // the groups that read a key tile
             else if (i >= S::B_P && i < S::B_PV) count = max(1, active_warps((i - S::B_P) >> 1));
-            else if (i >= S::B_Q) count = max(1, active_warps(i - S::B_Q));
+            else if (i >= S::B_Q && i < S::B_V_LAND) count = max(1, active_warps(i - S::B_Q));
             mbar_init(bar(i), count);
         }
         mbar_init_fence();
@@ -411,9 +421,10 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 
     constexpr int LPR = D / 8, RPI = 32 / LPR;                // lanes a row of 16-byte pieces, rows an instruction
     const int rsel = lane / LPR, sub = lane % LPR;
-    const int qt = warp < 4 * NQ ? warp >> 2 : (warp - 4 * NQ) >> 1;           // query tile of a row warp or an issuer
-    const bool has_rows = warp < 4 * NQ && (warp & 3) < active_warps(qt);
-    const int row = row0 + qt * QM + (warp & 3) * 32 + lane;  // a row thread's row of the segment and head
+    const int grp = warp < 8 ? warp >> 2 : ((warp - 8) >> 1) & 1;              // group of a row warp or an issuer
+    const int qt = STREAMS ? 0 : grp, n_mine = tiles_of(grp);
+    const bool has_rows = warp < 8 && (warp & 3) < active_warps(grp);
+    const int r = (warp & 3) * 32 + lane, row = row0 + qt * QM + r;            // a row thread's row of the tile, of the segment and head
     const bool row_valid = has_rows && row - row0 < rows;
     const size_t token = (size_t)sg.q_begin + (row_valid ? row / G : 0);
     const int h = kvh * G + (row_valid ? row % G : 0);
@@ -428,51 +439,56 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         return (below(sg.c - j_base) & ~below(lo_r - j_base)) | nodes;
     };
     const unsigned lane_addr = tmem + ((unsigned)((warp & 3) * 32) << 16);
-    const unsigned o_addr = lane_addr + S::O_COL + qt * D;
+    const unsigned o_addr = lane_addr + S::O_COL + grp * D;
+    // a row's maximum and sum of a group, in that group's P, which none of its products reads any more by then
+    auto joined = [&](int g) { return reinterpret_cast<float2*>(sP + g * 2 * S::P_BYTES) + r; };
 
     if (has_rows) {
         // ================================================================== one row per thread
-        unsigned char* tile = sQ + qt * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
+        if (!STREAMS || grp == 0) {
+            unsigned char* tile = sQ + qt * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
 #pragma unroll 1
-        for (int i = 0; i < 32 / RPI; ++i) {                  // a row's pieces by neighbouring lanes
-            const int r = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + qt * QM + r;
-            const bool there = rr - row0 < rows;
-            const bf16* src = q + (there ? (size_t)(sg.q_begin + rr / G) * ld + (size_t)(kvh * G + rr % G) * D + sub * 8 : 0);
-            cp16u(smem_u32(tile + sw128_offset(r, sub & 7)), src, there);
+            for (int i = 0; i < 32 / RPI; ++i) {              // a row's pieces by neighbouring lanes
+                const int rt = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + qt * QM + rt;
+                const bool there = rr - row0 < rows;
+                const bf16* src = q + (there ? (size_t)(sg.q_begin + rr / G) * ld + (size_t)(kvh * G + rr % G) * D + sub * 8 : 0);
+                cp16u(smem_u32(tile + sw128_offset(rt, sub & 7)), src, there);
+            }
+            asm volatile("cp.async.commit_group;\n" ::);
         }
-        asm volatile("cp.async.commit_group;\n" ::);
         const int depth = tree_line(parent, row_valid ? row / G : 0, window, line);
         lo_r = window > 0 ? max(0, sg.c + depth - window + 1) : 0;
-        cp_wait<0>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
-        unsigned char* myPs = sP + qt * 2 * S::P_BYTES;
-        const int r = (warp & 3) * 32 + lane;
-        for (int t = 0; t < n_tiles; ++t) {
-            const int j_base = (jt_begin + t) * KN;
-            ok = mbar_wait(bar(S::B_S + qt * 2 + (t & 1)), (t >> 1) & 1) && ok;
+        if (!STREAMS || grp == 0) {
+            cp_wait<0>();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
+        }
+        unsigned char* myPs = sP + grp * 2 * S::P_BYTES;
+        for (int i = 0; i < n_mine; ++i) {
+            const int j_base = (jt_begin + tile_no(grp, i)) * KN, buf = i & 1;
+            ok = mbar_wait(bar(S::B_S + grp * 2 + buf), (i >> 1) & 1) && ok;
             fence_after_sync();
             unsigned a[64];
-            tmem_ld32(lane_addr + (qt * 2 + (t & 1)) * KN, reinterpret_cast<unsigned(&)[32]>(a[0]));
-            tmem_ld32(lane_addr + (qt * 2 + (t & 1)) * KN + 32, reinterpret_cast<unsigned(&)[32]>(a[32]));
+            tmem_ld32(lane_addr + (grp * 2 + buf) * KN, reinterpret_cast<unsigned(&)[32]>(a[0]));
+            tmem_ld32(lane_addr + (grp * 2 + buf) * KN + 32, reinterpret_cast<unsigned(&)[32]>(a[32]));
             tmem_ld_wait();
             if (softcap > 0.f) {
                 const float k = scale / softcap;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) a[i] = __float_as_uint(fast_tanh(__uint_as_float(a[i]) * k));
+                for (int e = 0; e < 64; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
             }
             float mx = -INFINITY;
             if (whole(j_base)) {
 #pragma unroll
-                for (int i = 0; i < 64; i += 2) mx = max3(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+                for (int e = 0; e < 64; e += 2) mx = max3(mx, __uint_as_float(a[e]), __uint_as_float(a[e + 1]));
             } else {
                 const unsigned long long vis = visible(j_base);
                 const unsigned vis_lo = (unsigned)vis, vis_hi = (unsigned)(vis >> 32);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    if (!((i < 32 ? vis_lo : vis_hi) & (1u << (i & 31)))) a[i] = 0xff800000u;
-                    mx = fmaxf(mx, __uint_as_float(a[i]));
+                for (int e = 0; e < 64; ++e) {
+                    if (!((e < 32 ? vis_lo : vis_hi) & (1u << (e & 31)))) a[e] = 0xff800000u;
+                    mx = fmaxf(mx, __uint_as_float(a[e]));
                 }
             }
             mx *= scale_eff;                                  // the scale is positive
@@ -484,10 +500,10 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 moved = true;
             }
             const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-            // P(t) goes into the buffer that P V(t - 2) read; O is touched only when P V(t - 1) is done
-            if (t > 1) ok = mbar_wait(bar(S::B_PV + qt * 2 + (t & 1)), ((t - 2) >> 1) & 1) && ok;
-            if (t > 0 && __any_sync(0xffffffffu, moved)) {
-                ok = mbar_wait(bar(S::B_PV + qt * 2 + ((t - 1) & 1)), ((t - 1) >> 1) & 1) && ok;
+            // P(i) goes into the buffer that P V(i - 2) read; O is touched only when P V(i - 1) is done
+            if (i > 1) ok = mbar_wait(bar(S::B_PV + grp * 2 + buf), ((i - 2) >> 1) & 1) && ok;
+            if (i > 0 && __any_sync(0xffffffffu, moved)) {
+                ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
                 fence_after_sync();
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
@@ -495,22 +511,22 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     tmem_ld32(o_addr + c0, o);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
                     tmem_st32(o_addr + c0, o);
                 }
                 tmem_st_wait();
             }
-            unsigned char* myP = myPs + (t & 1) * S::P_BYTES;
+            unsigned char* myP = myPs + buf * S::P_BYTES;
             const unsigned long long scale2 = pack2(scale_eff, scale_eff), shift2 = pack2(-mu, -mu);
             unsigned long long sum2 = pack2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) {
+            for (int e = 0; e < 64; e += 2) {
                 float x0, x1;
-                unpack2(fma2(pack2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), scale2, shift2), x0, x1);
+                unpack2(fma2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), scale2, shift2), x0, x1);
                 const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                 sum2 = add2(sum2, pack2(p0, p1));
-                a[i] = __float_as_uint(p0);
-                a[i + 1] = __float_as_uint(p1);
+                a[e] = __float_as_uint(p0);
+                a[e + 1] = __float_as_uint(p1);
             }
             float sum_lo, sum_hi;
             unpack2(sum2, sum_lo, sum_hi);
@@ -527,144 +543,216 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             fence_proxy_async();
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(S::B_P + qt * 2 + (t & 1)));        // S(t) is read, O is rescaled, P(t) is written
+            if (lane == 0) mbar_arrive(bar(S::B_P + grp * 2 + buf));           // S(i) is read, O is rescaled, P(i) is written
         }
-        ok = mbar_wait(bar(S::B_PV + qt * 2 + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1) && ok;
-    } else if (warp >= 4 * NQ && warp < 6 * NQ && qt < nq && lane == 0) {
+        if (n_mine > 0) ok = mbar_wait(bar(S::B_PV + grp * 2 + ((n_mine - 1) & 1)), ((n_mine - 1) >> 1) & 1) && ok;
+    } else if (warp >= 8 && warp < 12 && n_mine > 0 && lane == 0) {
         // ================================================================== an issuing thread: descriptors are a base plus a constant
         ok = mbar_wait(bar(S::B_Q + qt), 0) && ok;
         fence_after_sync();
-        if (((warp - 4 * NQ) & 1) == 0) {                     // S
+        if ((warp & 1) == 0) {                                // S
             const unsigned idesc = instr_desc_bf16(QM, KN, false);
             const unsigned long long dQ = smem_desc_sw128(smem_u32(sQ) + qt * S::Q_BYTES, 0), dK = smem_desc_sw128(smem_u32(sK), 0);
-            int st = 0;
-            unsigned par = 0;
-            for (int t = 0; t < n_tiles; ++t) {
-                ok = mbar_wait(bar(S::B_K_FULL + st), par) && ok;
-                if (t > 1) ok = mbar_wait(bar(S::B_P + qt * 2 + (t & 1)), ((t - 2) >> 1) & 1) && ok;      // the rows have read S(t - 2)
+            for (int i = 0; i < n_mine; ++i) {
+                const int t = tile_no(grp, i), st = t % STAGES;
+                ok = mbar_wait(bar(S::B_K_FULL + st), (t / STAGES) & 1) && ok;
+                if (i > 1) ok = mbar_wait(bar(S::B_P + grp * 2 + (i & 1)), ((i - 2) >> 1) & 1) && ok;     // the rows have read S(i - 2)
                 fence_after_sync();
                 const unsigned long long k_tile = dK + (unsigned long long)(st * (S::K_BYTES >> 4));
-                const unsigned d_s = tmem + (qt * 2 + (t & 1)) * KN;
+                const unsigned d_s = tmem + (grp * 2 + (i & 1)) * KN;
 #pragma unroll
                 for (int d16 = 0; d16 < D / 16; ++d16)        // 64-wide slabs of the head size, four steps of 16 (32 bytes) in each
                     mma_ss(d_s, dQ + (unsigned long long)(((d16 >> 2) * (QM * 128) + (d16 & 3) * 32) >> 4),
                            k_tile + (unsigned long long)(((d16 >> 2) * (KN * 128) + (d16 & 3) * 32) >> 4), idesc, d16 > 0);
-                mma_commit(bar(S::B_S + qt * 2 + (t & 1)));
+                mma_commit(bar(S::B_S + grp * 2 + (i & 1)));
                 mma_commit(bar(S::B_K_EMPTY + st));
-                if (++st == STAGES) { st = 0; par ^= 1u; }
             }
         } else {                                              // P V
             const unsigned idesc = instr_desc_bf16(QM, D, true);
-            const unsigned long long dP = smem_desc_sw128(smem_u32(sP) + qt * 2 * S::P_BYTES, 0);
+            const unsigned long long dP = smem_desc_sw128(smem_u32(sP) + grp * 2 * S::P_BYTES, 0);
             const unsigned long long dV = smem_desc_sw128_mn(smem_u32(sV), KN * 128, 1024u);
-            const unsigned d_o = tmem + S::O_COL + qt * D;
-            int st = 0;
-            unsigned par = 0;
-            for (int t = 0; t < n_tiles; ++t) {
-                ok = mbar_wait(bar(S::B_V_FULL + st), par) && ok;
-                ok = mbar_wait(bar(S::B_P + qt * 2 + (t & 1)), (t >> 1) & 1) && ok;
+            const unsigned d_o = tmem + S::O_COL + grp * D;
+            for (int i = 0; i < n_mine; ++i) {
+                const int t = tile_no(grp, i), st = t % STAGES;
+                ok = mbar_wait(bar(S::B_V_FULL + st), (t / STAGES) & 1) && ok;
+                ok = mbar_wait(bar(S::B_P + grp * 2 + (i & 1)), (i >> 1) & 1) && ok;
                 fence_after_sync();
-                const unsigned long long v_tile = dV + (unsigned long long)(st * (S::K_BYTES >> 4)), p_tile = dP + (unsigned long long)((t & 1) * (S::P_BYTES >> 4));
+                const unsigned long long v_tile = dV + (unsigned long long)(st * (S::K_BYTES >> 4)), p_tile = dP + (unsigned long long)((i & 1) * (S::P_BYTES >> 4));
 #pragma unroll
                 for (int k16 = 0; k16 < KN / 16; ++k16)       // 16 keys: 32 bytes along P's rows, 2048 bytes down V's
-                    mma_ss(d_o, p_tile + (unsigned long long)(k16 * 2), v_tile + (unsigned long long)(k16 * 128), idesc, t > 0 || k16 > 0);
-                mma_commit(bar(S::B_PV + qt * 2 + (t & 1)));
+                    mma_ss(d_o, p_tile + (unsigned long long)(k16 * 2), v_tile + (unsigned long long)(k16 * 128), idesc, i > 0 || k16 > 0);
+                mma_commit(bar(S::B_PV + grp * 2 + (i & 1)));
                 mma_commit(bar(S::B_V_EMPTY + st));
-                if (++st == STAGES) { st = 0; par ^= 1u; }
             }
         }
-    } else if (warp >= 6 * NQ) {
+    } else if (warp >= 12) {
         // ================================================================== the loaders
-        const bool is_k = warp == 6 * NQ;
+        const bool is_k = warp == 12;
         const bf16* pool = is_k ? kpool : vpool;
         unsigned char* ring = is_k ? sK : sV;
         const int b_full = is_k ? S::B_K_FULL : S::B_V_FULL, b_empty = is_k ? S::B_K_EMPTY : S::B_V_EMPTY;
-        // The pages of rows `lane` and `lane + 32` of a tile are asked for one tile ahead.
-        auto ask_pages = [&](int jt, int (&page)[2]) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int j = jt * KN + u * 32 + lane;
-                page[u] = j >= sg.lo && j <= sg.hi ? bt_row[pg.block(j)] : -1;
-            }
-        };
-        auto announce = [&](int t) {                          // tile t has landed
-            if (!is_k && !whole((jt_begin + t) * KN)) {
-                uint4* piece = reinterpret_cast<uint4*>(ring + (t % STAGES) * S::K_BYTES);
-                __syncwarp();
-                bool odd = false;
+        // Values of a tile that has landed and that some row does not see in full: rows of no key of this CTA become zero, and so do
+        // values that are no numbers, which are noted.
+        auto clean = [&](int t) {
+            uint4* piece = reinterpret_cast<uint4*>(ring + (t % STAGES) * S::K_BYTES);
+            const int j_base = (jt_begin + t) * KN;
+            bool odd = false;
 #pragma unroll 4
-                for (int i = lane; i < (int)(S::K_BYTES / 16); i += 32) {
-                    uint4 v = piece[i];
-                    const unsigned x = odd_halves(v.x), y = odd_halves(v.y), z = odd_halves(v.z), w = odd_halves(v.w);
-                    if (x | y | z | w) {
-                        odd = true;
-                        v.x &= ~((x >> 15) * 0xffffu); v.y &= ~((y >> 15) * 0xffffu);
-                        v.z &= ~((z >> 15) * 0xffffu); v.w &= ~((w >> 15) * 0xffffu);
-                        piece[i] = v;
+            for (int i = lane; i < (int)(S::K_BYTES / 16); i += 32) {
+                uint4 v = piece[i];
+                const int j = j_base + ((i >> 3) & (KN - 1));         // 8 pieces a row of 128 bytes, KN rows a slab
+                const unsigned x = odd_halves(v.x), y = odd_halves(v.y), z = odd_halves(v.z), w = odd_halves(v.w);
+                if (j < sg.lo || j > sg.hi) {
+                    piece[i] = make_uint4(0u, 0u, 0u, 0u);
+                } else if (x | y | z | w) {
+                    odd = true;
+                    v.x &= ~((x >> 15) * 0xffffu); v.y &= ~((y >> 15) * 0xffffu);
+                    v.z &= ~((z >> 15) * 0xffffu); v.w &= ~((w >> 15) * 0xffffu);
+                    piece[i] = v;
+                }
+            }
+            if (odd) *odd_values = 1;
+        };
+        if (by_tma) {
+            // A lane for each (page of the tile, slab): it knows the page one tile ahead and asks for its box.  A whole tile's bytes are counted
+            // on the barrier that its product waits for; values that have to be looked through first land on a barrier of the loader's.
+            const CUtensorMap* map = is_k ? &kmap : &vmap;
+            const int box = min(pg.page_size, KN), pi = lane / S::DS, slab = lane % S::DS;
+            const bool mine = pi * box < KN;
+            auto in_sight = [&](int jt) { const int j = jt * KN + pi * box; return mine && j + box > sg.lo && j <= sg.hi; };
+            auto ask_page = [&](int jt) { return in_sight(jt) ? bt_row[pg.block(jt * KN + pi * box)] : -1; };
+            unsigned land_par = 0u;                           // the parity of each stage's next landing
+            auto finish = [&](int t) {                        // values of tile t, which was not whole, have landed
+                const int st = t % STAGES;
+                if (whole((jt_begin + t) * KN)) return;
+                ok = mbar_wait(bar(S::B_V_LAND + st), (land_par >> st) & 1u) && ok;
+                land_par ^= 1u << st;
+                clean(t);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(S::B_V_FULL + st));
+            };
+            int next = ask_page(jt_begin);
+            for (int t = 0; t < n_tiles; ++t) {
+                const int st = t % STAGES, page = next;
+                if (t >= STAGES) ok = mbar_wait(bar(b_empty + st), (t / STAGES - 1) & 1) && ok;
+                const unsigned dst = smem_u32(ring) + st * S::K_BYTES + slab * (KN * 128) + pi * box * 128;
+                const unsigned boxes = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                const bool gone = in_sight(jt_begin + t) && page < 0;
+                if (__any_sync(0xffffffffu, gone)) {          // a block that is marked as gone reads as zero
+                    if (gone)
+                        for (int i = 0; i < box * 8; ++i) reinterpret_cast<uint4*>(ring + (dst - smem_u32(ring)))[i] = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                const unsigned land = bar(is_k || whole((jt_begin + t) * KN) ? b_full + st : S::B_V_LAND + st);
+                if (lane == 0) mbar_arrive_expect_tx(land, boxes * (unsigned)(box * 128));
+                __syncwarp();
+                if (page >= 0) tma::load_2d(dst, map, slab * 64, (page * Hkv + kvh) * pg.page_size + pg.row((jt_begin + t) * KN + pi * box), land);
+                if (t + 1 < n_tiles) next = ask_page(jt_begin + t + 1);
+                if (!is_k && t >= S::LAG) finish(t - S::LAG);
+            }
+            if (!is_k)
+                for (int t = max(0, n_tiles - S::LAG); t < n_tiles; ++t) finish(t);
+        } else {
+            // The pages of rows `lane` and `lane + 32` of a tile are asked for one tile ahead.
+            auto ask_pages = [&](int jt, int (&page)[2]) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int j = jt * KN + u * 32 + lane;
+                    page[u] = j >= sg.lo && j <= sg.hi ? bt_row[pg.block(j)] : -1;
+                }
+            };
+            auto announce = [&](int t) {                      // tile t has landed
+                if (!is_k && !whole((jt_begin + t) * KN)) {
+                    __syncwarp();
+                    clean(t);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(b_full + t % STAGES));
+            };
+            int next_page[2];
+            ask_pages(jt_begin, next_page);
+            for (int t = 0; t < n_tiles; ++t) {
+                const int st = t % STAGES;
+                if (t >= STAGES) ok = mbar_wait(bar(b_empty + st), (t / STAGES - 1) & 1) && ok;
+                const unsigned tile_smem = smem_u32(ring) + st * S::K_BYTES;
+                // Lane L knows where rows L and L + 32 lie (0: not to be read); D / 8 neighbouring lanes then copy one row, so that an
+                // instruction reads whole lines.
+                unsigned long long where[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    where[u] = next_page[u] < 0 ? 0ull : reinterpret_cast<unsigned long long>(
+                        pool + (((size_t)next_page[u] * Hkv + kvh) * pg.page_size + pg.row((jt_begin + t) * KN + u * 32 + lane)) * D);
+                const unsigned slab = (unsigned)(sub >> 3) * (KN * 128), c7 = (unsigned)(sub & 7);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 32 / RPI; ++i) {
+                        const int owner = i * RPI + rsel, krow = u * 32 + owner;
+                        const unsigned long long w = __shfl_sync(0xffffffffu, where[u], owner);
+                        const bf16* src = w ? reinterpret_cast<const bf16*>(w) + sub * 8 : pool;
+                        cp16u(tile_smem + (krow >> 3) * 1024 + (krow & 7) * 128 + slab + ((c7 ^ (unsigned)(krow & 7)) << 4), src, w != 0ull);
                     }
                 }
-                if (odd) *odd_values = 1;
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(b_full + t % STAGES));
-        };
-        int next_page[2];
-        ask_pages(jt_begin, next_page);
-        for (int t = 0; t < n_tiles; ++t) {
-            const int st = t % STAGES;
-            if (t >= STAGES) ok = mbar_wait(bar(b_empty + st), (t / STAGES - 1) & 1) && ok;
-            const unsigned tile_smem = smem_u32(ring) + st * S::K_BYTES;
-            // Lane L knows where rows L and L + 32 lie (0: not to be read); D / 8 neighbouring lanes then copy one row, so that an
-            // instruction reads whole lines.
-            unsigned long long where[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                where[u] = next_page[u] < 0 ? 0ull : reinterpret_cast<unsigned long long>(
-                    pool + (((size_t)next_page[u] * Hkv + kvh) * pg.page_size + pg.row((jt_begin + t) * KN + u * 32 + lane)) * D);
-            const unsigned slab = (unsigned)(sub >> 3) * (KN * 128), c7 = (unsigned)(sub & 7);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int i = 0; i < 32 / RPI; ++i) {
-                    const int owner = i * RPI + rsel, krow = u * 32 + owner;
-                    const unsigned long long w = __shfl_sync(0xffffffffu, where[u], owner);
-                    const bf16* src = w ? reinterpret_cast<const bf16*>(w) + sub * 8 : pool;
-                    cp16u(tile_smem + (krow >> 3) * 1024 + (krow & 7) * 128 + slab + ((c7 ^ (unsigned)(krow & 7)) << 4), src, w != 0ull);
+                asm volatile("cp.async.commit_group;\n" ::);
+                if (t + 1 < n_tiles) ask_pages(jt_begin + t + 1, next_page);
+                if (t >= S::LAG) {
+                    cp_wait<S::LAG>();
+                    announce(t - S::LAG);
                 }
             }
-            asm volatile("cp.async.commit_group;\n" ::);
-            if (t + 1 < n_tiles) ask_pages(jt_begin + t + 1, next_page);
-            if (t >= S::LAG) {
-                cp_wait<S::LAG>();
-                announce(t - S::LAG);
-            }
+            cp_wait<0>();
+            for (int t = max(0, n_tiles - S::LAG); t < n_tiles; ++t) announce(t);
         }
-        cp_wait<0>();
-        for (int t = max(0, n_tiles - S::LAG); t < n_tiles; ++t) announce(t);
     }
+    if (STREAMS && has_rows) *joined(grp) = make_float2(m_ref, l_run);
     pdl_trigger_late();
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
     if (has_rows) {
-        // the rows leave: the finished ones, or O as it stands with the reference maximum and the sum
+        // The rows leave: the finished ones, or O as it stands with the reference maximum and the sum.  Streams are joined first, either group
+        // for half of the columns.
         const bool odd = *odd_values != 0, part = sg.n_split > 1;
         const size_t at = token * Hq + h, slot = (size_t)split * total_rows * Hq + at;
+        float w_a = 1.f, w_b = 0.f;
+        if (STREAMS && n_tiles > 1) {
+            const float2 a = *joined(0), b = *joined(1);
+            m_ref = fmaxf(a.x, b.x);
+            const float top = m_ref == -INFINITY ? 0.f : m_ref;
+            w_a = fast_exp2(a.x - top);
+            w_b = fast_exp2(b.x - top);
+            l_run = a.y * w_a + b.y * w_b;
+        } else if (STREAMS) {
+            const float2 a = *joined(0);
+            m_ref = a.x;
+            l_run = a.y;
+        }
         const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-        if (part && row_valid) {
+        if (part && row_valid && (!STREAMS || grp == 0)) {
             part_ml[2 * slot] = m_ref;
             part_ml[2 * slot + 1] = l_run;
         }
         float l_all = l_run;
         if (sink != nullptr && !part) l_all += exp2f(sink[h] * LOG2E - mu);
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        const unsigned o_first = lane_addr + S::O_COL + (STREAMS ? 0 : grp * D);
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 32) {
+        for (int c0 = STREAMS ? grp * (D / 2) : 0; c0 < (STREAMS ? (grp + 1) * (D / 2) : D); c0 += 32) {
             unsigned o[32];
             __syncwarp();
-            tmem_ld32(o_addr + c0, o);
-            tmem_ld_wait();
+            tmem_ld32(o_first + c0, o);
+            if (STREAMS && n_tiles > 1) {
+                unsigned o_b[32];
+                tmem_ld32(o_first + D + c0, o_b);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), w_a, __uint_as_float(o_b[i]) * w_b));
+            } else {
+                tmem_ld_wait();
+            }
             if (odd && row_valid) {
                 // what the products left out: values that are no numbers, where this row sees their keys
                 for (int t = 0; t < n_tiles; ++t) {
@@ -713,7 +801,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     if (!ok) atomicExch(status, 1);
     fence_before_sync();
     __syncthreads();
-    if (warp == 4 * NQ) tmem_dealloc(tmem, S::TMEM_COLS);
+    if (warp == 8) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
 // out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).
@@ -762,7 +850,7 @@ struct TreeCall {
     const int *cu_q, *seg_pos0, *parent, *block_table;
     int bt_stride, page_size;
     void* out;
-    int segments, max_nodes, total_rows, Hq, Hkv, D;
+    int segments, max_nodes, total_rows, Hq, Hkv, D, pages;
     float scale;
     int window;
     float softcap;
@@ -800,18 +888,26 @@ int simt(const TreeCall& a) {
     return e ? e : merge<TA>(a);
 }
 
-template <int D, int NQ>
+template <int D, bool STREAMS>
 int tc5_launch(const TreeCall& a) {
-    typedef Shape<D, NQ> S;
+    typedef Shape<D, STREAMS> S;
+    constexpr int ROWS = S::NQ * QM;
     static PerDevice configured;
     const int rc = configured.once([&](int) {
-        return cudaFuncSetAttribute(tree_tc5_kernel<D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        return cudaFuncSetAttribute(tree_tc5_kernel<D, STREAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     });
     if (rc) return rc;
-    dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + NQ * QM - 1) / (NQ * QM) * a.Hkv, a.segments, a.splits);
-    const int e = rb_launch_pdl(tree_tc5_kernel<D, NQ>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
+    // pages are whole boxes of whole groups of eight rows, and their rows can be counted in 31 bits
+    const long long pool_rows = (long long)a.pages * a.Hkv * a.page_size;
+    int by_tma = a.page_size % 8 == 0 && (KN % a.page_size == 0 || a.page_size % KN == 0) && pool_rows <= 0x7fffffffll;
+    CUtensorMap kmap = {}, vmap = {};
+    const int box = a.page_size < KN ? a.page_size : KN;
+    if (by_tma && !(tma::make_map_bf16(&kmap, a.kpool, (int)pool_rows, D, D, box) && tma::make_map_bf16(&vmap, a.vpool, (int)pool_rows, D, D, box)))
+        return (int)cudaErrorInvalidValue;
+    dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
+    const int e = rb_launch_pdl(tree_tc5_kernel<D, STREAMS>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
                                 (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, (bf16*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, a.status);
+                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
 }
 
@@ -824,7 +920,7 @@ RB_EXPORT int rb_tree_max_nodes() { return TREE_MAX_NODES; }
 // query_tiles: 0 the CUDA cores; 1 or 2 the tensor cores with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, pools and
 // queries on 16-byte boundaries, ld a multiple of 8).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
-                                const int* parent, const int* block_table, int bt_stride, int page_size, void* out, int act_dtype,
+                                const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
                                 int segments, int max_nodes, int total_rows, int Hq, int Hkv, int D, float scale, int window,
                                 float softcap, const float* sink, int splits, int share, void* scratch, int query_tiles, int* status,
                                 cudaStream_t st) {
@@ -832,12 +928,12 @@ RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const 
     if (segments > 65535 || max_nodes > TREE_MAX_NODES || D <= 0 || D > TREE_MAX_D || Hkv <= 0 || Hq % Hkv || page_size <= 0) return (int)cudaErrorInvalidValue;
     if (splits < 1 || splits > 64 || (splits > 1 && (share <= 0 || scratch == nullptr))) return (int)cudaErrorInvalidValue;
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
-                  D, scale, window, softcap, sink, splits, share, (float*)scratch, status, st};
+                  D, pages, scale, window, softcap, sink, splits, share, (float*)scratch, status, st};
     if (query_tiles > 0) {
         if (act_dtype != RB_BF16 || (D != 64 && D != 128) || query_tiles > 2 || status == nullptr) return (int)cudaErrorInvalidValue;
         if ((((uintptr_t)q | (uintptr_t)kpool | (uintptr_t)vpool | (uintptr_t)out) & 15) || ld % 8) return (int)cudaErrorInvalidValue;
-        if (D == 64) return query_tiles == 1 ? tc5_launch<64, 1>(a) : tc5_launch<64, 2>(a);
-        return query_tiles == 1 ? tc5_launch<128, 1>(a) : tc5_launch<128, 2>(a);
+        if (D == 64) return query_tiles == 1 ? tc5_launch<64, true>(a) : tc5_launch<64, false>(a);
+        return query_tiles == 1 ? tc5_launch<128, true>(a) : tc5_launch<128, false>(a);
     }
     if (act_dtype == RB_F32) return D <= 128 ? simt<float, 1>(a) : simt<float, 2>(a);
     return D <= 128 ? simt<bf16, 1>(a) : simt<bf16, 2>(a);

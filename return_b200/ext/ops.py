@@ -2255,7 +2255,7 @@ def tree_lib() -> ctypes.CDLL:
     if _tree is None:
         lib = build.load("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE})
         P, I, F = c_void_p, c_int, c_float
-        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, I, P, P]
+        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, I, P, P]
         lib.rb_tree_attention.restype = c_int
         _tree = build.native_calls(lib)
     return _tree
@@ -2381,7 +2381,7 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
     scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
     _check(lib.rb_tree_attention(q_at, ld, _ptr(k_pool), _ptr(v_pool), _ptr(batch.cu_q), _ptr(batch.seg_pos0),
-                                 _ptr(batch.tree_parent), _ptr(block_table), block_table.stride(0), page_size, _ptr(out),
+                                 _ptr(batch.tree_parent), _ptr(block_table), block_table.stride(0), page_size, k_pool.shape[0], _ptr(out),
                                  dtype_code(qkv.dtype), n, longest, T, num_heads, num_kv_heads, head_dim, float(scale), window,
                                  float(softcap or 0.0), _sink_ptr(sink, num_heads), splits, share, _ptr(scratch), tiles,
                                  _status_word(qkv.device) if tiles else None, _stream()),
