@@ -2279,20 +2279,22 @@ def branch_lib() -> ctypes.CDLL:
     return _branch
 
 
-def _same_device(device, *tensors) -> None:
-    """Every tensor of a call lies on one CUDA device, the current one: kernels are launched there."""
+def _same_device(*tensors) -> None:
+    """Every tensor of a call lies on the current CUDA device: kernels are launched there."""
+    device = None
     for t in tensors:
         if t is not None:
-            if not (t.is_cuda):
+            at = t.get_device()
+            if at < 0:
                 raise KernelError("the engine's kernels run on a CUDA device only; got a CPU tensor")
-            if not (t.device == device):
-                raise KernelError(f"tensors on {t.device} and {device} in one call")
-    if not (device.index == _device_index()):
-        raise KernelError(f"tensors on {device}, but the current device is cuda:{_device_index()}")
+            if device is None:
+                device = _device_index()
+            if at != device:
+                raise KernelError(f"a tensor on cuda:{at}, but the current device is cuda:{device}")
 
 
 def _ints(what: str, t: torch.Tensor, *shape) -> None:
-    if not (t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape):
+    if t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous():
         raise KernelError(f"{what}: contiguous int32 of shape {shape} wanted, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -2346,46 +2348,64 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     stands at position ``seg_pos0 + depth(i)``; it sees the segment's cached keys, its ancestors and itself, with a window those
     less than ``window`` positions back.  ``qkv``: rows that begin with the rotated queries (row stride any).  ``softcap``,
     ``sink``: as in ``paged_attention``.  A segment has up to TREE_MAX_NODES nodes."""
-    T = qkv.shape[0]
-    n, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
+    key = (qkv.shape, k_pool.shape, v_pool.shape, out.shape, block_table.shape, qkv.dtype, page_size, num_heads, num_kv_heads, head_dim, window,
+           scale, softcap, sink is None)
+    plan = batch.scratch.get(key)                      # the step's layers are alike: what follows from shapes is looked at once
+    if plan is None:
+        plan = batch.scratch[key] = _tree_plan(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim,
+                                               scale, window, sink, softcap)
+    n, T, longest, window, softcap, dtype, code, shares = plan
+    if not (k_pool.dtype == dtype and v_pool.dtype == dtype and out.dtype == dtype):
+        raise KernelError("queries, keys, values and output are of one type")
+    if not (qkv.stride(1) == 1 and k_pool.is_contiguous() and v_pool.is_contiguous() and out.is_contiguous()
+            and block_table.dtype == torch.int32 and block_table.stride(1) == 1):
+        raise KernelError("qkv and block_table (int32): unit stride along a row; pools and out: contiguous")
+    _same_device(qkv, k_pool, v_pool, block_table, out, batch.cu_q, batch.seg_pos0, batch.tree_parent, sink)
+    q_at, k_at, v_at, out_at, ld = qkv.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), qkv.stride(0)
+    kind = 0 if (q_at | k_at | v_at | out_at) & 15 or ld & 7 else 1          # kernels that move 16 bytes at a time, or any
+    if shares[kind] is None:
+        shares[kind] = _tree_launch(batch, page_size, block_table, num_heads, num_kv_heads, head_dim, window, dtype, kind)
+    tiles, splits, share = shares[kind]
+    # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
+    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
+    _check(tree_lib().rb_tree_attention(q_at, ld, k_at, v_at, batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), batch.tree_parent.data_ptr(),
+                                        block_table.data_ptr(), block_table.stride(0), page_size, k_pool.shape[0], out_at, code, n, longest, T,
+                                        num_heads, num_kv_heads, head_dim, scale, window, softcap, _sink_ptr(sink, num_heads), splits, share,
+                                        None if scratch is None else scratch.data_ptr(), tiles, _status_word(qkv.device) if tiles else None,
+                                        _stream()), "tree_attention", 2 if splits > 1 else 1)
+
+
+def _tree_plan(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window, sink, softcap):
+    """What ``tree_attention`` knows of a step from shapes and settings alone; raises where they do not fit."""
+    if block_table.dim() != 2:
+        raise KernelError("block_table: int32 [segments, blocks]")
+    n, rows, longest, _, _ = _tree_lengths(batch, page_size, block_table.shape[1])
     if not (num_heads % num_kv_heads == 0 and 0 < head_dim <= 256):
         raise KernelError("query heads: a multiple of the kv heads; head size: up to 256")
-    if not (qkv.dim() == 2 and qkv.stride(1) == 1 and T == rows and qkv.shape[1] >= num_heads * head_dim):
-        raise KernelError("qkv: a row per node, unit stride")
-    if not (k_pool.dtype == v_pool.dtype == qkv.dtype == out.dtype):
-        raise KernelError("queries, keys, values and output are of one type")
-    if not (tuple(k_pool.shape[1:]) == (num_kv_heads, page_size, head_dim) and k_pool.shape == v_pool.shape and k_pool.is_contiguous() and v_pool.is_contiguous()):
+    if not (qkv.dim() == 2 and qkv.shape[0] == rows and qkv.shape[1] >= num_heads * head_dim):
+        raise KernelError("qkv: a row per node, of the query heads at least")
+    if not (k_pool.shape[1:] == (num_kv_heads, page_size, head_dim) and k_pool.shape == v_pool.shape):
         raise KernelError("pools: contiguous [pages, kv heads, page size, head size]")
-    if not (tuple(out.shape) == (T, num_heads * head_dim) and out.is_contiguous()):
+    if out.shape != (rows, num_heads * head_dim):
         raise KernelError("out: contiguous [nodes, heads * head size]")
-    if not (block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == n and block_table.stride(1) == 1):
+    if block_table.shape[0] != n:
         raise KernelError("block_table: int32 [segments, blocks]")
     if not (window is None or window >= 0):
         raise KernelError("window: not negative")
     if not (scale > 0 and (softcap is None or softcap >= 0)):
         raise KernelError("scale: positive; softcap: not negative")
-    _same_device(qkv.device, qkv, k_pool, v_pool, block_table, out, batch.cu_q, batch.tree_parent, sink)
-    window = int(window or 0)
-    lib = tree_lib()
+    return n, rows, longest, int(window or 0), float(softcap or 0.0), qkv.dtype, dtype_code(qkv.dtype), [None, None]
+
+
+def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_heads: int, head_dim: int, window: int, dtype, kind: int):
+    """(query tiles of the tensor cores' kernel or 0, splits, share) of a step's launches."""
+    _, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
     group = num_heads // num_kv_heads
-    q_at, ld = _ptr(qkv), qkv.stride(0)
     tiles = 0                                          # the tensor cores take up to two tiles of TREE_TILE_ROWS rows a CTA
-    if qkv.dtype == torch.bfloat16 and head_dim in TC5_ATTENTION_HEAD_DIMS and not ((q_at | _ptr(k_pool) | _ptr(v_pool) | _ptr(out)) & 15 or ld & 7):
+    if kind and dtype == torch.bfloat16 and head_dim in TC5_ATTENTION_HEAD_DIMS:
         tiles = 1 if longest * group <= TREE_TILE_ROWS else 2
-    key = ("tree.shares", num_heads, num_kv_heads, head_dim, window, tiles)
-    shares = batch.scratch.get(key)
-    if shares is None:
-        shares = batch.scratch[key] = tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim,
-                                                  tiles * TREE_TILE_ROWS or 32, 1 if tiles or head_dim > 128 else 2)
-    splits, share = shares
-    # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
-    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
-    _check(lib.rb_tree_attention(q_at, ld, _ptr(k_pool), _ptr(v_pool), _ptr(batch.cu_q), _ptr(batch.seg_pos0),
-                                 _ptr(batch.tree_parent), _ptr(block_table), block_table.stride(0), page_size, k_pool.shape[0], _ptr(out),
-                                 dtype_code(qkv.dtype), n, longest, T, num_heads, num_kv_heads, head_dim, float(scale), window,
-                                 float(softcap or 0.0), _sink_ptr(sink, num_heads), splits, share, _ptr(scratch), tiles,
-                                 _status_word(qkv.device) if tiles else None, _stream()),
-           "tree_attention", 2 if splits > 1 else 1)
+    return (tiles,) + tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim, tiles * TREE_TILE_ROWS or 32,
+                                  1 if tiles or head_dim > 128 else 2)
 
 
 def _pool_shape(pool):
@@ -2406,33 +2426,39 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
     ``caches``: (pool, block_table) of every group of layers; the row of slot ``seg_pos0 + path[i]`` goes to slot ``seg_pos0 + i``.  The
     request then holds ``seg_pos0 + count`` tokens.  Other rows stay as they are; a move from or to a page that the table marks as
     gone is left out."""
-    n, T = len(batch.host.seg_pos0), int(batch.host.cu_q[-1])
     width = path.shape[1] if path.dim() == 2 else 0
-    pools = [(pool, table, _pool_shape(pool)) for pool, table in caches]
-    lengths = None
-    for _, table, shape in pools:
-        if not (table.dtype == torch.int32 and table.dim() == 2 and table.shape[0] == n and table.stride(1) == 1):
-            raise KernelError("block_table: int32 [segments, blocks]")
-        lengths = _tree_lengths(batch, shape[3], table.shape[1])
+    lengths, shapes = None, []
+    for pool, table in caches:
+        key = ("tree.commit", pool.shape, pool.dtype, table.shape)
+        held = batch.scratch.get(key)                  # what follows from the shapes is looked at once a step
+        if held is None:
+            shape = _pool_shape(pool)
+            if table.dim() != 2 or table.shape[0] != len(batch.host.seg_pos0):
+                raise KernelError("block_table: int32 [segments, blocks]")
+            held = batch.scratch[key] = (shape, _tree_lengths(batch, shape[3], table.shape[1]))
+        if not (pool.is_contiguous() and table.dtype == torch.int32 and table.stride(1) == 1):
+            raise KernelError("a pool: contiguous; its block_table: int32, unit stride along a row")
+        shapes.append(held[0])
+        lengths = held[1]
     if lengths is None:                                # a model without paged layers: the walk alone
         lengths = _tree_lengths(batch, 1 << 30, 1)
+    n, T, longest = lengths[:3]
+    if width < longest:
+        raise KernelError(f"path: {longest} columns at least")
     _ints("sampled", sampled, T)
     _ints("tokens", batch.tokens, T)
-    if not (width >= lengths[2]):
-        raise KernelError(f"path: {lengths[2]} columns at least")
     _ints("path", path, n, width)
     _ints("emitted", emitted, n, width)
     _ints("count", count, n)
-    _same_device(sampled.device, sampled, batch.tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted,
-                 *[t for pool, table, _ in pools for t in (pool, table)])
-    lib = branch_lib()
-    args = (_ptr(batch.tokens), _ptr(batch.tree_parent), _ptr(sampled), _ptr(batch.cu_q), _ptr(batch.seg_pos0), n)
-    outs = (_ptr(path), _ptr(count), _ptr(emitted), width)
-    if not pools:
-        _check(lib.rb_tree_commit(*args, None, 0, 1, None, 0, 0, 0, 0, *outs, _stream()), "tree_commit")
-    for pool, table, (planes, pages, heads, page_size, row_bytes) in pools:
-        _check(lib.rb_tree_commit(*args, _ptr(table), table.stride(0), page_size, _ptr(pool), planes, pages, heads, row_bytes, *outs, _stream()),
-               "tree_commit")
+    _same_device(sampled, batch.tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted)
+    entry, st = branch_lib().rb_tree_commit, _stream()
+    args = (batch.tokens.data_ptr(), batch.tree_parent.data_ptr(), sampled.data_ptr(), batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), n)
+    outs = (path.data_ptr(), count.data_ptr(), emitted.data_ptr(), width)
+    if not shapes:
+        _check(entry(*args, None, 0, 1, None, 0, 0, 0, 0, *outs, st), "tree_commit")
+    for (pool, table), (planes, pages, heads, page_size, row_bytes) in zip(caches, shapes):
+        _same_device(pool, table)
+        _check(entry(*args, table.data_ptr(), table.stride(0), page_size, pool.data_ptr(), planes, pages, heads, row_bytes, *outs, st), "tree_commit")
         outs = (None, None, None, 0)
 
 
@@ -2444,7 +2470,7 @@ def copy_pages(pool, src, dst, rows) -> None:
     planes, pages, heads, page_size, row_bytes = _pool_shape(pool)
     for name, t in (("src", src), ("dst", dst), ("rows", rows)):
         _ints(name, t, n)
-    _same_device(pool.device, pool, src, dst, rows)
+    _same_device(pool, src, dst, rows)
     if n:
         _check(branch_lib().rb_copy_pages(_ptr(pool), _ptr(src), _ptr(dst), _ptr(rows), n, planes, pages, heads, page_size, row_bytes,
                                           _stream()), "copy_pages")
@@ -2483,7 +2509,7 @@ def copy_slots(table: SlotTable, src, dst) -> None:
     n = src.numel()
     _ints("src", src, n)
     _ints("dst", dst, n)
-    _same_device(table.device, src, dst)
+    _same_device(src, dst, table.states[0])
     if n:
         _check(branch_lib().rb_copy_slots(table.address, len(table.states), _ptr(src), _ptr(dst), n, table.slots, _stream()), "copy_slots",
                table.launches)
@@ -2492,32 +2518,36 @@ def copy_slots(table: SlotTable, src, dst) -> None:
 BEAM_MAX_KEEP, BEAM_MAX_BEAMS = 128, 64
 
 
+@functools.lru_cache(maxsize=256)
+def _beam_scratch(rows: int, V: int, keep: int, device: int) -> int:
+    return branch_lib().rb_beam_scratch(rows, V, keep)
+
+
 def beam_select(logits, scores, beams: int, scores_out, beams_out, tokens_out) -> None:
     """The ``scores_out.shape[1]`` best continuations of every request, best first.  ``logits`` float32 [requests * beams, V];
     ``scores`` float32 [requests * beams], the beams' sums of log-probabilities.  A continuation (b, v) has the total
     scores[b] + log_softmax(logits[b])[v]; ties go to the lowest (b, v).  A total that is no number, and every one of a beam whose
     score is not finite, counts as -inf.  Out: totals (float32), beams and tokens (int32), [requests, keep] each."""
-    if not (logits.dim() == 2 and scores_out.dim() == 2):
+    if logits.dim() != 2 or scores_out.dim() != 2:
         raise KernelError("logits [requests * beams, V], scores_out [requests, keep]")
     (rows, V), (requests, keep) = logits.shape, scores_out.shape
     if not (1 <= beams <= BEAM_MAX_BEAMS and rows == requests * beams):
         raise KernelError(f"logits: a row per request and beam, up to {BEAM_MAX_BEAMS} beams")
-    if not (1 <= keep <= min(BEAM_MAX_KEEP, beams * V)):
+    if not 1 <= keep <= min(BEAM_MAX_KEEP, beams * V):
         raise KernelError(f"{keep} continuations asked for: 1 to {BEAM_MAX_KEEP}, and no more than there are")
-    if not (rows <= 65535 and beams * V < 2 ** 31 - 1):
+    if rows > 65535 or beams * V >= 2 ** 31 - 1:
         raise KernelError("at most 65,535 rows, and beams * V within 31 bits")
-    if not (logits.dtype == torch.float32 and logits.stride(1) == 1):
+    if logits.dtype != torch.float32 or logits.stride(1) != 1:
         raise KernelError("logits: float32, unit stride along a row")
-    if not (scores.dtype == torch.float32 and scores.is_contiguous() and scores.numel() == rows):
+    if scores.dtype != torch.float32 or not scores.is_contiguous() or scores.numel() != rows:
         raise KernelError("scores: float32, one per row of logits")
-    if not (scores_out.dtype == torch.float32 and scores_out.is_contiguous()):
+    if scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
         raise KernelError("scores_out: contiguous float32")
     _ints("beams_out", beams_out, requests, keep)
     _ints("tokens_out", tokens_out, requests, keep)
-    _same_device(logits.device, logits, scores, scores_out, beams_out, tokens_out)
+    _same_device(logits, scores, scores_out, beams_out, tokens_out)
     if requests == 0:
         return
-    lib = branch_lib()
-    scratch = torch.empty(lib.rb_beam_scratch(rows, V, keep), dtype=torch.float32, device=logits.device)
-    _check(lib.rb_beam_select(_ptr(logits), logits.stride(0), _ptr(scores), requests, beams, V, keep, _ptr(scores_out), _ptr(beams_out),
-                              _ptr(tokens_out), _ptr(scratch), _stream()), "beam_select", 2)
+    scratch = torch.empty(_beam_scratch(rows, V, keep, logits.get_device()), dtype=torch.float32, device=logits.device)
+    _check(branch_lib().rb_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), requests, beams, V, keep, scores_out.data_ptr(),
+                              beams_out.data_ptr(), tokens_out.data_ptr(), scratch.data_ptr(), _stream()), "beam_select", 2)
