@@ -22,6 +22,7 @@
 #define TREE_MAX_NODES 256
 #define TREE_WORDS (TREE_MAX_NODES / 32)
 #define TREE_MAX_D 256
+#define TREE_MAX_SPLITS 64
 
 namespace {
 
@@ -66,199 +67,403 @@ __device__ __forceinline__ unsigned line_bits(const unsigned* line, int at) {
     return __funnelshift_r(lo, hi, s);
 }
 
-// ---------------------------------------------------------------------------------------- CUDA cores, any type and head size
-constexpr int SW = 8, RW = 4;                 // warps, rows a warp
-constexpr int SROWS = SW * RW;
-constexpr int SKEYS = 32;                     // keys of a tile in shared memory
+// ---------------------------------------------------------------------------------------- matrix instructions of a warp, any type and head size
+// A CTA of eight warps takes 32 rows and walks its keys in tiles of 64.  Scores: a warp 16 rows by 16 keys; softmax: a warp four rows, a lane two
+// keys; outputs: a warp 16 rows by a quarter of the columns, a tile's sum made by itself and added to the running one.  While the
+// scores are made the tile's values arrive, while the outputs are summed the next tile's keys.
+// bfloat16: operands as they are, probabilities rounded to bfloat16.  float32: an operand is split into three bfloat16 parts, which hold its 24
+// bits, as it is read (queries once), six of the nine products are made (the rest is below 2^-24 of a product), the largest in an accumulator
+// of its own; values are multiplied by 2^16 first, so that small ones keep their bits, and the sums by 2^-16.
+// Values that are no numbers (float32: or that 2^16 would take beyond them), of tiles that some row does not see in full in bfloat16 and of all
+// tiles in float32, are set to zero in shared memory (zero times infinity would reach every row), and added to the rows that see them from the
+// operands themselves; scores of float32 keys that have such elements are made again in the same way.
+constexpr int MROWS = 32, MTHREADS = 256;
+constexpr int SP = KEY_TILE + 8;              // floats of a row of scores: eight-byte reads of four rows by four lanes hit all banks
+constexpr float UP = 65536.f, DOWN = 1.f / UP;
 
-__device__ __forceinline__ void cp16(float* smem, const float* gmem, int bytes) {       // bytes behind `bytes` become zero
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(smem)), "l"(gmem), "r"(bytes));
+__device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
 }
+__device__ __forceinline__ void ldsm(unsigned (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void ldsm_trans(unsigned (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+struct Parts { unsigned h, m, l; };           // of two neighbouring values, the first in the low half
+__device__ __forceinline__ Parts split(float x, float y) {
+    Parts p;
+    p.h = pack_bf16(x, y);
+    x -= __uint_as_float(p.h << 16);
+    y -= __uint_as_float(p.h & 0xffff0000u);
+    p.m = pack_bf16(x, y);
+    x -= __uint_as_float(p.m << 16);
+    y -= __uint_as_float(p.m & 0xffff0000u);
+    p.l = pack_bf16(x, y);
+    return p;
+}
+// The six products of a first operand's parts (h, m, l) and a second's.
+__device__ __forceinline__ void mma_parts(float (&big)[4], float (&rest)[4], const unsigned (&ah)[4], const unsigned (&am)[4], const unsigned (&al)[4],
+                                          const Parts& b0, const Parts& b1) {
+    mma16(big, ah, b0.h, b1.h);
+    mma16(rest, ah, b0.l, b1.l);
+    mma16(rest, al, b0.h, b1.h);
+    mma16(rest, am, b0.m, b1.m);
+    mma16(rest, ah, b0.m, b1.m);
+    mma16(rest, am, b0.h, b1.h);
+}
+// Whether the products cannot take a value.
+__device__ __forceinline__ bool is_odd(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x77800000u; }        // |x| >= 2^112, or no number
+__device__ __forceinline__ bool is_odd(bf16 x) { return (__bfloat16_as_ushort(x) & 0x7f80u) == 0x7f80u; }
 
-// A warp owns four rows; lane j of a tile scores key j, the online softmax advances tile by tile, a lane keeps columns
-// 4 lane + 128 k ..+ 3 of the rows' outputs.  The eight warps share a tile of keys and values in shared memory, the next one on
-// its way meanwhile.  A key that a row does not see is left out, not multiplied by zero: it may hold anything.
-// grid: (row blocks x kv heads, segments, splits).  NC: runs of 128 columns.
-template <typename TA, int NC>
-__global__ void __launch_bounds__(32 * SW, NC == 1 ? 2 : 1)
-tree_simt_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, const TA* __restrict__ vpool,
-                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
-                 const int* __restrict__ block_table, int bt_stride, int page_size, TA* __restrict__ out,
-                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, int D, float scale, int window,
-                 float softcap, const float* __restrict__ sink, int share, int vec) {
-    const int seg = blockIdx.y, kvh = blockIdx.x % Hkv, row0 = blockIdx.x / Hkv * SROWS, split = blockIdx.z, G = Hq / Hkv;
-    const Segment sg(cu_q, seg_pos0, seg, window, share, gridDim.z);
-    const int rows = min(SROWS, sg.n * G - row0);
-    if (rows <= 0 || split >= sg.n_split) return;
-    const int D4 = (D + 3) & ~3, pitch = D4 + 4;
-    extern __shared__ __align__(16) float tree_smem[];
-    float* qs = tree_smem;                                             // [SROWS][pitch]
-    float* tiles = qs + SROWS * pitch;                                 // [2][keys, values][SKEYS][pitch]
+template <typename TA, int DP> struct MmaShape {
+    static constexpr bool F32 = sizeof(TA) == 4;
+    static constexpr int KPITCH = DP + 8, VPITCH = F32 ? DP + 4 : DP + 8, QPITCH = DP + 8;        // elements; reads of fragments hit all banks
+    static constexpr size_t K_BYTES = (size_t)KEY_TILE * KPITCH * sizeof(TA), V_BYTES = (size_t)KEY_TILE * VPITCH * sizeof(TA),
+                            Q_BYTES = (F32 ? 3 : 1) * (size_t)MROWS * QPITCH * 2, S_BYTES = (size_t)MROWS * SP * 4, P_BYTES = F32 ? 0 : (size_t)MROWS * SP * 2;
+    static constexpr size_t SMEM = K_BYTES + V_BYTES + Q_BYTES + S_BYTES + P_BYTES;
+};
+
+// grid: (row blocks x kv heads, segments, splits).  DP: the head size rounded up to 32, 64, 128 or 256; what lies behind D is zero.
+template <typename TA, int DP>
+__global__ void __launch_bounds__(MTHREADS, DP <= 128 ? 2 : 1)
+tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, const TA* __restrict__ vpool,
+                const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
+                const int* __restrict__ block_table, int bt_stride, int page_size, TA* __restrict__ out,
+                float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, int D, float scale, int window,
+                float softcap, const float* __restrict__ sink, int share, int vec) {
+    typedef MmaShape<TA, DP> S;
+    constexpr bool F32 = S::F32;
+    constexpr int PER16 = 16 / sizeof(TA);                             // elements of a 16-byte piece
+    constexpr int K16 = DP / 16, NT = DP / 32;                         // steps along the head size; blocks of eight columns of a warp's quarter
+    extern __shared__ __align__(16) unsigned char mma_smem[];
+    TA* ks = reinterpret_cast<TA*>(mma_smem);                          // [KEY_TILE][KPITCH]
+    TA* vs = reinterpret_cast<TA*>(mma_smem + S::K_BYTES);             // [KEY_TILE][VPITCH]
+    bf16* qs = reinterpret_cast<bf16*>(mma_smem + S::K_BYTES + S::V_BYTES);              // [parts][MROWS][QPITCH]
+    float* ss = reinterpret_cast<float*>(mma_smem + S::K_BYTES + S::V_BYTES + S::Q_BYTES);       // [MROWS][SP]: scores, then probabilities
+    bf16* ps = reinterpret_cast<bf16*>(mma_smem + S::K_BYTES + S::V_BYTES + S::Q_BYTES + S::S_BYTES);     // [MROWS][SP] in bfloat16
     __shared__ int parent[TREE_MAX_NODES];
-    __shared__ unsigned lines[SROWS][TREE_WORDS];
-    __shared__ int depths[SROWS];
+    __shared__ unsigned lines[MROWS][TREE_WORDS];
+    __shared__ long long where[2][KEY_TILE];
+    __shared__ int lows[MROWS];                                        // a row's first key
+    __shared__ unsigned odd_keys[2], odd_values[2];                    // a tile's keys that have elements the products cannot take
+    __shared__ float s_alpha[MROWS], s_m[MROWS], s_l[MROWS];
+    pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int seg = blockIdx.y, kvh = blockIdx.x % Hkv, row0 = blockIdx.x / Hkv * MROWS, sp = blockIdx.z, G = Hq / Hkv;
+    const Segment sg(cu_q, seg_pos0, seg, window, share, gridDim.z);
+    const int rows = min(MROWS, sg.n * G - row0);
+    if (rows <= 0 || sp >= sg.n_split) return;
     const int* bt = block_table + (size_t)seg * bt_stride;
-    const size_t head_stride = (size_t)page_size * D;
-    const int r0 = warp * RW, nr = min(RW, rows - r0);                 // this warp's rows (nr <= 0: none)
+    const int t0 = share > 0 ? sp * share : 0, t1 = share > 0 && sp + 1 < sg.n_split ? t0 + share : sg.tiles;      // this CTA's tiles
+    auto q_row = [&](int r) { return q + (size_t)(sg.q_begin + (row0 + r) / G) * ld + (size_t)(kvh * G + (row0 + r) % G) * D; };
 
-    // this CTA's keys: [j_begin, j_end)
-    const int t0 = share > 0 ? split * share : 0, t1 = share > 0 && split + 1 < sg.n_split ? t0 + share : sg.tiles;
-    const int j_begin = max((sg.jt0 + t0) * KEY_TILE, sg.lo / SKEYS * SKEYS), j_end = min((sg.jt0 + t1) * KEY_TILE, sg.hi + 1);
-
-    const int per = D4 >> 2;
-    auto fetch = [&](int j0, int buf) {
-        float* ks = tiles + buf * 2 * SKEYS * pitch;
-        int page_r[SKEYS / SW];                                        // looked up together, not one behind the other
-#pragma unroll
-        for (int i = 0; i < SKEYS / SW; ++i) {
-            const int j = j0 + warp + i * SW;
-            page_r[i] = j >= sg.lo && j < j_end ? bt[j / page_size] : -1;
+    // Where a tile's rows lie in a pool, -1: no key of this CTA's, or a block marked as gone.
+    auto locate = [&](int jt) {
+        if (tid < KEY_TILE) {
+            const int j = jt * KEY_TILE + tid, page = j >= sg.lo && j <= sg.hi ? bt[j / page_size] : -1;
+            where[jt & 1][tid] = page < 0 ? -1 : (((long long)page * Hkv + kvh) * page_size + j % page_size) * D;
         }
+    };
+    // A tile's keys or values on their way: PIECES lanes a row; rows at -1 become zero.
+    constexpr int PIECES = DP / PER16 < 32 ? DP / PER16 : 32;
+    const int d_first = PER16 * (lane % PIECES);
+    auto fetch = [&](TA* to, int pitch, const TA* pool, int jt) {
+#pragma unroll 4
+        for (int r = warp * (32 / PIECES) + lane / PIECES; r < KEY_TILE; r += (MTHREADS / 32) * (32 / PIECES)) {
+            const long long at = where[jt & 1][r];
 #pragma unroll
-        for (int i = 0; i < SKEYS / SW; ++i) {
-            const int jj = warp + i * SW, j = j0 + jj, page = page_r[i];
-            const size_t at = page < 0 ? 0 : ((size_t)page * Hkv + kvh) * head_stride + (size_t)(j % page_size) * D;
-            float* kd = ks + jj * pitch;
-            float* vd = kd + SKEYS * pitch;
-            for (int c = lane; c < per; c += 32) {
-                const int d = 4 * c;
+            for (int d = d_first; d < DP; d += PER16 * PIECES) {
+                if (d >= D) continue;
                 if (vec) {
-                    cp16(kd + d, reinterpret_cast<const float*>(kpool) + at + d, page < 0 ? 0 : 16);
-                    cp16(vd + d, reinterpret_cast<const float*>(vpool) + at + d, page < 0 ? 0 : 16);
+                    const int bytes = at < 0 ? 0 : 16;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr(to + r * pitch + d)), "l"(pool + (at < 0 ? 0 : at + d)), "r"(bytes));
                 } else {
-                    for (int e = d; e < d + 4; ++e) {
-                        const bool there = page >= 0 && e < D;
-                        kd[e] = there ? to_f32(kpool[at + e]) : 0.f;
-                        vd[e] = there ? to_f32(vpool[at + e]) : 0.f;
-                    }
+#pragma unroll
+                    for (int e = 0; e < PER16; ++e)
+                        if (d + e < D) to[r * pitch + d + e] = at >= 0 ? pool[at + d + e] : from_f32<TA>(0.f);
                 }
             }
         }
         asm volatile("cp.async.commit_group;\n" ::);
     };
-    fetch(j_begin, 0);
-    for (int i = tid; i < sg.n; i += 32 * SW) parent[i] = tree_parent[sg.q_begin + i];
-    for (int d = lane; d < D4; d += 32)                                // a warp reads its own rows only; rows that do not exist are zero
+    locate(sg.jt0 + t0);
+    for (int i = tid; i < sg.n; i += MTHREADS) parent[i] = tree_parent[sg.q_begin + i];
+    if (tid < 2) odd_keys[tid] = odd_values[tid] = 0u;
+    for (int i = tid; i < KEY_TILE * (DP - D); i += MTHREADS) {        // behind the head size, for good
+        const int r = i / (DP - D), d = D + i % (DP - D);
+        ks[r * S::KPITCH + d] = vs[r * S::VPITCH + d] = from_f32<TA>(0.f);
+    }
+    // Queries, split: rows that do not exist are zero.
+    for (int r = warp; r < MROWS; r += MTHREADS / 32) {
+        const TA* src = q_row(r < rows ? r : 0);
+        float2 x[(DP + 63) / 64];
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
-            const int row = row0 + r0 + i;
-            qs[(r0 + i) * pitch + d] = i < nr && d < D ? to_f32(q[(size_t)(sg.q_begin + row / G) * ld + (size_t)(kvh * G + row % G) * D + d]) : 0.f;
+        for (int u = 0; u < (DP + 63) / 64; ++u) {
+            const int d = 2 * lane + 64 * u;
+            x[u] = make_float2(r < rows && d < D ? to_f32(src[d]) : 0.f, r < rows && d + 1 < D ? to_f32(src[d + 1]) : 0.f);
         }
+#pragma unroll
+        for (int u = 0; u < (DP + 63) / 64; ++u) {
+            const int d = 2 * lane + 64 * u;
+            if (d >= DP) continue;
+            unsigned* to = reinterpret_cast<unsigned*>(qs + r * S::QPITCH + d);
+            if (F32) {
+                const Parts p = split(x[u].x, x[u].y);
+                to[0] = p.h;
+                to[MROWS * S::QPITCH / 2] = p.m;
+                to[MROWS * S::QPITCH] = p.l;
+            } else {
+                to[0] = pack_bf16(x[u].x, x[u].y);
+            }
+        }
+    }
     __syncthreads();
-    if (tid < rows) {
+    fetch(ks, S::KPITCH, kpool, sg.jt0 + t0);
+    if (tid < MROWS) {
         unsigned line[TREE_WORDS];
-        depths[tid] = tree_line(parent, (row0 + tid) / G, window, line);
+        const int depth = tree_line(parent, tid < rows ? (row0 + tid) / G : 0, window, line);
+        lows[tid] = tid < rows ? (window > 0 ? max(0, sg.c + depth - window + 1) : 0) : sg.hi + 1;
 #pragma unroll
-        for (int w = 0; w < TREE_WORDS; ++w) lines[tid][w] = line[w];
+        for (int w = 0; w < TREE_WORDS; ++w) lines[tid][w] = tid < rows ? line[w] : 0u;
     }
-    __syncthreads();
-    int lo[RW];
-    float m[RW], l[RW], acc[RW][4 * NC];
+    auto sees = [&](int r, int j) { return j <= sg.hi && (j < sg.c ? j >= lows[r] : (line_bits(lines[r], (j & ~31) - sg.c) >> (j & 31)) & 1u); };
+    // Sets to zero what the products cannot take in a tile, and notes the keys.
+    auto clean = [&](TA* tile, int pitch, unsigned* odd) {
+        constexpr int PIECE_COLS = DP / PER16;
+        for (int i = tid; i < KEY_TILE * PIECE_COLS; i += MTHREADS) {
+            const int r = i / PIECE_COLS;
+            TA* at = tile + r * pitch + (i % PIECE_COLS) * PER16;
+            const uint4 raw = *reinterpret_cast<const uint4*>(at);
+            TA v[PER16];
+            *reinterpret_cast<uint4*>(v) = raw;
+            bool any = false;
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        lo[i] = window > 0 && i < nr ? max(0, sg.c + depths[r0 + i] - window + 1) : 0;
-        m[i] = -INFINITY;
-        l[i] = 0.f;
+            for (int e = 0; e < PER16; ++e) any = any || is_odd(v[e]);
+            if (any) {
 #pragma unroll
-        for (int c = 0; c < 4 * NC; ++c) acc[i][c] = 0.f;
-    }
-    int buf = 0;
-    for (int j0 = j_begin; j0 < j_end; j0 += SKEYS, buf ^= 1) {
-        asm volatile("cp.async.wait_group 0;\n" ::);
-        __syncthreads();                                               // this tile is there, and the one before it has been used
-        if (j0 + SKEYS < j_end) fetch(j0 + SKEYS, buf ^ 1);
-        if (nr <= 0) continue;
-        const float* ks = tiles + buf * 2 * SKEYS * pitch;
-        const float* vs = ks + SKEYS * pitch;
-        const int j = j0 + lane;
-        float dot[RW];
-#pragma unroll
-        for (int i = 0; i < RW; ++i) dot[i] = 0.f;
-        const float* kr = ks + lane * pitch;
-        const float* qr = qs + r0 * pitch;
-#pragma unroll 4
-        for (int d = 0; d < D4; d += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(kr + d);
-#pragma unroll
-            for (int i = 0; i < RW; ++i) {
-                const float4 q4 = *reinterpret_cast<const float4*>(qr + i * pitch + d);
-                dot[i] = fmaf(q4.x, k4.x, dot[i]);
-                dot[i] = fmaf(q4.y, k4.y, dot[i]);
-                dot[i] = fmaf(q4.z, k4.z, dot[i]);
-                dot[i] = fmaf(q4.w, k4.w, dot[i]);
+                for (int e = 0; e < PER16; ++e) if (is_odd(v[e])) at[e] = from_f32<TA>(0.f);
+                atomicOr(&odd[r >> 5], 1u << (r & 31));
             }
         }
-        float pj[RW];
-        unsigned vis[RW];
-        bool all = true;
+    };
+    const int rt = 16 * (warp & 1), part = warp >> 1;                  // a warp's rows, and its block of keys or columns
+    const int g = lane >> 2, t4 = lane & 3;
+    const int r_a = rt + (lane & 7) + ((lane >> 3) & 1) * 8, c_a = 8 * (lane >> 4);      // a lane's row and column of a first operand's ldmatrix
+    float m[4], l[4], o[NT][4];                                        // m, l: of rows 4 warp ..+ 3
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
-            vis[i] = 0u;
-            pj[i] = 0.f;
-            if (i >= nr) continue;
-            const bool valid = j < j_end && (j < sg.c ? j >= lo[i] : (line_bits(lines[r0 + i], j0 - sg.c) >> lane) & 1u);
-            vis[i] = __ballot_sync(0xffffffffu, valid);
-            all = all && vis[i] == 0xffffffffu;
-            if (vis[i] == 0u) continue;
-            float s = -INFINITY;
-            if (valid) {
-                s = dot[i] * scale;
-                if (softcap > 0.f) s = softcap * tanhf(s / softcap);
-            }
-            const float m_new = fmaxf(m[i], warp_max(s)), ref = m_new == -INFINITY ? 0.f : m_new;
-            pj[i] = valid ? expf(s - ref) : 0.f;
-            const float alpha = expf(m[i] - ref);                      // m = -inf on the first tile gives 0
-            l[i] = l[i] * alpha + warp_sum(pj[i]);
+    for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
 #pragma unroll
-            for (int c = 0; c < 4 * NC; ++c) acc[i][c] *= alpha;
-            m[i] = m_new;
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    for (int t = t0; t < t1; ++t) {
+        const int jt = sg.jt0 + t, j0 = jt * KEY_TILE;
+        const bool whole = j0 + KEY_TILE - 1 < sg.c && (window <= 0 || j0 > sg.c + sg.n - 1 - window);
+        const bool look = F32 || !whole;                               // for values that the products cannot take
+        fetch(vs, S::VPITCH, vpool, jt);                               // the last reader passed the barrier behind the outputs
+        asm volatile("cp.async.wait_group 1;\n" ::);
+        __syncthreads();                                               // the keys are there
+        if (F32) {
+            clean(ks, S::KPITCH, odd_keys);
+            __syncthreads();
         }
-#pragma unroll 4
-        for (int jj = 0; jj < SKEYS; ++jj) {
-            float4 v4[NC];
+        {
+            float big[2][4] = {}, rest[2][4] = {};
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-                v4[c] = 4 * lane + 128 * c < D4 ? *reinterpret_cast<const float4*>(vs + jj * pitch + 4 * lane + 128 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < K16; ++k) {
+                unsigned ah[4], am[4], al[4];
+                ldsm(ah, qs + r_a * S::QPITCH + 16 * k + c_a);
+                if (F32) {
+                    ldsm(am, qs + (MROWS + r_a) * S::QPITCH + 16 * k + c_a);
+                    ldsm(al, qs + (2 * MROWS + r_a) * S::QPITCH + 16 * k + c_a);
 #pragma unroll
-            for (int i = 0; i < RW; ++i) {
-                const float p = __shfl_sync(0xffffffffu, pj[i], jj);
-                if (!all && !((vis[i] >> jj) & 1u)) continue;          // uniform over the warp
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    acc[i][4 * c] = fmaf(p, v4[c].x, acc[i][4 * c]);
-                    acc[i][4 * c + 1] = fmaf(p, v4[c].y, acc[i][4 * c + 1]);
-                    acc[i][4 * c + 2] = fmaf(p, v4[c].z, acc[i][4 * c + 2]);
-                    acc[i][4 * c + 3] = fmaf(p, v4[c].w, acc[i][4 * c + 3]);
+                    for (int n = 0; n < 2; ++n) {
+                        const float* at = reinterpret_cast<const float*>(ks) + (16 * part + 8 * n + g) * S::KPITCH + 16 * k + 2 * t4;
+                        const float2 x = *reinterpret_cast<const float2*>(at), y = *reinterpret_cast<const float2*>(at + 8);
+                        mma_parts(big[n], rest[n], ah, am, al, split(x.x, x.y), split(y.x, y.y));
+                    }
+                } else {
+                    unsigned b[4];
+                    ldsm(b, ks + (16 * part + ((lane >> 4) << 3) + (lane & 7)) * S::KPITCH + 16 * k + 8 * ((lane >> 3) & 1));
+                    mma16(big[0], ah, b[0], b[1]);
+                    mma16(big[1], ah, b[2], b[3]);
                 }
             }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float2*>(ss + (rt + g + 8 * h) * SP + 16 * part + 8 * n + 2 * t4) =
+                        make_float2(big[n][2 * h] + rest[n][2 * h], big[n][2 * h + 1] + rest[n][2 * h + 1]);
         }
+        if (t + 1 < t1) locate(jt + 1);
+        __syncthreads();                                               // scores are there, the keys have been used
+        if (t + 1 < t1) fetch(ks, S::KPITCH, kpool, jt + 1);
+        else asm volatile("cp.async.commit_group;\n" ::);
+        if (F32 && (odd_keys[0] | odd_keys[1])) {                      // these keys' scores, from the operands themselves
+            for (unsigned long long w = odd_keys[0] | ((unsigned long long)odd_keys[1] << 32); w != 0ull; w &= w - 1ull) {
+                const int r = __ffsll((long long)w) - 1;
+                const TA* key = kpool + max(where[jt & 1][r], 0ll);
+                if (tid < rows) {
+                    const TA* query = q_row(tid);
+                    float sum = 0.f;
+                    for (int d = 0; d < D; ++d) sum = fmaf(to_f32(query[d]), to_f32(key[d]), sum);
+                    ss[tid * SP + r] = sum;
+                }
+            }
+            __syncthreads();
+            if (tid < 2) odd_keys[tid] = 0u;
+        }
+        {
+            float x[2][4];
+            unsigned vis[2] = {0xfu, 0xfu};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = 4 * warp + i;
+                    x[u][i] = ss[r * SP + lane + 32 * u] * scale;
+                    if (softcap > 0.f) x[u][i] = softcap * tanhf(x[u][i] / softcap);
+                    if (!whole && !sees(r, j0 + lane + 32 * u)) { x[u][i] = -INFINITY; vis[u] &= ~(1u << i); }
+                }
+            float a4[4], top[4], sum[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = fmaxf(x[0][i], x[1][i]);
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], w));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float m_new = fmaxf(m[i], top[i]), ref = m_new == -INFINITY ? 0.f : m_new;
+                a4[i] = expf(m[i] - ref);                              // m = -inf on the first tile gives 0
+                x[0][i] = (vis[0] >> i) & 1u ? expf(x[0][i] - ref) : 0.f;
+                x[1][i] = (vis[1] >> i) & 1u ? expf(x[1][i] - ref) : 0.f;
+                sum[i] = x[0][i] + x[1][i];
+                m[i] = m_new;
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                l[i] = l[i] * a4[i] + sum[i];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int at = (4 * warp + i) * SP + lane + 32 * u;
+                    ss[at] = x[u][i];
+                    if (!F32) ps[at] = __float2bfloat16_rn(x[u][i]);
+                }
+            }
+            if (lane < 4) s_alpha[4 * warp + lane] = lane == 0 ? a4[0] : lane == 1 ? a4[1] : lane == 2 ? a4[2] : a4[3];
+        }
+        asm volatile("cp.async.wait_group 1;\n" ::);
+        __syncthreads();                                               // probabilities and values are there
+        if (look) {
+            clean(vs, S::VPITCH, odd_values);
+            __syncthreads();
+        }
+        {
+            float tile[NT][4] = {}, rest[F32 ? NT : 1][4] = {};
+            const int col0 = part * (DP / 4);                          // a warp's quarter of the columns
+#pragma unroll
+            for (int k = 0; k < KEY_TILE / 16; ++k) {
+                if (F32) {
+                    Parts a[4];                                        // rows g and g + 8, keys 2 t4 and 2 t4 + 8
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 p = *reinterpret_cast<const float2*>(ss + (rt + g + 8 * (i & 1)) * SP + 16 * k + 2 * t4 + 8 * (i >> 1));
+                        a[i] = split(p.x, p.y);
+                    }
+                    const unsigned ah[4] = {a[0].h, a[1].h, a[2].h, a[3].h}, am[4] = {a[0].m, a[1].m, a[2].m, a[3].m}, al[4] = {a[0].l, a[1].l, a[2].l, a[3].l};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float* at = reinterpret_cast<const float*>(vs) + (16 * k + 2 * t4) * S::VPITCH + col0 + 8 * n + g;
+                        const Parts b0 = split(at[0] * UP, at[S::VPITCH] * UP), b1 = split(at[8 * S::VPITCH] * UP, at[9 * S::VPITCH] * UP);
+                        mma_parts(tile[n], rest[F32 ? n : 0], ah, am, al, b0, b1);
+                    }
+                } else {
+                    unsigned a[4];
+                    ldsm(a, ps + r_a * SP + 16 * k + c_a);
+                    const bf16* at = reinterpret_cast<const bf16*>(vs) + (16 * k + (lane & 7) + ((lane >> 3) & 1) * 8) * S::VPITCH + col0;
+                    if (NT == 1) {                                     // one block: the other half of the four matrices is not used
+                        unsigned b[4];
+                        ldsm_trans(b, at);
+                        mma16(tile[0], a, b[0], b[1]);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n + 1 < NT; n += 2) {
+                            unsigned b[4];
+                            ldsm_trans(b, at + 8 * n + c_a);
+                            mma16(tile[n], a, b[0], b[1]);
+                            mma16(tile[n + 1], a, b[2], b[3]);
+                        }
+                    }
+                }
+            }
+            const float al0 = s_alpha[rt + g], al1 = s_alpha[rt + g + 8];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    o[n][e] = fmaf(o[n][e], e < 2 ? al0 : al1, F32 ? (tile[n][e] + rest[F32 ? n : 0][e]) * DOWN : tile[n][e]);
+            if (look && (odd_values[0] | odd_values[1])) {             // values that the products left out, for the rows that see them
+                for (unsigned long long w = odd_values[0] | ((unsigned long long)odd_values[1] << 32); w != 0ull; w &= w - 1ull) {
+                    const int r = __ffsll((long long)w) - 1;
+                    const TA* value = vpool + max(where[jt & 1][r], 0ll);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int row = rt + g + 8 * (e >> 1), d = col0 + 8 * n + 2 * t4 + (e & 1);
+                            if (d < D && is_odd(value[d]) && (whole || sees(row, j0 + r))) o[n][e] = fmaf(ss[row * SP + r], to_f32(value[d]), o[n][e]);
+                        }
+                }
+                __syncthreads();
+                if (tid < 2) odd_values[tid] = 0u;
+            }
+        }
+        __syncthreads();                                               // the values have been used
     }
+    pdl_trigger_late();
+    if (lane < 4) {
+        s_m[4 * warp + lane] = lane == 0 ? m[0] : lane == 1 ? m[1] : lane == 2 ? m[2] : m[3];
+        s_l[4 * warp + lane] = lane == 0 ? l[0] : lane == 1 ? l[1] : lane == 2 ? l[2] : l[3];
+    }
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        if (i >= nr) continue;
-        const int row = row0 + r0 + i, h = kvh * G + row % G;
-        const size_t at = (size_t)(sg.q_begin + row / G) * Hq + h;
+    for (int hh = 0; hh < 2; ++hh) {
+        const int r = rt + g + 8 * hh, row = row0 + r;
+        if (r >= rows) continue;
+        const int h = kvh * G + row % G;
+        const size_t at = (size_t)(sg.q_begin + row / G) * Hq + h, slot = (size_t)sp * total_rows * Hq + at;
+        float total = s_l[r];
         if (sg.n_split > 1) {
-            const size_t slot = (size_t)split * total_rows * Hq + at;
-            if (lane == 0) {
-                part_ml[2 * slot] = m[i] * LOG2E;                      // in units of log2, as the merge takes it
-                part_ml[2 * slot + 1] = l[i];
+            if (part == 0 && t4 == 0) {
+                part_ml[2 * slot] = s_m[r] * LOG2E;                    // in units of log2, as the merge takes it
+                part_ml[2 * slot + 1] = total;
             }
-#pragma unroll
-            for (int c = 0; c < 4 * NC; ++c) {
-                const int d = 4 * lane + 128 * (c >> 2) + (c & 3);
-                if (d < D) part_o[slot * D + d] = acc[i][c];
-            }
-        } else {
-            if (sink != nullptr) l[i] += m[i] == -INFINITY ? 1.f : expf(sink[h] - m[i]);
-            const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
-#pragma unroll
-            for (int c = 0; c < 4 * NC; ++c) {
-                const int d = 4 * lane + 128 * (c >> 2) + (c & 3);
-                if (d < D) out[at * D + d] = from_f32<TA>(acc[i][c] * inv);
-            }
+        } else if (sink != nullptr) {
+            total += s_m[r] == -INFINITY ? 1.f : expf(sink[h] - s_m[r]);
         }
+        const float inv = total == 0.f ? 0.f : 1.0f / total;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = part * (DP / 4) + 8 * n + 2 * t4 + e;
+                if (d >= D) continue;
+                if (sg.n_split > 1) part_o[slot * D + d] = o[n][2 * hh + e];
+                else out[at * D + d] = from_f32<TA>(o[n][2 * hh + e] * inv);
+            }
     }
 }
 
@@ -329,10 +534,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ void cp16u(unsigned smem_addr, const void* gmem, bool pred) {
     const int bytes = pred ? 16 : 0;          // 0: nothing is read, the 16 bytes become zero
@@ -804,44 +1005,76 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     if (warp == 8) tmem_dealloc(tmem, S::TMEM_COLS);
 }
 
-// out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).
-// grid: (nodes of the longest tree x Hq / 8, segments).
-template <typename TA>
+// out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).  All
+// maxima and sums are asked for at once (a lane a share), then the shares' rows eight at a time: about two trips to memory.
+// grid: (nodes of the longest tree x Hq / 8, segments).  VEC: values of a row that lie together in a lane.
+template <typename TA, int VEC>
 __global__ void __launch_bounds__(256)
 tree_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ cu_q,
                   const int* __restrict__ seg_pos0, int total_rows, int Hq, int D, int window, int share, int max_split,
                   TA* __restrict__ out, const float* __restrict__ sink) {
+    constexpr int RUNS = TREE_MAX_D / 32 / VEC, AT_ONCE = VEC == 4 ? 8 : 2;      // VEC 4: heads up to 128
+    constexpr int USED = VEC == 4 ? 1 : RUNS;
     pdl_wait();
     const Segment sg(cu_q, seg_pos0, blockIdx.y, window, share, max_split);
     const int pair = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (pair >= sg.n * Hq || sg.n_split == 1) return;         // one share: its CTA wrote the row
     const int h = pair % Hq;
     const size_t at = (size_t)sg.q_begin * Hq + pair, stride = (size_t)total_rows * Hq;
-    float top = -INFINITY;
-    for (int s = 0; s < sg.n_split; ++s) top = fmaxf(top, part_ml[2 * (s * stride + at)]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float l = sink != nullptr ? exp2f(sink[h] * LOG2E - ref) : 0.f;
-    float acc[TREE_MAX_D / 32];
+    static_assert(TREE_MAX_SPLITS <= 64, "two shares a lane");
+    float2 ml[2];
 #pragma unroll
-    for (int i = 0; i < TREE_MAX_D / 32; ++i) acc[i] = 0.f;
-    for (int s = 0; s < sg.n_split; ++s) {
-        const size_t slot = s * stride + at;
-        const float ls = part_ml[2 * slot + 1];
-        if (ls == 0.f) continue;                              // a share without keys for this row left no output
-        const float w = exp2f(part_ml[2 * slot] - ref);
-        l += ls * w;
+    for (int u = 0; u < 2; ++u)
+        ml[u] = lane + 32 * u < sg.n_split ? *reinterpret_cast<const float2*>(part_ml + 2 * ((lane + 32 * u) * stride + at)) : make_float2(-INFINITY, 0.f);
+    const float top = warp_max(fmaxf(ml[0].x, ml[1].x)), ref = top == -INFINITY ? 0.f : top;
+    float w[2];                                               // a share without keys for this row left no output: weight 0, nothing is read
 #pragma unroll
-        for (int i = 0; i < TREE_MAX_D / 32; ++i) {
-            const int d = lane + 32 * i;
-            if (d < D) acc[i] += part_o[slot * D + d] * w;
+    for (int u = 0; u < 2; ++u) w[u] = ml[u].y == 0.f ? 0.f : exp2f(ml[u].x - ref);
+    float l = warp_sum(ml[0].y * w[0] + ml[1].y * w[1]);
+    if (sink != nullptr) l += exp2f(sink[h] * LOG2E - ref);
+    float acc[USED][VEC];
+#pragma unroll
+    for (int i = 0; i < USED; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[i][k] = 0.f;
+    for (int s0 = 0; s0 < sg.n_split; s0 += AT_ONCE) {
+        float o[AT_ONCE][USED][VEC], ws[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int s = s0 + u;
+            ws[u] = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+            if (s >= sg.n_split) ws[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < USED; ++i) {
+                const int d = VEC * (lane + 32 * i);
+                const float* from = part_o + (s * stride + at) * D + d;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) o[u][i][k] = 0.f;
+                if (ws[u] != 0.f && d < D) {
+                    if (VEC == 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(from);
+                        o[u][i][0] = f.x; o[u][i][VEC > 1 ? 1 : 0] = f.y; o[u][i][VEC > 2 ? 2 : 0] = f.z; o[u][i][VEC > 3 ? 3 : 0] = f.w;
+                    } else {
+                        o[u][i][0] = *from;
+                    }
+                }
+            }
         }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int i = 0; i < USED; ++i)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) acc[i][k] = ws[u] != 0.f ? fmaf(o[u][i][k], ws[u], acc[i][k]) : acc[i][k];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < TREE_MAX_D / 32; ++i) {
-        const int d = lane + 32 * i;
-        if (d < D) out[at * D + d] = from_f32<TA>(acc[i] * inv);
-    }
+    for (int i = 0; i < USED; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const int d = VEC * (lane + 32 * i) + k;
+            if (d < D) out[at * D + d] = from_f32<TA>(acc[i][k] * inv);
+        }
 }
 
 struct TreeCall {
@@ -866,26 +1099,28 @@ template <typename TA>
 int merge(const TreeCall& a) {
     if (a.splits <= 1) return 0;
     dim3 grid((a.max_nodes * a.Hq + 7) / 8, a.segments);
-    return rb_launch_pdl(tree_merge_kernel<TA>, grid, dim3(256), 0, a.st, a.scratch, a.part_ml(), a.cu_q, a.seg_pos0, a.total_rows, a.Hq, a.D,
+    return rb_launch_pdl(a.D % 4 == 0 && a.D <= 128 ? tree_merge_kernel<TA, 4> : tree_merge_kernel<TA, 1>, grid, dim3(256), 0, a.st, a.scratch, a.part_ml(), a.cu_q, a.seg_pos0, a.total_rows, a.Hq, a.D,
                          a.window, a.share, a.splits, (TA*)a.out, a.sink);
 }
 
-template <typename TA, int NC>
-int simt(const TreeCall& a) {
-    const size_t smem = (size_t)(SROWS + 4 * SKEYS) * (((a.D + 3) & ~3) + 4) * sizeof(float);
+template <typename TA, int DP>
+int mma_launch(const TreeCall& a) {
+    constexpr int SMEM = (int)MmaShape<TA, DP>::SMEM;
     static PerDevice configured;
-    const int rc = configured.once([&](int) {
-        return cudaFuncSetAttribute(tree_simt_kernel<TA, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)((SROWS + 4 * SKEYS) * (128 * NC + 4) * sizeof(float)));
-    });
+    const int rc = configured.once([&](int) { return cudaFuncSetAttribute(tree_mma_kernel<TA, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
     if (rc) return rc;
-    const int vec = sizeof(TA) == 4 && a.D % 4 == 0 && (((uintptr_t)a.kpool | (uintptr_t)a.vpool) & 15) == 0;
-    dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + SROWS - 1) / SROWS * a.Hkv, a.segments, a.splits);
-    tree_simt_kernel<TA, NC><<<grid, 32 * SW, smem, a.st>>>(
-        (const TA*)a.q, a.ld, (const TA*)a.kpool, (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size,
-        (TA*)a.out, a.scratch, a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, vec);
-    const int e = rb_launch_status();
+    const int vec = a.D * sizeof(TA) % 16 == 0 && (((uintptr_t)a.kpool | (uintptr_t)a.vpool) & 15) == 0;
+    dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + MROWS - 1) / MROWS * a.Hkv, a.segments, a.splits);
+    const int e = rb_launch_pdl(tree_mma_kernel<TA, DP>, grid, dim3(MTHREADS), SMEM, a.st, (const TA*)a.q, a.ld, (const TA*)a.kpool,
+                                (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, (TA*)a.out, a.scratch,
+                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, vec);
     return e ? e : merge<TA>(a);
+}
+template <typename TA>
+int mma_any(const TreeCall& a) {
+    if (a.D <= 32) return mma_launch<TA, 32>(a);
+    if (a.D <= 64) return mma_launch<TA, 64>(a);
+    return a.D <= 128 ? mma_launch<TA, 128>(a) : mma_launch<TA, 256>(a);
 }
 
 template <int D, bool STREAMS>
@@ -917,7 +1152,7 @@ RB_EXPORT int rb_tree_max_nodes() { return TREE_MAX_NODES; }
 
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys
 // go to one CTA for every `share` key tiles of 64, `splits` at most; scratch then holds splits * total_rows * Hq * (D + 2) floats.
-// query_tiles: 0 the CUDA cores; 1 or 2 the tensor cores with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, pools and
+// query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, pools and
 // queries on 16-byte boundaries, ld a multiple of 8).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
                                 const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
@@ -926,7 +1161,7 @@ RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const 
                                 cudaStream_t st) {
     if (segments <= 0 || max_nodes <= 0) return 0;
     if (segments > 65535 || max_nodes > TREE_MAX_NODES || D <= 0 || D > TREE_MAX_D || Hkv <= 0 || Hq % Hkv || page_size <= 0) return (int)cudaErrorInvalidValue;
-    if (splits < 1 || splits > 64 || (splits > 1 && (share <= 0 || scratch == nullptr))) return (int)cudaErrorInvalidValue;
+    if (splits < 1 || splits > TREE_MAX_SPLITS || (splits > 1 && (share <= 0 || scratch == nullptr))) return (int)cudaErrorInvalidValue;
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
                   D, pages, scale, window, softcap, sink, splits, share, (float*)scratch, status, st};
     if (query_tiles > 0) {
@@ -935,6 +1170,5 @@ RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const 
         if (D == 64) return query_tiles == 1 ? tc5_launch<64, true>(a) : tc5_launch<64, false>(a);
         return query_tiles == 1 ? tc5_launch<128, true>(a) : tc5_launch<128, false>(a);
     }
-    if (act_dtype == RB_F32) return D <= 128 ? simt<float, 1>(a) : simt<float, 2>(a);
-    return D <= 128 ? simt<bf16, 1>(a) : simt<bf16, 2>(a);
+    return act_dtype == RB_F32 ? mma_any<float>(a) : mma_any<bf16>(a);
 }

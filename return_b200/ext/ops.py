@@ -2244,7 +2244,7 @@ _tree = _branch = None
 TREE_MAX_NODES = 256               # drafted nodes of a segment
 TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
-TREE_MIN_SHARE = 4                 # a CTA of split keys walks at least so many tiles
+TREE_MIN_SHARE = 2                 # a CTA of split keys walks at least so many tiles
 TREE_MAX_SPLITS = 64
 TREE_SCRATCH_BYTES = 256 << 20
 
