@@ -68,15 +68,15 @@ __device__ __forceinline__ unsigned line_bits(const unsigned* line, int at) {
 }
 
 // ---------------------------------------------------------------------------------------- matrix instructions of a warp, any type and head size
-// A CTA of eight warps takes 32 rows and walks its keys in tiles of 64.  Scores: a warp 16 rows by 16 keys; softmax: a warp four rows, a lane two
-// keys; outputs: a warp 16 rows by a quarter of the columns, a tile's sum made by itself and added to the running one.  While the
+// A CTA of eight warps takes 32 rows and walks its keys in tiles of 64.  Scores: a warp 16 rows by 16 keys; softmax: eight lanes a row;
+// outputs: a warp 16 rows by a quarter of the columns, a tile's sum made by itself and added to the running one.  While the
 // scores are made the tile's values arrive, while the outputs are summed the next tile's keys.
 // bfloat16: operands as they are, probabilities rounded to bfloat16.  float32: an operand is split into three bfloat16 parts, which hold its 24
 // bits, as it is read (queries once), six of the nine products are made (the rest is below 2^-24 of a product), the largest in an accumulator
 // of its own; values are multiplied by 2^16 first, so that small ones keep their bits, and the sums by 2^-16.
-// Values that are no numbers (float32: or that 2^16 would take beyond them), of tiles that some row does not see in full in bfloat16 and of all
-// tiles in float32, are set to zero in shared memory (zero times infinity would reach every row), and added to the rows that see them from the
-// operands themselves; scores of float32 keys that have such elements are made again in the same way.
+// A product with a value that is no number reaches every row (zero times infinity), and float32's parts cannot hold one, nor one that 2^16 takes
+// beyond the numbers.  Where a float32 score is no finite number it is made again from the operands.  Where an output's sum over a tile is none,
+// such values are set to zero in shared memory, the tile's sums are made again, and the values are added for the rows that see them.
 constexpr int MROWS = 32, MTHREADS = 256;
 constexpr int SP = KEY_TILE + 8;              // floats of a row of scores: eight-byte reads of four rows by four lanes hit all banks
 constexpr float UP = 65536.f, DOWN = 1.f / UP;
@@ -95,8 +95,8 @@ __device__ __forceinline__ void ldsm_trans(unsigned (&r)[4], const void* p) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)));
 }
 __device__ __forceinline__ void mma16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 struct Parts { unsigned h, m, l; };           // of two neighbouring values, the first in the low half
 __device__ __forceinline__ Parts split(float x, float y) {
@@ -154,7 +154,7 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
     __shared__ unsigned lines[MROWS][TREE_WORDS];
     __shared__ long long where[2][KEY_TILE];
     __shared__ int lows[MROWS];                                        // a row's first key
-    __shared__ unsigned odd_keys[2], odd_values[2];                    // a tile's keys that have elements the products cannot take
+    __shared__ unsigned odd_keys[2];                                   // a tile's keys whose values the products cannot take
     __shared__ float s_alpha[MROWS], s_m[MROWS], s_l[MROWS];
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -197,34 +197,41 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
     };
     locate(sg.jt0 + t0);
     for (int i = tid; i < sg.n; i += MTHREADS) parent[i] = tree_parent[sg.q_begin + i];
-    if (tid < 2) odd_keys[tid] = odd_values[tid] = 0u;
+    if (tid < 2) odd_keys[tid] = 0u;
     for (int i = tid; i < KEY_TILE * (DP - D); i += MTHREADS) {        // behind the head size, for good
         const int r = i / (DP - D), d = D + i % (DP - D);
         ks[r * S::KPITCH + d] = vs[r * S::VPITCH + d] = from_f32<TA>(0.f);
     }
     // Queries, split: rows that do not exist are zero.
-    for (int r = warp; r < MROWS; r += MTHREADS / 32) {
-        const TA* src = q_row(r < rows ? r : 0);
-        float2 x[(DP + 63) / 64];
+    {
+        constexpr int QR = MROWS * 32 / MTHREADS, QU = (DP + 63) / 64;
+        float2 x[QR][QU];
 #pragma unroll
-        for (int u = 0; u < (DP + 63) / 64; ++u) {
-            const int d = 2 * lane + 64 * u;
-            x[u] = make_float2(r < rows && d < D ? to_f32(src[d]) : 0.f, r < rows && d + 1 < D ? to_f32(src[d + 1]) : 0.f);
-        }
+        for (int i = 0; i < QR; ++i) {
+            const int r = warp * QR + i;
+            const TA* src = q_row(r < rows ? r : 0);
 #pragma unroll
-        for (int u = 0; u < (DP + 63) / 64; ++u) {
-            const int d = 2 * lane + 64 * u;
-            if (d >= DP) continue;
-            unsigned* to = reinterpret_cast<unsigned*>(qs + r * S::QPITCH + d);
-            if (F32) {
-                const Parts p = split(x[u].x, x[u].y);
-                to[0] = p.h;
-                to[MROWS * S::QPITCH / 2] = p.m;
-                to[MROWS * S::QPITCH] = p.l;
-            } else {
-                to[0] = pack_bf16(x[u].x, x[u].y);
+            for (int u = 0; u < QU; ++u) {
+                const int d = 2 * lane + 64 * u;
+                x[i][u] = make_float2(r < rows && d < D ? to_f32(src[d]) : 0.f, r < rows && d + 1 < D ? to_f32(src[d + 1]) : 0.f);
             }
         }
+#pragma unroll
+        for (int i = 0; i < QR; ++i)
+#pragma unroll
+            for (int u = 0; u < QU; ++u) {
+                const int d = 2 * lane + 64 * u;
+                if (d >= DP) continue;
+                unsigned* to = reinterpret_cast<unsigned*>(qs + (warp * QR + i) * S::QPITCH + d);
+                if (F32) {
+                    const Parts p = split(x[i][u].x, x[i][u].y);
+                    to[0] = p.h;
+                    to[MROWS * S::QPITCH / 2] = p.m;
+                    to[MROWS * S::QPITCH] = p.l;
+                } else {
+                    to[0] = pack_bf16(x[i][u].x, x[i][u].y);
+                }
+            }
     }
     __syncthreads();
     fetch(ks, S::KPITCH, kpool, sg.jt0 + t0);
@@ -236,44 +243,18 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
         for (int w = 0; w < TREE_WORDS; ++w) lines[tid][w] = tid < rows ? line[w] : 0u;
     }
     auto sees = [&](int r, int j) { return j <= sg.hi && (j < sg.c ? j >= lows[r] : (line_bits(lines[r], (j & ~31) - sg.c) >> (j & 31)) & 1u); };
-    // Sets to zero what the products cannot take in a tile, and notes the keys.
-    auto clean = [&](TA* tile, int pitch, unsigned* odd) {
-        constexpr int PIECE_COLS = DP / PER16;
-        for (int i = tid; i < KEY_TILE * PIECE_COLS; i += MTHREADS) {
-            const int r = i / PIECE_COLS;
-            TA* at = tile + r * pitch + (i % PIECE_COLS) * PER16;
-            const uint4 raw = *reinterpret_cast<const uint4*>(at);
-            TA v[PER16];
-            *reinterpret_cast<uint4*>(v) = raw;
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < PER16; ++e) any = any || is_odd(v[e]);
-            if (any) {
-#pragma unroll
-                for (int e = 0; e < PER16; ++e) if (is_odd(v[e])) at[e] = from_f32<TA>(0.f);
-                atomicOr(&odd[r >> 5], 1u << (r & 31));
-            }
-        }
-    };
     const int rt = 16 * (warp & 1), part = warp >> 1;                  // a warp's rows, and its block of keys or columns
     const int g = lane >> 2, t4 = lane & 3;
     const int r_a = rt + (lane & 7) + ((lane >> 3) & 1) * 8, c_a = 8 * (lane >> 4);      // a lane's row and column of a first operand's ldmatrix
-    float m[4], l[4], o[NT][4];                                        // m, l: of rows 4 warp ..+ 3
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+    float m = -INFINITY, l = 0.f, o[NT][4];                            // m, l: of row 4 warp + lane / 8
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     for (int t = t0; t < t1; ++t) {
         const int jt = sg.jt0 + t, j0 = jt * KEY_TILE;
         const bool whole = j0 + KEY_TILE - 1 < sg.c && (window <= 0 || j0 > sg.c + sg.n - 1 - window);
-        const bool look = F32 || !whole;                               // for values that the products cannot take
         fetch(vs, S::VPITCH, vpool, jt);                               // the last reader passed the barrier behind the outputs
         asm volatile("cp.async.wait_group 1;\n" ::);
         __syncthreads();                                               // the keys are there
-        if (F32) {
-            clean(ks, S::KPITCH, odd_keys);
-            __syncthreads();
-        }
         {
             float big[2][4] = {}, rest[2][4] = {};
 #pragma unroll
@@ -307,73 +288,74 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
         __syncthreads();                                               // scores are there, the keys have been used
         if (t + 1 < t1) fetch(ks, S::KPITCH, kpool, jt + 1);
         else asm volatile("cp.async.commit_group;\n" ::);
-        if (F32 && (odd_keys[0] | odd_keys[1])) {                      // these keys' scores, from the operands themselves
-            for (unsigned long long w = odd_keys[0] | ((unsigned long long)odd_keys[1] << 32); w != 0ull; w &= w - 1ull) {
-                const int r = __ffsll((long long)w) - 1;
-                const TA* key = kpool + max(where[jt & 1][r], 0ll);
-                if (tid < rows) {
-                    const TA* query = q_row(tid);
-                    float sum = 0.f;
-                    for (int d = 0; d < D; ++d) sum = fmaf(to_f32(query[d]), to_f32(key[d]), sum);
-                    ss[tid * SP + r] = sum;
-                }
-            }
-            __syncthreads();
-            if (tid < 2) odd_keys[tid] = 0u;
-        }
         {
-            float x[2][4];
-            unsigned vis[2] = {0xfu, 0xfu};
+            // Softmax: eight lanes a row; lane i of them keys 4 i ..+ 3 and 32 + 4 i ..+ 3.
+            const int r = 4 * warp + (lane >> 3), key0 = 4 * (lane & 7);
+            float x[8];
+            auto key_of = [&](int e) { return key0 + (e & 3) + 8 * (e & 4); };
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int r = 4 * warp + i;
-                    x[u][i] = ss[r * SP + lane + 32 * u] * scale;
-                    if (softcap > 0.f) x[u][i] = softcap * tanhf(x[u][i] / softcap);
-                    if (!whole && !sees(r, j0 + lane + 32 * u)) { x[u][i] = -INFINITY; vis[u] &= ~(1u << i); }
-                }
-            float a4[4], top[4], sum[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) top[i] = fmaxf(x[0][i], x[1][i]);
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], w));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float m_new = fmaxf(m[i], top[i]), ref = m_new == -INFINITY ? 0.f : m_new;
-                a4[i] = expf(m[i] - ref);                              // m = -inf on the first tile gives 0
-                x[0][i] = (vis[0] >> i) & 1u ? expf(x[0][i] - ref) : 0.f;
-                x[1][i] = (vis[1] >> i) & 1u ? expf(x[1][i] - ref) : 0.f;
-                sum[i] = x[0][i] + x[1][i];
-                m[i] = m_new;
+            for (int u = 0; u < 2; ++u) {
+                const float4 f = *reinterpret_cast<const float4*>(ss + r * SP + key0 + 32 * u);
+                x[4 * u] = f.x; x[4 * u + 1] = f.y; x[4 * u + 2] = f.z; x[4 * u + 3] = f.w;
             }
+            if (F32) {                                                 // scores that are no finite number, from the operands
+                bool odd = false;
 #pragma unroll
-            for (int w = 16; w > 0; w >>= 1)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], w);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                l[i] = l[i] * a4[i] + sum[i];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int at = (4 * warp + i) * SP + lane + 32 * u;
-                    ss[at] = x[u][i];
-                    if (!F32) ps[at] = __float2bfloat16_rn(x[u][i]);
+                for (int e = 0; e < 8; ++e) odd = odd || !isfinite(x[e]);
+                if (odd && r < rows) {
+                    const TA* query = q_row(r);
+#pragma unroll 1
+                    for (int e = 0; e < 8; ++e) {
+                        const long long at = where[jt & 1][key_of(e)];
+                        if (isfinite(x[e]) || at < 0) continue;
+                        float sum = 0.f;
+#pragma unroll 1
+                        for (int d = 0; d < D; ++d) sum = fmaf(to_f32(query[d]), to_f32(kpool[at + d]), sum);
+                        x[e] = sum;
+                    }
                 }
             }
-            if (lane < 4) s_alpha[4 * warp + lane] = lane == 0 ? a4[0] : lane == 1 ? a4[1] : lane == 2 ? a4[2] : a4[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= scale;
+            if (softcap > 0.f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = softcap * tanhf(x[e] / softcap);
+            }
+            unsigned vis = 0xffu;
+            if (!whole) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!sees(r, j0 + key_of(e))) { x[e] = -INFINITY; vis &= ~(1u << e); }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+#pragma unroll
+            for (int w = 4; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = expf(m - ref);                         // m = -inf on the first tile gives 0
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (vis >> e) & 1u ? expf(x[e] - ref) : 0.f;
+            float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+            for (int w = 4; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            l = l * alpha + sum;
+            m = m_new;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                *reinterpret_cast<float4*>(ss + r * SP + key0 + 32 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                if (!F32)
+                    *reinterpret_cast<uint2*>(ps + r * SP + key0 + 32 * u) = make_uint2(pack_bf16(x[4 * u], x[4 * u + 1]), pack_bf16(x[4 * u + 2], x[4 * u + 3]));
+            }
+            if ((lane & 7) == 0) s_alpha[r] = alpha;
         }
         asm volatile("cp.async.wait_group 1;\n" ::);
         __syncthreads();                                               // probabilities and values are there
-        if (look) {
-            clean(vs, S::VPITCH, odd_values);
-            __syncthreads();
-        }
-        {
-            float tile[NT][4] = {}, rest[F32 ? NT : 1][4] = {};
-            const int col0 = part * (DP / 4);                          // a warp's quarter of the columns
+        float tile[NT][4];
+        bool redone = false;
+        const int col0 = part * (DP / 4);                              // a warp's quarter of the columns
+        while (true) {
+            float rest[F32 ? NT : 1][4] = {};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) tile[n][0] = tile[n][1] = tile[n][2] = tile[n][3] = 0.f;
 #pragma unroll
             for (int k = 0; k < KEY_TILE / 16; ++k) {
                 if (F32) {
@@ -409,34 +391,52 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
                     }
                 }
             }
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (F32) tile[n][e] = (tile[n][e] + rest[F32 ? n : 0][e]) * DOWN;
+                    odd = odd || !isfinite(tile[n][e]);
+                }
+            if (redone || !__syncthreads_or(odd)) break;               // the values have been used
+            for (int i = tid; i < KEY_TILE * D; i += MTHREADS) {
+                TA* at = vs + (i / D) * S::VPITCH + i % D;
+                if (is_odd(*at)) {
+                    *at = from_f32<TA>(0.f);
+                    atomicOr(&odd_keys[i / D >> 5], 1u << (i / D & 31));
+                }
+            }
+            __syncthreads();
+            redone = true;
+        }
+        {
             const float al0 = s_alpha[rt + g], al1 = s_alpha[rt + g + 8];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o[n][e] = fmaf(o[n][e], e < 2 ? al0 : al1, F32 ? (tile[n][e] + rest[F32 ? n : 0][e]) * DOWN : tile[n][e]);
-            if (look && (odd_values[0] | odd_values[1])) {             // values that the products left out, for the rows that see them
-                for (unsigned long long w = odd_values[0] | ((unsigned long long)odd_values[1] << 32); w != 0ull; w &= w - 1ull) {
-                    const int r = __ffsll((long long)w) - 1;
-                    const TA* value = vpool + max(where[jt & 1][r], 0ll);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int row = rt + g + 8 * (e >> 1), d = col0 + 8 * n + 2 * t4 + (e & 1);
-                            if (d < D && is_odd(value[d]) && (whole || sees(row, j0 + r))) o[n][e] = fmaf(ss[row * SP + r], to_f32(value[d]), o[n][e]);
-                        }
-                }
-                __syncthreads();
-                if (tid < 2) odd_values[tid] = 0u;
-            }
+                for (int e = 0; e < 4; ++e) o[n][e] = fmaf(o[n][e], e < 2 ? al0 : al1, tile[n][e]);
         }
-        __syncthreads();                                               // the values have been used
+        if (redone) {                                                  // what the products left out
+            for (unsigned long long w = odd_keys[0] | ((unsigned long long)odd_keys[1] << 32); w != 0ull; w &= w - 1ull) {
+                const int key = __ffsll((long long)w) - 1;
+                const TA* value = vpool + max(where[jt & 1][key], 0ll);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = rt + g + 8 * (e >> 1), d = col0 + 8 * n + 2 * t4 + (e & 1);
+                        if (d < D && is_odd(value[d]) && (whole || sees(r, j0 + key))) o[n][e] = fmaf(ss[r * SP + key], to_f32(value[d]), o[n][e]);
+                    }
+            }
+            __syncthreads();
+            if (tid < 2) odd_keys[tid] = 0u;
+        }
     }
     pdl_trigger_late();
-    if (lane < 4) {
-        s_m[4 * warp + lane] = lane == 0 ? m[0] : lane == 1 ? m[1] : lane == 2 ? m[2] : m[3];
-        s_l[4 * warp + lane] = lane == 0 ? l[0] : lane == 1 ? l[1] : lane == 2 ? l[2] : l[3];
+    if ((lane & 7) == 0) {
+        s_m[4 * warp + (lane >> 3)] = m;
+        s_l[4 * warp + (lane >> 3)] = l;
     }
     __syncthreads();
 #pragma unroll
