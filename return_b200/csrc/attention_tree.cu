@@ -44,6 +44,19 @@ struct Segment {
     }
 };
 
+// x / G and x % G for the rows of a CTA: a quotient by the reciprocal, put right where it is one off.
+struct ByGroup {
+    int G;
+    float inv;
+    __device__ __forceinline__ explicit ByGroup(int g) : G(g), inv(1.0f / (float)g) {}
+    __device__ __forceinline__ int2 operator()(int x) const {
+        int q = (int)((float)x * inv), r = x - q * G;
+        if (r < 0) { --q; r += G; }
+        if (r >= G) { ++q; r -= G; }
+        return make_int2(q, r);
+    }
+};
+
 // The node's own line: bit a of `line` for node x itself and its ancestors less than `window` steps up (window <= 0: all); returns
 // the node's depth.  parent: the segment's list in shared memory.
 __device__ __forceinline__ int tree_line(const int* parent, int x, int window, unsigned (&line)[TREE_WORDS]) {
@@ -470,8 +483,10 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
 // bfloat16, head sizes 64 and 128.  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
 // tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
-//   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn, each with a maximum, sum and output of its own,
-//                  joined at the end;
+//   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn.  With 64 rows or fewer the tile holds them twice, with
+//                  32 four times, and of a key tile each copy's warps take a half or a quarter (their P is zero elsewhere): a row's thread has
+//                  to sit on the warp of its tensor-memory lane, and this way all four have exponentials to make.  Every copy of either group
+//                  has a maximum, sum and output of its own; they are joined at the end;
 //   else           up to 256 rows: a query tile of 128 rows a group, both go through every key tile.
 // Per key tile and group:
 //   S = Q K^T      tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a group;
@@ -492,6 +507,8 @@ constexpr int QM = 128;                       // rows of a query tile
 constexpr int KN = KEY_TILE;
 constexpr float RESCALE_STEP = 8.0f;          // log2 units the true maximum may run ahead of the reference
 
+template <int N> struct Width { static constexpr int value = N; };
+
 template <int D, bool STREAMS> struct Shape {
     static constexpr int NQ = STREAMS ? 1 : 2;               // query tiles
     static constexpr int DS = D / 64;         // 64-wide slabs of the head size
@@ -506,6 +523,7 @@ template <int D, bool STREAMS> struct Shape {
     static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 4 * P_BYTES + TAIL;
     static constexpr unsigned SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;       // one CTA an SM: it takes all of the tensor memory
     static_assert(SMEM <= 227 * 1024 && O_COL + 2 * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
+    static_assert(2 * STAGES * K_BYTES + 4 * P_BYTES >= 2 * QM * D * 4, "room for the outputs behind Q");
     static_assert(!STREAMS || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
 };
 
@@ -592,43 +610,64 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const int jt_begin = sg.jt0 + t0, n_tiles = t1 - t0;      // one tile at least
     const int* bt_row = block_table + (size_t)seg * bt_stride;
     const Paging pg(page_size);
+    const ByGroup by_group(G);
     const unsigned bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
+    // STREAMS: the query tile holds its rows `copies` times, copy_rows rows each
+    const int copy_rows = rows > 64 ? 128 : rows > 32 ? 64 : 32, copies = STREAMS ? QM / copy_rows : 1;
     // a group's rows (as warps), its key tiles, and the number of its i-th among the CTA's
-    auto active_warps = [&](int g) { return max(0, min(4, (rows - (STREAMS ? 0 : g * QM) + 31) >> 5)); };
+    auto active_warps = [&](int g) { return STREAMS && copies > 1 ? 4 : max(0, min(4, (rows - (STREAMS ? 0 : g * QM) + 31) >> 5)); };
     auto tiles_of = [&](int g) { return STREAMS ? (n_tiles - g + 1) >> 1 : active_warps(g) > 0 ? n_tiles : 0; };
     auto tile_no = [&](int g, int i) { return STREAMS ? 2 * i + g : i; };
     // whether every row sees every key of a tile
     auto whole = [&](int j_base) { return j_base + KN - 1 < sg.c && (window <= 0 || j_base > sg.c + sg.n - 1 - window); };
 
-    if (warp == 8) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
-    if (tid == 0) {
-        for (int i = 0; i < S::N_BARS; ++i) {
-            int count = 1;
-            if (i >= S::B_K_EMPTY && i < S::B_S) count = !STREAMS && rows > QM ? 2 : 1;       // the groups that read a key tile
-            else if (i >= S::B_P && i < S::B_PV) count = max(1, active_warps((i - S::B_P) >> 1));
-            else if (i >= S::B_Q && i < S::B_V_LAND) count = max(1, active_warps(i - S::B_Q));
-            mbar_init(bar(i), count);
+    // Everything that waits for memory is asked for before the barrier: queries, parents, the loaders' first pages.
+    constexpr int LPR = D / 8, RPI = 32 / LPR;                // lanes a row of 16-byte pieces, rows an instruction
+    const int rsel = lane / LPR, sub = lane % LPR;
+    if (warp < 8 && (!STREAMS || warp < 4) && (warp & 3) < active_warps(warp >> 2)) {
+        unsigned char* tile = sQ + (STREAMS ? 0 : warp >> 2) * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
+#pragma unroll 4
+        for (int i = 0; i < 32 / RPI; ++i) {                  // a row's pieces by neighbouring lanes
+            const int rt = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + (STREAMS ? rt & (copy_rows - 1) : (warp >> 2) * QM + rt);
+            const bool there = rr - row0 < rows;
+            const int2 nh = by_group(rr);
+            const bf16* src = q + (there ? (size_t)(sg.q_begin + nh.x) * ld + (size_t)(kvh * G + nh.y) * D + sub * 8 : 0);
+            cp16u(smem_u32(tile + sw128_offset(rt, sub & 7)), src, there);
         }
-        mbar_init_fence();
-        *odd_values = 0;
     }
+    asm volatile("cp.async.commit_group;\n" ::);
     for (int i = tid; i < sg.n; i += S::THREADS) parent[i] = tree_parent[sg.q_begin + i];
+    const int box = min(pg.page_size, KN), pi = lane / S::DS, slab = lane % S::DS;       // a loader's lane by TMA: page of the tile, slab
+    auto in_sight = [&](int jt) { const int j = jt * KN + pi * box; return pi * box < KN && j + box > sg.lo && j <= sg.hi; };
+    auto ask_page = [&](int jt) { return in_sight(jt) ? bt_row[pg.block(jt * KN + pi * box)] : -1; };
+    int next = warp >= 12 && by_tma ? ask_page(jt_begin) : -1;
+    if (warp == 8) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
+    if (tid < S::N_BARS) {
+        const int i = tid;
+        int count = 1;
+        if (i >= S::B_K_EMPTY && i < S::B_S) count = !STREAMS && rows > QM ? 2 : 1;           // the groups that read a key tile
+        else if (i >= S::B_P && i < S::B_PV) count = max(1, active_warps((i - S::B_P) >> 1));
+        else if (i >= S::B_Q && i < S::B_V_LAND) count = max(1, active_warps(i - S::B_Q));
+        mbar_init(bar(i), count);
+        mbar_init_fence();
+    }
+    if (tid == 0) *odd_values = 0;
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
     const unsigned tmem = *tmem_slot;
     bool ok = true;
 
-    constexpr int LPR = D / 8, RPI = 32 / LPR;                // lanes a row of 16-byte pieces, rows an instruction
-    const int rsel = lane / LPR, sub = lane % LPR;
     const int grp = warp < 8 ? warp >> 2 : ((warp - 8) >> 1) & 1;              // group of a row warp or an issuer
     const int qt = STREAMS ? 0 : grp, n_mine = tiles_of(grp);
     const bool has_rows = warp < 8 && (warp & 3) < active_warps(grp);
-    const int r = (warp & 3) * 32 + lane, row = row0 + qt * QM + r;            // a row thread's row of the tile, of the segment and head
-    const bool row_valid = has_rows && row - row0 < rows;
-    const size_t token = (size_t)sg.q_begin + (row_valid ? row / G : 0);
-    const int h = kvh * G + (row_valid ? row % G : 0);
+    // a row thread's row of the tile (its lane of tensor memory), its copy, its row in the CTA, of the segment and head
+    const int r = (warp & 3) * 32 + lane, copy = STREAMS ? r / copy_rows : 0, in_cta = STREAMS ? r & (copy_rows - 1) : qt * QM + r, row = row0 + in_cta;
+    const bool row_valid = has_rows && in_cta < rows;
+    const int2 node_head = by_group(row_valid ? row : 0);
+    const size_t token = (size_t)sg.q_begin + node_head.x;
+    const int h = kvh * G + node_head.y;
     const float scale_log2 = scale * LOG2E, scale_eff = softcap > 0.f ? softcap * LOG2E : scale_log2;
     unsigned line[TREE_WORDS];
     int lo_r = 0;
@@ -641,23 +680,15 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     };
     const unsigned lane_addr = tmem + ((unsigned)((warp & 3) * 32) << 16);
     const unsigned o_addr = lane_addr + S::O_COL + grp * D;
-    // a row's maximum and sum of a group, in that group's P, which none of its products reads any more by then
-    auto joined = [&](int g) { return reinterpret_cast<float2*>(sP + g * 2 * S::P_BYTES) + r; };
 
     if (has_rows) {
-        // ================================================================== one row per thread
-        if (!STREAMS || grp == 0) {
-            unsigned char* tile = sQ + qt * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
-#pragma unroll 1
-            for (int i = 0; i < 32 / RPI; ++i) {              // a row's pieces by neighbouring lanes
-                const int rt = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + qt * QM + rt;
-                const bool there = rr - row0 < rows;
-                const bf16* src = q + (there ? (size_t)(sg.q_begin + rr / G) * ld + (size_t)(kvh * G + rr % G) * D + sub * 8 : 0);
-                cp16u(smem_u32(tile + sw128_offset(rt, sub & 7)), src, there);
-            }
-            asm volatile("cp.async.commit_group;\n" ::);
+        // ================================================================== one row per thread, W keys of a tile
+        unsigned char* myPs = sP + grp * 2 * S::P_BYTES;
+        if (STREAMS && copies > 1) {                          // the other copies' keys: P stays zero there
+            for (int c = 0; c < 16; ++c)
+                *reinterpret_cast<uint4*>(myPs + (c >> 3) * S::P_BYTES + sw128_offset(r, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
         }
-        const int depth = tree_line(parent, row_valid ? row / G : 0, window, line);
+        const int depth = tree_line(parent, node_head.x, window, line);
         lo_r = window > 0 ? max(0, sg.c + depth - window + 1) : 0;
         if (!STREAMS || grp == 0) {
             cp_wait<0>();
@@ -665,87 +696,92 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
         }
-        unsigned char* myPs = sP + grp * 2 * S::P_BYTES;
-        for (int i = 0; i < n_mine; ++i) {
-            const int j_base = (jt_begin + tile_no(grp, i)) * KN, buf = i & 1;
-            ok = mbar_wait(bar(S::B_S + grp * 2 + buf), (i >> 1) & 1) && ok;
-            fence_after_sync();
-            unsigned a[64];
-            tmem_ld32(lane_addr + (grp * 2 + buf) * KN, reinterpret_cast<unsigned(&)[32]>(a[0]));
-            tmem_ld32(lane_addr + (grp * 2 + buf) * KN + 32, reinterpret_cast<unsigned(&)[32]>(a[32]));
-            tmem_ld_wait();
-            if (softcap > 0.f) {
-                const float k = scale / softcap;
-#pragma unroll
-                for (int e = 0; e < 64; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
-            }
-            float mx = -INFINITY;
-            if (whole(j_base)) {
-#pragma unroll
-                for (int e = 0; e < 64; e += 2) mx = max3(mx, __uint_as_float(a[e]), __uint_as_float(a[e + 1]));
-            } else {
-                const unsigned long long vis = visible(j_base);
-                const unsigned vis_lo = (unsigned)vis, vis_hi = (unsigned)(vis >> 32);
-#pragma unroll
-                for (int e = 0; e < 64; ++e) {
-                    if (!((e < 32 ? vis_lo : vis_hi) & (1u << (e & 31)))) a[e] = 0xff800000u;
-                    mx = fmaxf(mx, __uint_as_float(a[e]));
-                }
-            }
-            mx *= scale_eff;                                  // the scale is positive
-            float alpha = 1.f;
-            bool moved = false;
-            if (mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx != -INFINITY)) {
-                alpha = fast_exp2(m_ref - mx);                // 0 on the first move
-                m_ref = mx;
-                moved = true;
-            }
-            const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-            // P(i) goes into the buffer that P V(i - 2) read; O is touched only when P V(i - 1) is done
-            if (i > 1) ok = mbar_wait(bar(S::B_PV + grp * 2 + buf), ((i - 2) >> 1) & 1) && ok;
-            if (i > 0 && __any_sync(0xffffffffu, moved)) {
-                ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
+        auto walk = [&](auto width) {
+            constexpr int W = decltype(width)::value;
+            const int col = W == 64 ? 0 : copy * W;           // of a tile's keys
+            for (int i = 0; i < n_mine; ++i) {
+                const int j_base = (jt_begin + tile_no(grp, i)) * KN, buf = i & 1;
+                ok = mbar_wait(bar(S::B_S + grp * 2 + buf), (i >> 1) & 1) && ok;
                 fence_after_sync();
-#pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    unsigned o[32];
-                    tmem_ld32(o_addr + c0, o);
-                    tmem_ld_wait();
+                unsigned a[W];
+                const unsigned from = lane_addr + (grp * 2 + buf) * KN + col;
+                if constexpr (W == 16) {
+                    tmem_ld16(from, a);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                    tmem_st32(o_addr + c0, o);
+                    for (int c = 0; c < W; c += 32) tmem_ld32(from + c, reinterpret_cast<unsigned(&)[32]>(a[c]));
                 }
-                tmem_st_wait();
-            }
-            unsigned char* myP = myPs + buf * S::P_BYTES;
-            const unsigned long long scale2 = pack2(scale_eff, scale_eff), shift2 = pack2(-mu, -mu);
-            unsigned long long sum2 = pack2(0.f, 0.f);
+                tmem_ld_wait();
+                if (softcap > 0.f) {
+                    const float k = scale / softcap;
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-                float x0, x1;
-                unpack2(fma2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), scale2, shift2), x0, x1);
-                const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                sum2 = add2(sum2, pack2(p0, p1));
-                a[e] = __float_as_uint(p0);
-                a[e + 1] = __float_as_uint(p1);
-            }
-            float sum_lo, sum_hi;
-            unpack2(sum2, sum_lo, sum_hi);
+                    for (int e = 0; e < W; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+                }
+                if (!whole(j_base)) {
+                    const unsigned long long vis = visible(j_base) >> col;
+                    const unsigned vis_lo = (unsigned)vis, vis_hi = (unsigned)(vis >> 32);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                uint4 v;
-                v.x = pack_bf16(__uint_as_float(a[8 * c]), __uint_as_float(a[8 * c + 1]));
-                v.y = pack_bf16(__uint_as_float(a[8 * c + 2]), __uint_as_float(a[8 * c + 3]));
-                v.z = pack_bf16(__uint_as_float(a[8 * c + 4]), __uint_as_float(a[8 * c + 5]));
-                v.w = pack_bf16(__uint_as_float(a[8 * c + 6]), __uint_as_float(a[8 * c + 7]));
-                *reinterpret_cast<uint4*>(myP + sw128_offset(r, c)) = v;
+                    for (int e = 0; e < W; ++e)
+                        if (!((e < 32 ? vis_lo : vis_hi) & (1u << (e & 31)))) a[e] = 0xff800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < W; e += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(a[e + 2 * k]), __uint_as_float(a[e + 2 * k + 1]));
+                const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale_eff;     // the scale is positive
+                float alpha = 1.f;
+                bool moved = false;
+                if (mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx != -INFINITY)) {
+                    alpha = fast_exp2(m_ref - mx);            // 0 on the first move
+                    m_ref = mx;
+                    moved = true;
+                }
+                const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+                // P(i) goes into the buffer that P V(i - 2) read; O is touched only when P V(i - 1) is done
+                if (i > 1) ok = mbar_wait(bar(S::B_PV + grp * 2 + buf), ((i - 2) >> 1) & 1) && ok;
+                if (i > 0 && __any_sync(0xffffffffu, moved)) {
+                    ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
+                    fence_after_sync();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        unsigned o[32];
+                        tmem_ld32(o_addr + c0, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(o_addr + c0, o);
+                    }
+                    tmem_st_wait();
+                }
+                unsigned char* myP = myPs + buf * S::P_BYTES;
+                const unsigned long long scale2 = pack2(scale_eff, scale_eff), shift2 = pack2(-mu, -mu);
+                unsigned long long sum2[4] = {};
+#pragma unroll
+                for (int c = 0; c < W / 8; ++c) {
+                    unsigned w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float x0, x1;
+                        unpack2(fma2(pack2(__uint_as_float(a[8 * c + 2 * k]), __uint_as_float(a[8 * c + 2 * k + 1])), scale2, shift2), x0, x1);
+                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                        sum2[k] = add2(sum2[k], pack2(p0, p1));
+                        w[k] = pack_bf16(p0, p1);
+                    }
+                    *reinterpret_cast<uint4*>(myP + sw128_offset(r, (col >> 3) + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                float sum_lo, sum_hi;
+                unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_lo, sum_hi);
+                l_run = l_run * alpha + (sum_lo + sum_hi);
+                fence_proxy_async();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(S::B_P + grp * 2 + buf));       // S(i) is read, O is rescaled, P(i) is written
             }
-            l_run = l_run * alpha + (sum_lo + sum_hi);
-            fence_proxy_async();
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(S::B_P + grp * 2 + buf));           // S(i) is read, O is rescaled, P(i) is written
-        }
+        };
+        if (copies == 1) walk(Width<64>());
+        else if (copies == 2) walk(Width<32>());
+        else walk(Width<16>());
         if (n_mine > 0) ok = mbar_wait(bar(S::B_PV + grp * 2 + ((n_mine - 1) & 1)), ((n_mine - 1) >> 1) & 1) && ok;
     } else if (warp >= 8 && warp < 12 && n_mine > 0 && lane == 0) {
         // ================================================================== an issuing thread: descriptors are a base plus a constant
@@ -818,10 +854,6 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             // A lane for each (page of the tile, slab): it knows the page one tile ahead and asks for its box.  A whole tile's bytes are counted
             // on the barrier that its product waits for; values that have to be looked through first land on a barrier of the loader's.
             const CUtensorMap* map = is_k ? &kmap : &vmap;
-            const int box = min(pg.page_size, KN), pi = lane / S::DS, slab = lane % S::DS;
-            const bool mine = pi * box < KN;
-            auto in_sight = [&](int jt) { const int j = jt * KN + pi * box; return mine && j + box > sg.lo && j <= sg.hi; };
-            auto ask_page = [&](int jt) { return in_sight(jt) ? bt_row[pg.block(jt * KN + pi * box)] : -1; };
             unsigned land_par = 0u;                           // the parity of each stage's next landing
             auto finish = [&](int t) {                        // values of tile t, which was not whole, have landed
                 const int st = t % STAGES;
@@ -833,7 +865,6 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(S::B_V_FULL + st));
             };
-            int next = ask_page(jt_begin);
             for (int t = 0; t < n_tiles; ++t) {
                 const int st = t % STAGES, page = next;
                 if (t >= STAGES) ok = mbar_wait(bar(b_empty + st), (t / STAGES - 1) & 1) && ok;
@@ -908,53 +939,52 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             for (int t = max(0, n_tiles - S::LAG); t < n_tiles; ++t) announce(t);
         }
     }
-    if (STREAMS && has_rows) *joined(grp) = make_float2(m_ref, l_run);
+    // The rows leave through shared memory, where K, V and P lay: each (group, copy) its outputs in float32, brought to the row's common maximum,
+    // a row of D by 16-byte pieces, piece p of row x at p ^ (x % 8).
+    float2* stats = reinterpret_cast<float2*>(sQ);            // [group][tile row]: maximum and sum
+    float* row_inv = reinterpret_cast<float*>(stats + 2 * QM);
     pdl_trigger_late();
     fence_before_sync();
-    __syncthreads();
+    __syncthreads();                                          // no product reads shared memory any more
     fence_after_sync();
-    if (has_rows) {
-        // The rows leave: the finished ones, or O as it stands with the reference maximum and the sum.  Streams are joined first, either group
-        // for half of the columns.
-        const bool odd = *odd_values != 0, part = sg.n_split > 1;
-        const size_t at = token * Hq + h, slot = (size_t)split * total_rows * Hq + at;
-        float w_a = 1.f, w_b = 0.f;
-        if (STREAMS && n_tiles > 1) {
-            const float2 a = *joined(0), b = *joined(1);
-            m_ref = fmaxf(a.x, b.x);
-            const float top = m_ref == -INFINITY ? 0.f : m_ref;
-            w_a = fast_exp2(a.x - top);
-            w_b = fast_exp2(b.x - top);
-            l_run = a.y * w_a + b.y * w_b;
-        } else if (STREAMS) {
-            const float2 a = *joined(0);
-            m_ref = a.x;
-            l_run = a.y;
+    if (has_rows) stats[grp * QM + r] = make_float2(m_ref, l_run);
+    __syncthreads();
+    const int groups = STREAMS && n_tiles == 1 ? 1 : 2;       // STREAMS: those that have had a tile
+    if (has_rows && n_mine > 0) {
+        float mu = m_ref == -INFINITY ? 0.f : m_ref, mine = 1.f;
+        if (STREAMS) {
+            float top = -INFINITY;
+            for (int g = 0; g < groups; ++g)
+                for (int c = 0; c < copies; ++c) top = fmaxf(top, stats[g * QM + c * copy_rows + in_cta].x);
+            mu = top == -INFINITY ? 0.f : top;
+            mine = fast_exp2(m_ref - mu);
+            if (grp == 0 && copy == 0) {
+                l_run = 0.f;
+                for (int g = 0; g < groups; ++g)
+                    for (int c = 0; c < copies; ++c) {
+                        const float2 f = stats[g * QM + c * copy_rows + in_cta];
+                        l_run += f.y * fast_exp2(f.x - mu);
+                    }
+                m_ref = top;
+            }
         }
-        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-        if (part && row_valid && (!STREAMS || grp == 0)) {
-            part_ml[2 * slot] = m_ref;
-            part_ml[2 * slot + 1] = l_run;
+        if (row_valid && (!STREAMS || (grp == 0 && copy == 0))) {
+            const size_t at = token * Hq + h;
+            if (sg.n_split > 1) *reinterpret_cast<float2*>(part_ml + 2 * ((size_t)split * total_rows * Hq + at)) = make_float2(m_ref, l_run);
+            else if (sink != nullptr) l_run += exp2f(sink[h] * LOG2E - mu);
+            row_inv[in_cta] = l_run == 0.f ? 0.f : 1.f / l_run;
         }
-        float l_all = l_run;
-        if (sink != nullptr && !part) l_all += exp2f(sink[h] * LOG2E - mu);
-        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-        const unsigned o_first = lane_addr + S::O_COL + (STREAMS ? 0 : grp * D);
+        const bool odd = *odd_values != 0 && row_valid && (!STREAMS || (grp == 0 && copy == 0));
+        unsigned char* slot = sK + (size_t)(grp * QM + r) * (D * 4);
 #pragma unroll 1
-        for (int c0 = STREAMS ? grp * (D / 2) : 0; c0 < (STREAMS ? (grp + 1) * (D / 2) : D); c0 += 32) {
+        for (int c0 = 0; c0 < D; c0 += 32) {
             unsigned o[32];
             __syncwarp();
-            tmem_ld32(o_first + c0, o);
-            if (STREAMS && n_tiles > 1) {
-                unsigned o_b[32];
-                tmem_ld32(o_first + D + c0, o_b);
-                tmem_ld_wait();
+            tmem_ld32(o_addr + c0, o);
+            tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), w_a, __uint_as_float(o_b[i]) * w_b));
-            } else {
-                tmem_ld_wait();
-            }
-            if (odd && row_valid) {
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mine);
+            if (odd) {
                 // what the products left out: values that are no numbers, where this row sees their keys
                 for (int t = 0; t < n_tiles; ++t) {
                     const int j_base = (jt_begin + t) * KN;
@@ -980,29 +1010,33 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     }
                 }
             }
-            if (part && row_valid) {
-                float4* to = reinterpret_cast<float4*>(part_o + slot * D + c0);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    to[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-            } else if (row_valid) {
-                uint4* to = reinterpret_cast<uint4*>(out + at * D + c0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 v;
-                    v.x = pack_bf16(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-                    v.y = pack_bf16(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-                    v.z = pack_bf16(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-                    v.w = pack_bf16(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-                    to[i] = v;
-                }
-            }
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint4*>(slot + ((((c0 >> 2) + i) ^ (r & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
     }
     if (!ok) atomicExch(status, 1);
     fence_before_sync();
     __syncthreads();
     if (warp == 8) tmem_dealloc(tmem, S::TMEM_COLS);
+    // a row's partial outputs added, whole lines written: a thread four columns
+    const bool parted = sg.n_split > 1;
+    const int slots = STREAMS ? groups * copies : 1;
+#pragma unroll 2
+    for (int i = tid; i < rows * (D / 4); i += S::THREADS) {
+        const int x = i / (D / 4), piece = i % (D / 4);
+        const int2 nh = by_group(row0 + x);
+        const size_t at = (size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < slots; ++c) {
+            const int at_row = STREAMS ? c * copy_rows + x : x;      // copies of a group lie side by side, groups QM apart
+            const float4 f = *reinterpret_cast<const float4*>(sK + (size_t)at_row * (D * 4) + ((piece ^ (at_row & 7)) << 4));
+            sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+        }
+        const float inv = row_inv[x];
+        if (parted) *reinterpret_cast<float4*>(part_o + ((size_t)split * total_rows * Hq + at) * D + 4 * piece) = sum;
+        else *reinterpret_cast<uint2*>(out + at * D + 4 * piece) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+    }
 }
 
 // out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).  All
