@@ -738,8 +738,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     moved = true;
                 }
                 const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-                // P(i) goes into the buffer that P V(i - 2) read; O is touched only when P V(i - 1) is done
-                if (i > 1) ok = mbar_wait(bar(S::B_PV + grp * 2 + buf), ((i - 2) >> 1) & 1) && ok;
+                // P(i) goes into the buffer that P V(i - 2) read: that was done when S(i) was issued.  O is touched only when P V(i - 1) is done.
                 if (i > 0 && __any_sync(0xffffffffu, moved)) {
                     ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
                     fence_after_sync();
@@ -793,7 +792,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             for (int i = 0; i < n_mine; ++i) {
                 const int t = tile_no(grp, i), st = t % STAGES;
                 ok = mbar_wait(bar(S::B_K_FULL + st), (t / STAGES) & 1) && ok;
-                if (i > 1) ok = mbar_wait(bar(S::B_P + grp * 2 + (i & 1)), ((i - 2) >> 1) & 1) && ok;     // the rows have read S(i - 2)
+                if (i > 1) ok = mbar_wait(bar(S::B_PV + grp * 2 + (i & 1)), ((i - 2) >> 1) & 1) && ok;    // the rows have read S(i - 2), and P(i - 2) is free
                 fence_after_sync();
                 const unsigned long long k_tile = dK + (unsigned long long)(st * (S::K_BYTES >> 4));
                 const unsigned d_s = tmem + (grp * 2 + (i & 1)) * KN;

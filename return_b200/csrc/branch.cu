@@ -42,29 +42,47 @@ __device__ int walk_tree(const int* token, const int* parent, const int* sampled
 }
 
 constexpr int COMMIT_THREADS = 256;
-constexpr int MOVES_AT_ONCE = 4;
+constexpr int MOVES_AT_ONCE = 8;
 
-// grid: (segments, parts of the planes x heads).  Node path[i] moves from slot c + path[i] to slot c + i.  A thread keeps to its
-// piece of a row and goes through the moves in order, a few loads before their stores.  No store meets a row that is still
-// to be read: path[k] >= k, so a later move's source lies behind every earlier move's destination.
-// The walk is done by every CTA for itself (a few hundred cycles); the first part writes it down.
+// x / d and x % d of small numbers: a quotient by the reciprocal, put right where it is one off.
+struct ByDivisor {
+    int d;
+    float inv;
+    __device__ __forceinline__ explicit ByDivisor(int n) : d(n), inv(1.0f / (float)n) {}
+    __device__ __forceinline__ int2 operator()(int x) const {
+        int q = (int)((float)x * inv), r = x - q * d;
+        if (r < 0) { --q; r += d; }
+        if (r >= d) { ++q; r -= d; }
+        return make_int2(q, r);
+    }
+};
+
+// grid: (segments, parts of the planes x heads).  Node path[i] moves from slot c + path[i] to slot c + i.  LPR lanes share a row's pieces; a
+// thread keeps to its piece of a (plane, head) and goes through the moves in order, eight loads before their stores.  No store meets a row
+// that is still to be read: path[k] >= k, so a later move's source lies behind every earlier move's destination.
+// The walk is done by every CTA for itself (a few hundred cycles); the first part writes it down.  What it takes is asked for at once, the
+// part of the block table that the tree lies on with it.
 template <int W>
 __global__ void __launch_bounds__(COMMIT_THREADS)
 tree_commit_kernel(const int* __restrict__ tokens, const int* __restrict__ tree_parent, const int* __restrict__ sampled,
                    const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ block_table, int bt_stride,
-                   int page_size, unsigned char* __restrict__ pool, int planes, long long pages, int heads, int row_bytes, int per_cta,
+                   int page_size, unsigned char* __restrict__ pool, int planes, long long pages, int heads, int row_bytes, int lpr_log, int per_cta,
                    int* __restrict__ path_out, int* __restrict__ count_out, int* __restrict__ emitted_out, int width) {
     typedef typename Piece<W>::type P;
     __shared__ int s_token[TREE_MAX_NODES], s_parent[TREE_MAX_NODES], s_sampled[TREE_MAX_NODES], s_path[TREE_MAX_NODES];
+    __shared__ int s_page[TREE_MAX_NODES + 1];                // of the blocks that the tree lies on, from its first slot's
     __shared__ int s_count;
     __shared__ long long s_src[TREE_MAX_NODES], s_dst[TREE_MAX_NODES];        // rows of head 0 in a plane, -1: nothing moves
+    pdl_wait();
     const int seg = blockIdx.x, tid = threadIdx.x;
     const int q_begin = cu_q[seg], n = min(cu_q[seg + 1] - q_begin, TREE_MAX_NODES), c = seg_pos0[seg];
+    const int block0 = c / page_size, blocks = pool != nullptr && n > 0 ? (c + n - 1) / page_size - block0 + 1 : 0;
     for (int i = tid; i < n; i += COMMIT_THREADS) {
         s_token[i] = tokens[q_begin + i];
         s_parent[i] = tree_parent[q_begin + i];
         s_sampled[i] = sampled[q_begin + i];
     }
+    for (int i = tid; i < blocks; i += COMMIT_THREADS) s_page[i] = block_table[(size_t)seg * bt_stride + block0 + i];
     __syncthreads();
     if (tid < 32) {
         const int count = n > 0 ? walk_tree(s_token, s_parent, s_sampled, n, s_path, tid) : 0;
@@ -81,39 +99,40 @@ tree_commit_kernel(const int* __restrict__ tokens, const int* __restrict__ tree_
         if (tid == 0) count_out[seg] = count;
     }
     if (pool == nullptr) return;
-    const int* bt = block_table + (size_t)seg * bt_stride;
     for (int i = tid; i < count; i += COMMIT_THREADS) {
         const int from = c + s_path[i], to = c + i;
         long long src = -1, dst = -1;
         if (from != to) {
-            const int ps = bt[from / page_size], pd = bt[to / page_size];
+            const int ps = s_page[from / page_size - block0], pd = s_page[to / page_size - block0];
             if (ps >= 0 && pd >= 0 && ps < pages && pd < pages) {
                 src = (long long)ps * heads * page_size + from % page_size;
                 dst = (long long)pd * heads * page_size + to % page_size;
             }
         }
-        s_src[i] = src;
-        s_dst[i] = dst;
+        s_src[i] = src * row_bytes;
+        s_dst[i] = dst * row_bytes;
     }
     __syncthreads();
     int first = 1;                                            // the moves begin behind the nodes that lie in place
     while (first < count && s_src[first] < 0) ++first;
     if (first >= count) return;
-    const int pieces = row_bytes / W;
-    const long long work = (long long)min(per_cta, planes * heads - (int)blockIdx.y * per_cta) * pieces;
-    for (long long w = tid; w < work; w += COMMIT_THREADS) {
-        const int pair = (int)blockIdx.y * per_cta + (int)(w / pieces), piece = (int)(w % pieces);
-        const int plane = pair / heads, head = pair % heads;
-        const long long plane_rows = pages * heads * page_size;
-        unsigned char* base = pool + ((long long)plane * plane_rows + (long long)head * page_size) * row_bytes + (long long)piece * W;
-        for (int i0 = first; i0 < count; i0 += MOVES_AT_ONCE) {
-            P v[MOVES_AT_ONCE];
+    const ByDivisor by_heads(heads);
+    const int lpr = 1 << lpr_log, pair_end = min(planes * heads, ((int)blockIdx.y + 1) * per_cta);
+    const long long plane_bytes = pages * heads * page_size * row_bytes, head_bytes = (long long)page_size * row_bytes;
+    for (int pair = (int)blockIdx.y * per_cta + (tid >> lpr_log); pair < pair_end; pair += COMMIT_THREADS >> lpr_log) {
+        const int2 at = by_heads(pair);                       // plane, head
+        unsigned char* head = pool + at.x * plane_bytes + at.y * head_bytes;
+        for (int byte = (tid & (lpr - 1)) * W; byte < row_bytes; byte += lpr * W) {
+            unsigned char* base = head + byte;
+            for (int i0 = first; i0 < count; i0 += MOVES_AT_ONCE) {
+                P v[MOVES_AT_ONCE];
 #pragma unroll
-            for (int u = 0; u < MOVES_AT_ONCE; ++u)
-                if (i0 + u < count && s_src[i0 + u] >= 0) v[u] = *reinterpret_cast<const P*>(base + s_src[i0 + u] * row_bytes);
+                for (int u = 0; u < MOVES_AT_ONCE; ++u)
+                    if (i0 + u < count && s_src[i0 + u] >= 0) v[u] = *reinterpret_cast<const P*>(base + s_src[i0 + u]);
 #pragma unroll
-            for (int u = 0; u < MOVES_AT_ONCE; ++u)
-                if (i0 + u < count && s_src[i0 + u] >= 0) *reinterpret_cast<P*>(base + s_dst[i0 + u] * row_bytes) = v[u];
+                for (int u = 0; u < MOVES_AT_ONCE; ++u)
+                    if (i0 + u < count && s_src[i0 + u] >= 0) *reinterpret_cast<P*>(base + s_dst[i0 + u]) = v[u];
+            }
         }
     }
 }
@@ -143,36 +162,35 @@ __device__ __forceinline__ void copy_bytes(unsigned char* dst, const unsigned ch
     }
 }
 
-// The first rows[i] rows of page src[i] to page dst[i], in every plane and head.  A head's rows of a page lie together, so a (plane,
-// head) is one run of bytes; a CTA takes per_cta of them, their pieces in one row of work for its threads.
+// The first rows[i] rows of page src[i] to page dst[i], in every plane and head.  A head's rows of a page lie together, so a (plane, head) is
+// one run of bytes; a warp takes one at a time, eight loads of a lane before their stores.
 // grid: (copies, parts of the planes x heads).
 template <int W>
 __global__ void __launch_bounds__(COPY_THREADS)
 copy_pages_kernel(unsigned char* __restrict__ pool, const int* __restrict__ src, const int* __restrict__ dst, const int* __restrict__ rows,
                   int planes, int pages, int heads, int page_size, int row_bytes, int per_cta) {
     typedef typename Piece<W>::type P;
-    const int i = blockIdx.x, tid = threadIdx.x;
+    constexpr int AT_ONCE = 8;
+    pdl_wait();
+    const int i = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int from = src[i], to = dst[i], n = min(rows[i], page_size);
     if (from < 0 || to < 0 || from >= pages || to >= pages || from == to || n <= 0) return;
-    const int pair0 = blockIdx.y * per_cta, pairs = min(per_cta, planes * heads - pair0);
-    const int pieces = n * (row_bytes / W);                   // of one (plane, head)
-    const long long run = (long long)page_size * row_bytes, page = run * heads, plane = page * pages;
-    const int work = pairs * pieces;
-    for (int w0 = 0; w0 < work; w0 += COPY_THREADS * COPY_UNROLL) {
-        P v[COPY_UNROLL];
-        long long at[COPY_UNROLL];
+    const int pair_end = min(planes * heads, ((int)blockIdx.y + 1) * per_cta);
+    const int bytes = n * row_bytes;                          // of one (plane, head)
+    const long long run = (long long)page_size * row_bytes, page = run * heads, plane = page * pages, step = (to - from) * page;
+    const ByDivisor by_heads(heads);
+    for (int pair = (int)blockIdx.y * per_cta + warp; pair < pair_end; pair += COPY_THREADS / 32) {
+        const int2 at = by_heads(pair);                       // plane, head
+        unsigned char* head = pool + at.x * plane + at.y * run + from * page;
+        for (int b0 = lane * W; b0 < bytes; b0 += 32 * W * AT_ONCE) {
+            P v[AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < COPY_UNROLL; ++u) {
-            const int w = w0 + u * COPY_THREADS + tid;
-            if (w < work) {
-                const int k = w / pieces, pair = pair0 + k;
-                at[u] = (pair / heads) * plane + (pair % heads) * run + (long long)(w - k * pieces) * W;
-                v[u] = *reinterpret_cast<const P*>(pool + at[u] + from * page);
-            }
+            for (int u = 0; u < AT_ONCE; ++u)
+                if (b0 + u * 32 * W < bytes) v[u] = *reinterpret_cast<const P*>(head + b0 + u * 32 * W);
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+                if (b0 + u * 32 * W < bytes) *reinterpret_cast<P*>(head + step + b0 + u * 32 * W) = v[u];
         }
-#pragma unroll
-        for (int u = 0; u < COPY_UNROLL; ++u)
-            if (w0 + u * COPY_THREADS + tid < work) *reinterpret_cast<P*>(pool + at[u] + to * page) = v[u];
     }
 }
 
@@ -198,10 +216,10 @@ copy_slots_kernel(const SlotTensors t, const int* __restrict__ src, const int* _
     else copy_bytes<1>(d, s, n, threadIdx.x);
 }
 
-// How many (plane, head) pairs a CTA takes: so many that `first` x parts CTAs give every SM a few, a multiple of `unit`.
-int pairs_per_cta(int first, int pairs, int unit) {
-    const int want = rb_num_sms() * 6;
-    const long long parts = first >= want ? 1 : (want + first - 1) / first;
+// How many (plane, head) pairs a CTA takes: so many that `first` x parts CTAs give every SM `per_sm`, which is as many as it holds, a multiple of `unit`.
+int pairs_per_cta(int first, int pairs, int unit, int per_sm) {
+    const int want = rb_num_sms() * per_sm;
+    const long long parts = first >= want ? 1 : want / first;
     long long per = (pairs + parts - 1) / parts;
     per = (per + unit - 1) / unit * unit;
     return (int)(per < unit ? unit : per);
@@ -218,16 +236,15 @@ RB_EXPORT int rb_tree_commit(const int* tokens, const int* parent, const int* sa
     if (segments <= 0) return 0;
     if (pool != nullptr && (planes <= 0 || heads <= 0 || page_size <= 0 || row_bytes <= 0 || row_bytes % 2)) return (int)cudaErrorInvalidValue;
     const bool wide = ((uintptr_t)pool & 15) == 0 && row_bytes % 16 == 0;
-    const int pairs = pool != nullptr ? planes * heads : 1;
-    const int pieces = pool != nullptr ? row_bytes / (wide ? 16 : 2) : 1;
-    const int unit = pieces >= COMMIT_THREADS ? 1 : COMMIT_THREADS / pieces;              // pairs that keep a CTA's threads busy once
-    const int per_cta = pairs_per_cta(segments, pairs, unit);
+    const int pairs = pool != nullptr ? planes * heads : 1, W = wide ? 16 : 2;
+    int lpr_log = 0;                                          // lanes that share a row
+    while ((W << lpr_log) < row_bytes && lpr_log < 5) ++lpr_log;
+    const int per_cta = pairs_per_cta(segments, pairs, COMMIT_THREADS >> lpr_log, 4);
     dim3 grid(segments, (pairs + per_cta - 1) / per_cta);
-    if (grid.y > 65535) return (int)cudaErrorInvalidValue;
+    if (grid.y > 65535 || pairs > (1 << 22)) return (int)cudaErrorInvalidValue;      // what ByDivisor takes
     auto kernel = wide ? tree_commit_kernel<16> : tree_commit_kernel<2>;
-    kernel<<<grid, COMMIT_THREADS, 0, st>>>(tokens, parent, sampled, cu_q, seg_pos0, block_table, bt_stride, page_size, (unsigned char*)pool,
-                                            planes, pages, heads, row_bytes, per_cta, path_out, count_out, emitted_out, width);
-    return rb_launch_status();
+    return rb_launch_pdl(kernel, grid, dim3(COMMIT_THREADS), 0, st, tokens, parent, sampled, cu_q, seg_pos0, block_table, bt_stride, page_size,
+                         (unsigned char*)pool, planes, (long long)pages, heads, row_bytes, lpr_log, per_cta, path_out, count_out, emitted_out, width);
 }
 
 RB_EXPORT int rb_copy_pages(void* pool, const int* src, const int* dst, const int* rows, int copies, int planes, int pages, int heads,
@@ -235,15 +252,12 @@ RB_EXPORT int rb_copy_pages(void* pool, const int* src, const int* dst, const in
     if (copies <= 0) return 0;
     if (planes <= 0 || heads <= 0 || page_size <= 0 || row_bytes <= 0 || row_bytes % 2) return (int)cudaErrorInvalidValue;
     const bool wide = ((uintptr_t)pool & 15) == 0 && row_bytes % 16 == 0;
-    const long long pieces = (long long)page_size * row_bytes / (wide ? 16 : 2);
-    const int unit = pieces >= COPY_THREADS ? 1 : (int)(COPY_THREADS / pieces);
-    int per_cta = pairs_per_cta(copies, planes * heads, unit);
-    if (per_cta * pieces > (1ll << 30)) per_cta = 1;
+    if ((long long)page_size * row_bytes > (1ll << 30) || planes * (long long)heads > (1 << 22)) return (int)cudaErrorInvalidValue;
+    const int per_cta = pairs_per_cta(copies, planes * heads, COPY_THREADS / 32, 4);
     dim3 grid(copies, (planes * heads + per_cta - 1) / per_cta);
-    if (grid.y > 65535 || pieces > (1ll << 30)) return (int)cudaErrorInvalidValue;
+    if (grid.y > 65535) return (int)cudaErrorInvalidValue;
     auto kernel = wide ? copy_pages_kernel<16> : copy_pages_kernel<2>;
-    kernel<<<grid, COPY_THREADS, 0, st>>>((unsigned char*)pool, src, dst, rows, planes, pages, heads, page_size, row_bytes, per_cta);
-    return rb_launch_status();
+    return rb_launch_pdl(kernel, grid, dim3(COPY_THREADS), 0, st, (unsigned char*)pool, src, dst, rows, planes, pages, heads, page_size, row_bytes, per_cta);
 }
 
 // tensors: host array of `count` addresses and then `count` row lengths in bytes.

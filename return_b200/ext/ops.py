@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 import threading
 from ctypes import c_float, c_int, c_void_p
 from typing import Optional
@@ -2244,7 +2245,6 @@ _tree = _branch = None
 TREE_MAX_NODES = 256               # drafted nodes of a segment
 TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
-TREE_MIN_SHARE = 2                 # a CTA of split keys walks at least so many tiles
 TREE_MAX_SPLITS = 64
 TREE_SCRATCH_BYTES = 256 << 20
 
@@ -2321,24 +2321,38 @@ def _tree_lengths(batch, page_size: int, blocks: int):
     return held
 
 
-def tree_shares(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int):
-    """(splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; (1, 0): no split.  The
-    shares are as long as they can be while the launch's CTAs fill the GPU once."""
+# What a CTA costs beside its key tiles, and what the merge of split keys costs, in key tiles of the kernel: the tcgen05 kernel's tiles take half a
+# microsecond each, those of the kernel for any type and head size 1.6 (bfloat16) and 4 (float32).  Measured in tree steps of 1 to 64
+# requests behind 500 to 8,000 tokens; one tree of 8 nodes behind 500: 10.3 us unsplit, 11.8 split in four.
+TREE_COSTS = {"tcgen05": (12.0, 8.0), "bfloat16": (3.0, 2.5), "float32": (1.5, 1.0)}
+TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64)
+
+
+def tree_shares(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int, kind: str):
+    """(splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; (1, 0): no split.  Of shares that
+    cut the longest walk into a number of TREE_PARTS, the one whose launch is done first: rounds of CTAs times a CTA's cost, and the merge."""
     tiles = [(e - 1) // TREE_KEY_TILE - (max(0, e - k - window + 1) if window else 0) // TREE_KEY_TILE + 1 for k, e in zip(nodes, ends)]
     blocks = [-(-k * rows_per_node // cta_rows) * kv_heads for k in nodes]
     slots, longest = num_sms() * ctas_per_sm, max(tiles)
-    if sum(blocks) >= slots or longest < 2 * TREE_MIN_SHARE:
-        return 1, 0
-    most = max(1, min(TREE_MAX_SPLITS, TREE_SCRATCH_BYTES // max(1, rows * (head_dim + 2) * 4)))
-    lo, hi = max(TREE_MIN_SHARE, -(-longest // most)), longest
-    while lo < hi:                                     # the smallest share whose CTAs fit at once
-        mid = (lo + hi) // 2
-        if sum([b * -(-t // mid) for b, t in zip(blocks, tiles)]) <= slots:
-            hi = mid
-        else:
-            lo = mid + 1
-    splits = -(-longest // lo)
-    return (splits, lo) if splits > 1 else (1, 0)
+    fixed, merge = TREE_COSTS[kind]
+
+    def done(ctas, share):                             # rounds count in parts: a last one that is not full is still a round for those in it
+        return max(1.0, -(-ctas // slots) - 0.3 if ctas > slots else 1.0) * (share + fixed)
+
+    best, best_done = (1, 0), done(sum(blocks), longest)
+    most = min(TREE_MAX_SPLITS, TREE_SCRATCH_BYTES // max(1, rows * (head_dim + 2) * 4))
+    for parts in TREE_PARTS:
+        share = -(-longest // parts)
+        splits = -(-longest // share)
+        if splits > most or splits == 1:
+            break
+        ctas = sum([b * -(-t // share) for b, t in zip(blocks, tiles)])
+        d = done(ctas, share) + merge * (1.0 + 0.03 * splits)
+        if d < best_done:
+            best, best_done = (splits, share), d
+        if ctas > 2 * slots:
+            break
+    return best
 
 
 def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window=None,
@@ -2405,7 +2419,7 @@ def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_head
     if kind and dtype == torch.bfloat16 and head_dim in TC5_ATTENTION_HEAD_DIMS:
         tiles = 1 if longest * group <= TREE_TILE_ROWS else 2
     return (tiles,) + tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim, tiles * TREE_TILE_ROWS or 32,
-                                  1 if tiles or head_dim > 128 else 2)
+                                  1 if tiles or head_dim > 128 else 2, "tcgen05" if tiles else "float32" if dtype == torch.float32 else "bfloat16")
 
 
 def _pool_shape(pool):
@@ -2426,33 +2440,22 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
     ``caches``: (pool, block_table) of every group of layers; the row of slot ``seg_pos0 + path[i]`` goes to slot ``seg_pos0 + i``.  The
     request then holds ``seg_pos0 + count`` tokens.  Other rows stay as they are; a move from or to a page that the table marks as
     gone is left out."""
-    width = path.shape[1] if path.dim() == 2 else 0
-    lengths, shapes = None, []
+    key = ("tree.commit", sampled.shape, path.shape, count.shape, emitted.shape, *[x for pool, table in caches for x in (pool.shape, pool.dtype, table.shape)])
+    plan = batch.scratch.get(key)                      # what follows from the shapes is looked at once a step
+    if plan is None:
+        plan = batch.scratch[key] = _commit_plan(sampled, batch, caches, path, count, emitted)
+    n, width, shapes = plan
+    ints = torch.int32
+    tokens = batch.tokens
+    if not (sampled.dtype == ints and path.dtype == ints and count.dtype == ints and emitted.dtype == ints and tokens.dtype == ints
+            and sampled.is_contiguous() and path.is_contiguous() and count.is_contiguous() and emitted.is_contiguous() and tokens.is_contiguous()):
+        raise KernelError("sampled, tokens, path, count and emitted: contiguous int32")
     for pool, table in caches:
-        key = ("tree.commit", pool.shape, pool.dtype, table.shape)
-        held = batch.scratch.get(key)                  # what follows from the shapes is looked at once a step
-        if held is None:
-            shape = _pool_shape(pool)
-            if table.dim() != 2 or table.shape[0] != len(batch.host.seg_pos0):
-                raise KernelError("block_table: int32 [segments, blocks]")
-            held = batch.scratch[key] = (shape, _tree_lengths(batch, shape[3], table.shape[1]))
-        if not (pool.is_contiguous() and table.dtype == torch.int32 and table.stride(1) == 1):
+        if not (pool.is_contiguous() and table.dtype == ints and table.stride(1) == 1):
             raise KernelError("a pool: contiguous; its block_table: int32, unit stride along a row")
-        shapes.append(held[0])
-        lengths = held[1]
-    if lengths is None:                                # a model without paged layers: the walk alone
-        lengths = _tree_lengths(batch, 1 << 30, 1)
-    n, T, longest = lengths[:3]
-    if width < longest:
-        raise KernelError(f"path: {longest} columns at least")
-    _ints("sampled", sampled, T)
-    _ints("tokens", batch.tokens, T)
-    _ints("path", path, n, width)
-    _ints("emitted", emitted, n, width)
-    _ints("count", count, n)
-    _same_device(sampled, batch.tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted)
+    _same_device(sampled, tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted)
     entry, st = branch_lib().rb_tree_commit, _stream()
-    args = (batch.tokens.data_ptr(), batch.tree_parent.data_ptr(), sampled.data_ptr(), batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), n)
+    args = (tokens.data_ptr(), batch.tree_parent.data_ptr(), sampled.data_ptr(), batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), n)
     outs = (path.data_ptr(), count.data_ptr(), emitted.data_ptr(), width)
     if not shapes:
         _check(entry(*args, None, 0, 1, None, 0, 0, 0, 0, *outs, st), "tree_commit")
@@ -2460,6 +2463,28 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
         _same_device(pool, table)
         _check(entry(*args, table.data_ptr(), table.stride(0), page_size, pool.data_ptr(), planes, pages, heads, row_bytes, *outs, st), "tree_commit")
         outs = (None, None, None, 0)
+
+
+def _commit_plan(sampled, batch, caches, path, count, emitted):
+    """What ``tree_commit`` knows of a step from shapes alone; raises where they do not fit."""
+    lengths, shapes = None, []
+    for pool, table in caches:
+        shape = _pool_shape(pool)
+        if table.dim() != 2 or table.shape[0] != len(batch.host.seg_pos0):
+            raise KernelError("block_table: int32 [segments, blocks]")
+        lengths = _tree_lengths(batch, shape[3], table.shape[1])
+        shapes.append(shape)
+    if lengths is None:                                # a model without paged layers: the walk alone
+        lengths = _tree_lengths(batch, 1 << 30, 1)
+    n, T, longest = lengths[:3]
+    width = path.shape[1] if path.dim() == 2 else 0
+    if width < longest:
+        raise KernelError(f"path: {longest} columns at least")
+    for name, t, shape in (("sampled", sampled, (T,)), ("tokens", batch.tokens, (T,)), ("path", path, (n, width)), ("emitted", emitted, (n, width)),
+                           ("count", count, (n,))):
+        if t.shape != shape:
+            raise KernelError(f"{name}: int32 of shape {shape} wanted, got {tuple(t.shape)}")
+    return n, width, shapes
 
 
 def copy_pages(pool, src, dst, rows) -> None:
@@ -2519,6 +2544,26 @@ BEAM_MAX_KEEP, BEAM_MAX_BEAMS = 128, 64
 
 
 @functools.lru_cache(maxsize=256)
+def _beam_plan(logits, scores, beams: int, scores_out, beams_out, tokens_out):
+    """(requests, continuations) of ``beam_select``'s shapes; raises where they do not fit."""
+    if len(logits) != 2 or len(scores_out) != 2:
+        raise KernelError("logits [requests * beams, V], scores_out [requests, keep]")
+    (rows, V), (requests, keep) = logits, scores_out
+    if not (1 <= beams <= BEAM_MAX_BEAMS and rows == requests * beams):
+        raise KernelError(f"logits: a row per request and beam, up to {BEAM_MAX_BEAMS} beams")
+    if not 1 <= keep <= min(BEAM_MAX_KEEP, beams * V):
+        raise KernelError(f"{keep} continuations asked for: 1 to {BEAM_MAX_KEEP}, and no more than there are")
+    if rows > 65535 or beams * V >= 2 ** 31 - 1:
+        raise KernelError("at most 65,535 rows, and beams * V within 31 bits")
+    if math.prod(scores) != rows:
+        raise KernelError("scores: float32, one per row of logits")
+    for name, shape in (("beams_out", beams_out), ("tokens_out", tokens_out)):
+        if shape != scores_out:
+            raise KernelError(f"{name}: int32 of shape {tuple(scores_out)} wanted, got {tuple(shape)}")
+    return requests, keep
+
+
+@functools.lru_cache(maxsize=256)
 def _beam_scratch(rows: int, V: int, keep: int, device: int) -> int:
     return branch_lib().rb_beam_scratch(rows, V, keep)
 
@@ -2528,26 +2573,17 @@ def beam_select(logits, scores, beams: int, scores_out, beams_out, tokens_out) -
     ``scores`` float32 [requests * beams], the beams' sums of log-probabilities.  A continuation (b, v) has the total
     scores[b] + log_softmax(logits[b])[v]; ties go to the lowest (b, v).  A total that is no number, and every one of a beam whose
     score is not finite, counts as -inf.  Out: totals (float32), beams and tokens (int32), [requests, keep] each."""
-    if logits.dim() != 2 or scores_out.dim() != 2:
-        raise KernelError("logits [requests * beams, V], scores_out [requests, keep]")
-    (rows, V), (requests, keep) = logits.shape, scores_out.shape
-    if not (1 <= beams <= BEAM_MAX_BEAMS and rows == requests * beams):
-        raise KernelError(f"logits: a row per request and beam, up to {BEAM_MAX_BEAMS} beams")
-    if not 1 <= keep <= min(BEAM_MAX_KEEP, beams * V):
-        raise KernelError(f"{keep} continuations asked for: 1 to {BEAM_MAX_KEEP}, and no more than there are")
-    if rows > 65535 or beams * V >= 2 ** 31 - 1:
-        raise KernelError("at most 65,535 rows, and beams * V within 31 bits")
-    if logits.dtype != torch.float32 or logits.stride(1) != 1:
+    requests, keep = _beam_plan(logits.shape, scores.shape, beams, scores_out.shape, beams_out.shape, tokens_out.shape)
+    f32, ints = torch.float32, torch.int32
+    if logits.dtype != f32 or logits.stride(1) != 1:
         raise KernelError("logits: float32, unit stride along a row")
-    if scores.dtype != torch.float32 or not scores.is_contiguous() or scores.numel() != rows:
-        raise KernelError("scores: float32, one per row of logits")
-    if scores_out.dtype != torch.float32 or not scores_out.is_contiguous():
-        raise KernelError("scores_out: contiguous float32")
-    _ints("beams_out", beams_out, requests, keep)
-    _ints("tokens_out", tokens_out, requests, keep)
+    if not (scores.dtype == f32 and scores_out.dtype == f32 and beams_out.dtype == ints and tokens_out.dtype == ints and scores.is_contiguous()
+            and scores_out.is_contiguous() and beams_out.is_contiguous() and tokens_out.is_contiguous()):
+        raise KernelError("scores and scores_out: contiguous float32; beams_out and tokens_out: contiguous int32")
     _same_device(logits, scores, scores_out, beams_out, tokens_out)
     if requests == 0:
         return
-    scratch = torch.empty(_beam_scratch(rows, V, keep, logits.get_device()), dtype=torch.float32, device=logits.device)
+    rows, V = logits.shape
+    scratch = torch.empty(_beam_scratch(rows, V, keep, logits.get_device()), dtype=f32, device=logits.device)
     _check(branch_lib().rb_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), requests, beams, V, keep, scores_out.data_ptr(),
                               beams_out.data_ptr(), tokens_out.data_ptr(), scratch.data_ptr(), _stream()), "beam_select", 2)

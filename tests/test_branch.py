@@ -104,21 +104,20 @@ def test_beam_select_refuses():
     refuse("65,535", ops.beam_select, **{**args(rows=65538, requests=21846, V=1, keep=1)})
 
 
-def test_tree_shares_cover_the_keys(monkeypatch):
-    """Every share is within the launch's splits, the shares cover the longest walk, and CTAs fill the device once at most."""
+@pytest.mark.parametrize("kind", sorted(ops.TREE_COSTS))
+def test_tree_shares_cover_the_keys(monkeypatch, kind):
+    """Every share is within the launch's splits, and the shares cover the longest walk; a full launch of long CTAs, and a short one, are not split."""
     monkeypatch.setattr(ops, "num_sms", lambda: 148)
-    for nodes, cached, window in (([8], [500], 0), ([16] * 8, [2040] * 8, 0), ([64] * 32, [250 * i for i in range(32)], 0), ([5, 1], [9000, 3], 700),
-                                  ([1], [0], 0), ([256], [130000], 0)):
+    for nodes, cached, window, split in (([8], [500], 0, None), ([16] * 8, [2040] * 8, 0, True), ([64] * 32, [250 * i for i in range(32)], 0, None),
+                                         ([5, 1], [9000, 3], 700, True), ([1], [0], 0, False), ([256], [130000], 0, True), ([8] * 64, [2000] * 64, 0, False if kind == "tcgen05" else None)):
         ends = [c + k for c, k in zip(cached, nodes)]
-        splits, share = ops.tree_shares(nodes, ends, window, 4, 8, sum(nodes) * 32, 128, 128, 1)
+        splits, share = ops.tree_shares(nodes, ends, window, 4, 8, sum(nodes) * 32, 128, 128, 1, kind)
         tiles = [(e - 1) // 64 - (max(0, e - k - window + 1) if window else 0) // 64 + 1 for e, k in zip(ends, nodes)]
-        assert 1 <= splits <= ops.TREE_MAX_SPLITS
+        assert 1 <= splits <= ops.TREE_MAX_SPLITS and split in (None, splits > 1)
         if splits == 1:
             assert share == 0
-            continue
-        assert share >= ops.TREE_MIN_SHARE and splits * share >= max(tiles) > (splits - 1) * share
-        blocks = sum(-(-k * 4 // 128) * 8 * -(-t // share) for k, t in zip(nodes, tiles))
-        assert blocks <= 148
+        else:
+            assert share >= 1 and splits * share >= max(tiles) > (splits - 1) * share
 
 
 # ---------------------------------------------------------------------------------------- drafted trees on the host
