@@ -481,19 +481,20 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 }
 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
-// bfloat16, head sizes 64 and 128.  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
+// bfloat16, head sizes 64, 128 and 256.  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
 // tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
 //   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn.  With 64 rows or fewer the tile holds them twice, with
 //                  32 four times, and of a key tile each copy's warps take a half or a quarter (their P is zero elsewhere): a row's thread has
 //                  to sit on the warp of its tensor-memory lane, and this way all four have exponentials to make.  Every copy of either group
-//                  has a maximum, sum and output of its own; they are joined at the end;
+//                  has a maximum, sum and output of its own; they are joined at the end.  Heads of 256 have one group (the outputs of two do not
+//                  fit into tensor memory);
 //   else           up to 256 rows: a query tile of 128 rows a group, both go through every key tile.
 // Per key tile and group:
 //   S = Q K^T      tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a group;
 //   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into shared memory.  The reference maximum moves only
 //                  when the true one has outrun it by 2^8, so O is rescaled in tensor memory a few times at most;
 //   O += P V       tcgen05.mma, M = 128, N = head size, V as it lies in the cache.
-// Warps: 8 of rows (those without rows have nothing to do, and nobody waits for them), for each group one that issues S and one that issues
+// Warps: four of rows a group (those without rows have nothing to do, and nobody waits for them), for each group one that issues S and one that issues
 // P V (an issuing thread pays some 230 cycles a wait and 60 to 90 an instruction, so two threads share that), one that gathers K and one
 // that gathers V into the 128-byte swizzle, through rings of STAGES tiles: page by page with TMA where pages are 8, 16, 32 or a multiple of 64
 // rows, else row by row with cp.async.
@@ -510,21 +511,21 @@ constexpr float RESCALE_STEP = 8.0f;          // log2 units the true maximum may
 template <int N> struct Width { static constexpr int value = N; };
 
 template <int D, bool STREAMS> struct Shape {
-    static constexpr int NQ = STREAMS ? 1 : 2;               // query tiles
+    static constexpr int GROUPS = D == 256 ? 1 : 2, NQ = STREAMS ? 1 : GROUPS;       // groups of row warps; query tiles
     static constexpr int DS = D / 64;         // 64-wide slabs of the head size
     static constexpr unsigned Q_BYTES = DS * QM * 128, K_BYTES = DS * KN * 128, P_BYTES = QM * 128;
-    static constexpr int STAGES = D == 128 ? (STREAMS ? 4 : 3) : (STREAMS ? 8 : 6);
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (STREAMS ? 4 : 3) : (STREAMS ? 8 : 6);
     static constexpr int LAG = STAGES >= 4 ? 2 : 1;           // a tile is announced when this many later ones have been asked for
-    static constexpr int THREADS = 32 * 14;
-    static constexpr unsigned TMEM_COLS = 512, O_COL = 4 * KN;
-    static constexpr int B_K_FULL = 0, B_V_FULL = STAGES, B_K_EMPTY = 2 * STAGES, B_V_EMPTY = 3 * STAGES, B_S = 4 * STAGES, B_P = B_S + 4,
-                         B_PV = B_P + 4, B_Q = B_PV + 4, B_V_LAND = B_Q + 2, N_BARS = B_V_LAND + STAGES;
+    static constexpr int W_ISSUE = 4 * GROUPS, W_LOAD = 6 * GROUPS, THREADS = 32 * (W_LOAD + 2);      // the first warps of the other roles
+    static constexpr unsigned TMEM_COLS = 512, O_COL = GROUPS * 2 * KN;
+    static constexpr int B_K_FULL = 0, B_V_FULL = STAGES, B_K_EMPTY = 2 * STAGES, B_V_EMPTY = 3 * STAGES, B_S = 4 * STAGES,
+                         B_P = B_S + 2 * GROUPS, B_PV = B_P + 2 * GROUPS, B_Q = B_PV + 2 * GROUPS, B_V_LAND = B_Q + GROUPS, N_BARS = B_V_LAND + STAGES;
     static constexpr unsigned TAIL = N_BARS * 8 + 16 + TREE_MAX_NODES * 4;
-    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 4 * P_BYTES + TAIL;
+    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 2 * GROUPS * P_BYTES + TAIL;
     static constexpr unsigned SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;       // one CTA an SM: it takes all of the tensor memory
-    static_assert(SMEM <= 227 * 1024 && O_COL + 2 * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
-    static_assert(2 * STAGES * K_BYTES + 4 * P_BYTES >= 2 * QM * D * 4, "room for the outputs behind Q");
-    static_assert(!STREAMS || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
+    static_assert(SMEM <= 227 * 1024 && O_COL + GROUPS * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
+    static_assert(2 * STAGES * K_BYTES + 2 * GROUPS * P_BYTES >= GROUPS * QM * D * 4, "room for the outputs behind Q");
+    static_assert(!STREAMS || GROUPS == 1 || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
 };
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -541,6 +542,11 @@ __device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& 
 __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
     unsigned long long d;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
@@ -574,8 +580,8 @@ struct Paging {
     __device__ __forceinline__ int row(int j) const { return shift >= 0 ? j & (page_size - 1) : j % page_size; }
 };
 
-// grid: (row blocks x kv heads, segments, splits).
-template <int D, bool STREAMS>
+// grid: (row blocks x kv heads, segments, splits).  CAP: scores are capped (the plain kernel is spared the registers).
+template <int D, bool STREAMS, bool CAP>
 __global__ void __launch_bounds__(Shape<D, STREAMS>::THREADS, 1)
 tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpool, const bf16* __restrict__ vpool,
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
@@ -584,7 +590,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 float softcap, const float* __restrict__ sink, int share, int* __restrict__ status, int by_tma,
                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     typedef Shape<D, STREAMS> S;
-    constexpr int STAGES = S::STAGES, NQ = S::NQ;
+    constexpr int STAGES = S::STAGES, NQ = S::NQ, GROUPS = S::GROUPS, W_ISSUE = S::W_ISSUE, W_LOAD = S::W_LOAD;
     // The swizzled tiles need 1024-byte alignment: the kernel has no static shared memory, so its window starts at the CTA's base.
     extern __shared__ __align__(1024) unsigned char tc5_smem[];
     if ((smem_u32(tc5_smem) & 1023u) != 0u) {
@@ -595,7 +601,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     unsigned char* sK = sQ + NQ * S::Q_BYTES;                 // [stage]
     unsigned char* sV = sK + STAGES * S::K_BYTES;             // [stage]
     unsigned char* sP = sV + STAGES * S::K_BYTES;             // [group][buffer]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sP + 4 * S::P_BYTES);
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sP + 2 * GROUPS * S::P_BYTES);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + S::N_BARS);
     volatile int* odd_values = reinterpret_cast<int*>(tmem_slot + 1);
     int* parent = reinterpret_cast<int*>(tmem_slot + 4);
@@ -617,15 +623,15 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const int copy_rows = rows > 64 ? 128 : rows > 32 ? 64 : 32, copies = STREAMS ? QM / copy_rows : 1;
     // a group's rows (as warps), its key tiles, and the number of its i-th among the CTA's
     auto active_warps = [&](int g) { return STREAMS && copies > 1 ? 4 : max(0, min(4, (rows - (STREAMS ? 0 : g * QM) + 31) >> 5)); };
-    auto tiles_of = [&](int g) { return STREAMS ? (n_tiles - g + 1) >> 1 : active_warps(g) > 0 ? n_tiles : 0; };
-    auto tile_no = [&](int g, int i) { return STREAMS ? 2 * i + g : i; };
+    auto tiles_of = [&](int g) { return STREAMS ? (n_tiles - g + GROUPS - 1) / GROUPS : active_warps(g) > 0 ? n_tiles : 0; };
+    auto tile_no = [&](int g, int i) { return STREAMS ? GROUPS * i + g : i; };
     // whether every row sees every key of a tile
     auto whole = [&](int j_base) { return j_base + KN - 1 < sg.c && (window <= 0 || j_base > sg.c + sg.n - 1 - window); };
 
     // Everything that waits for memory is asked for before the barrier: queries, parents, the loaders' first pages.
     constexpr int LPR = D / 8, RPI = 32 / LPR;                // lanes a row of 16-byte pieces, rows an instruction
     const int rsel = lane / LPR, sub = lane % LPR;
-    if (warp < 8 && (!STREAMS || warp < 4) && (warp & 3) < active_warps(warp >> 2)) {
+    if (warp < W_ISSUE && (!STREAMS || warp < 4) && (warp & 3) < active_warps(warp >> 2)) {
         unsigned char* tile = sQ + (STREAMS ? 0 : warp >> 2) * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
 #pragma unroll 4
         for (int i = 0; i < 32 / RPI; ++i) {                  // a row's pieces by neighbouring lanes
@@ -641,8 +647,8 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const int box = min(pg.page_size, KN), pi = lane / S::DS, slab = lane % S::DS;       // a loader's lane by TMA: page of the tile, slab
     auto in_sight = [&](int jt) { const int j = jt * KN + pi * box; return pi * box < KN && j + box > sg.lo && j <= sg.hi; };
     auto ask_page = [&](int jt) { return in_sight(jt) ? bt_row[pg.block(jt * KN + pi * box)] : -1; };
-    int next = warp >= 12 && by_tma ? ask_page(jt_begin) : -1;
-    if (warp == 8) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
+    int next = warp >= W_LOAD && by_tma ? ask_page(jt_begin) : -1;
+    if (warp == W_ISSUE) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
     if (tid < S::N_BARS) {
         const int i = tid;
         int count = 1;
@@ -659,16 +665,16 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const unsigned tmem = *tmem_slot;
     bool ok = true;
 
-    const int grp = warp < 8 ? warp >> 2 : ((warp - 8) >> 1) & 1;              // group of a row warp or an issuer
+    const int grp = warp < W_ISSUE ? warp >> 2 : warp < W_LOAD ? (warp - W_ISSUE) >> 1 : 0;      // group of a row warp or an issuer
     const int qt = STREAMS ? 0 : grp, n_mine = tiles_of(grp);
-    const bool has_rows = warp < 8 && (warp & 3) < active_warps(grp);
+    const bool has_rows = warp < W_ISSUE && (warp & 3) < active_warps(grp);
     // a row thread's row of the tile (its lane of tensor memory), its copy, its row in the CTA, of the segment and head
     const int r = (warp & 3) * 32 + lane, copy = STREAMS ? r / copy_rows : 0, in_cta = STREAMS ? r & (copy_rows - 1) : qt * QM + r, row = row0 + in_cta;
     const bool row_valid = has_rows && in_cta < rows;
     const int2 node_head = by_group(row_valid ? row : 0);
     const size_t token = (size_t)sg.q_begin + node_head.x;
     const int h = kvh * G + node_head.y;
-    const float scale_log2 = scale * LOG2E, scale_eff = softcap > 0.f ? softcap * LOG2E : scale_log2;
+    const float scale_log2 = scale * LOG2E, scale_eff = CAP ? softcap * LOG2E : scale_log2;
     unsigned line[TREE_WORDS];
     int lo_r = 0;
     float m_ref = -INFINITY, l_run = 0.f;                     // the reference maximum and the sum relative to it
@@ -712,10 +718,28 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     for (int c = 0; c < W; c += 32) tmem_ld32(from + c, reinterpret_cast<unsigned(&)[32]>(a[c]));
                 }
                 tmem_ld_wait();
-                if (softcap > 0.f) {
+                if (CAP) {                                    // a polynomial where all of the warp's scores are well below the cap
                     const float k = scale / softcap;
+                    float far = 0.f;
 #pragma unroll
-                    for (int e = 0; e < W; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+                    for (int e = 0; e < W; e += 2) far = max3(far, fabsf(__uint_as_float(a[e])), fabsf(__uint_as_float(a[e + 1])));
+                    if (!__any_sync(0xffffffffu, !(far * k <= TANH_POLY_MAX))) {
+                        const unsigned long long k2 = pack2(k, k);
+#pragma unroll
+                        for (int e = 0; e < W; e += 2) {
+                            const unsigned long long x = mul2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), k2), u = mul2(x, x);
+                            unsigned long long t = fma2(u, pack2(TANH_P4, TANH_P4), pack2(TANH_P3, TANH_P3));
+                            t = fma2(u, t, pack2(TANH_P2, TANH_P2));
+                            t = fma2(u, t, pack2(TANH_P1, TANH_P1));
+                            float t0, t1;
+                            unpack2(mul2(x, fma2(u, t, pack2(TANH_P0, TANH_P0))), t0, t1);
+                            a[e] = __float_as_uint(t0);
+                            a[e + 1] = __float_as_uint(t1);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < W; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+                    }
                 }
                 if (!whole(j_base)) {
                     const unsigned long long vis = visible(j_base) >> col;
@@ -782,7 +806,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         else if (copies == 2) walk(Width<32>());
         else walk(Width<16>());
         if (n_mine > 0) ok = mbar_wait(bar(S::B_PV + grp * 2 + ((n_mine - 1) & 1)), ((n_mine - 1) >> 1) & 1) && ok;
-    } else if (warp >= 8 && warp < 12 && n_mine > 0 && lane == 0) {
+    } else if (warp >= W_ISSUE && warp < W_LOAD && n_mine > 0 && lane == 0) {
         // ================================================================== an issuing thread: descriptors are a base plus a constant
         ok = mbar_wait(bar(S::B_Q + qt), 0) && ok;
         fence_after_sync();
@@ -821,9 +845,9 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 mma_commit(bar(S::B_V_EMPTY + st));
             }
         }
-    } else if (warp >= 12) {
+    } else if (warp >= W_LOAD) {
         // ================================================================== the loaders
-        const bool is_k = warp == 12;
+        const bool is_k = warp == W_LOAD;
         const bf16* pool = is_k ? kpool : vpool;
         unsigned char* ring = is_k ? sK : sV;
         const int b_full = is_k ? S::B_K_FULL : S::B_V_FULL, b_empty = is_k ? S::B_K_EMPTY : S::B_V_EMPTY;
@@ -941,14 +965,14 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     // The rows leave through shared memory, where K, V and P lay: each (group, copy) its outputs in float32, brought to the row's common maximum,
     // a row of D by 16-byte pieces, piece p of row x at p ^ (x % 8).
     float2* stats = reinterpret_cast<float2*>(sQ);            // [group][tile row]: maximum and sum
-    float* row_inv = reinterpret_cast<float*>(stats + 2 * QM);
+    float* row_inv = reinterpret_cast<float*>(stats + GROUPS * QM);
     pdl_trigger_late();
     fence_before_sync();
     __syncthreads();                                          // no product reads shared memory any more
     fence_after_sync();
     if (has_rows) stats[grp * QM + r] = make_float2(m_ref, l_run);
     __syncthreads();
-    const int groups = STREAMS && n_tiles == 1 ? 1 : 2;       // STREAMS: those that have had a tile
+    const int groups = STREAMS && n_tiles == 1 ? 1 : GROUPS;  // STREAMS: those that have had a tile
     if (has_rows && n_mine > 0) {
         float mu = m_ref == -INFINITY ? 0.f : m_ref, mine = 1.f;
         if (STREAMS) {
@@ -999,7 +1023,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                         float s = 0.f;
                         const bf16* qrow = q + token * ld + (size_t)h * D;
                         for (int d = 0; d < D; ++d) s = fmaf(__bfloat162float(qrow[d]), __bfloat162float(kpool[key + d]), s);
-                        s = softcap > 0.f ? fast_tanh(s * (scale / softcap)) : s;
+                        s = CAP ? fast_tanh(s * (scale / softcap)) : s;
                         const float p = fast_exp2(fmaf(s, scale_eff, -mu));
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
@@ -1017,7 +1041,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     if (!ok) atomicExch(status, 1);
     fence_before_sync();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem, S::TMEM_COLS);
+    if (warp == W_ISSUE) tmem_dealloc(tmem, S::TMEM_COLS);
     // a row's partial outputs added, whole lines written: a thread four columns
     const bool parted = sg.n_split > 1;
     const int slots = STREAMS ? groups * copies : 1;
@@ -1156,13 +1180,13 @@ int mma_any(const TreeCall& a) {
     return a.D <= 128 ? mma_launch<TA, 128>(a) : mma_launch<TA, 256>(a);
 }
 
-template <int D, bool STREAMS>
-int tc5_launch(const TreeCall& a) {
+template <int D, bool STREAMS, bool CAP>
+int tc5_kernel_launch(const TreeCall& a) {
     typedef Shape<D, STREAMS> S;
     constexpr int ROWS = S::NQ * QM;
     static PerDevice configured;
     const int rc = configured.once([&](int) {
-        return cudaFuncSetAttribute(tree_tc5_kernel<D, STREAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        return cudaFuncSetAttribute(tree_tc5_kernel<D, STREAMS, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     });
     if (rc) return rc;
     // pages are whole boxes of whole groups of eight rows, and their rows can be counted in 31 bits
@@ -1173,10 +1197,15 @@ int tc5_launch(const TreeCall& a) {
     if (by_tma && !(tma::make_map_bf16(&kmap, a.kpool, (int)pool_rows, D, D, box) && tma::make_map_bf16(&vmap, a.vpool, (int)pool_rows, D, D, box)))
         return (int)cudaErrorInvalidValue;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
-    const int e = rb_launch_pdl(tree_tc5_kernel<D, STREAMS>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
+    const int e = rb_launch_pdl(tree_tc5_kernel<D, STREAMS, CAP>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
                                 (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, (bf16*)a.out, a.scratch,
                                 a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
+}
+
+template <int D, bool STREAMS>
+int tc5_launch(const TreeCall& a) {
+    return a.softcap > 0.f ? tc5_kernel_launch<D, STREAMS, true>(a) : tc5_kernel_launch<D, STREAMS, false>(a);
 }
 
 }  // namespace
@@ -1185,7 +1214,7 @@ RB_EXPORT int rb_tree_max_nodes() { return TREE_MAX_NODES; }
 
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys
 // go to one CTA for every `share` key tiles of 64, `splits` at most; scratch then holds splits * total_rows * Hq * (D + 2) floats.
-// query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, pools and
+// query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, or 256 with one; pools and
 // queries on 16-byte boundaries, ld a multiple of 8).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
                                 const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
@@ -1198,8 +1227,9 @@ RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const 
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
                   D, pages, scale, window, softcap, sink, splits, share, (float*)scratch, status, st};
     if (query_tiles > 0) {
-        if (act_dtype != RB_BF16 || (D != 64 && D != 128) || query_tiles > 2 || status == nullptr) return (int)cudaErrorInvalidValue;
+        if (act_dtype != RB_BF16 || (D != 64 && D != 128 && D != 256) || query_tiles > (D == 256 ? 1 : 2) || status == nullptr) return (int)cudaErrorInvalidValue;
         if ((((uintptr_t)q | (uintptr_t)kpool | (uintptr_t)vpool | (uintptr_t)out) & 15) || ld % 8) return (int)cudaErrorInvalidValue;
+        if (D == 256) return tc5_launch<256, true>(a);
         if (D == 64) return query_tiles == 1 ? tc5_launch<64, true>(a) : tc5_launch<64, false>(a);
         return query_tiles == 1 ? tc5_launch<128, true>(a) : tc5_launch<128, false>(a);
     }

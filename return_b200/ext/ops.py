@@ -2244,6 +2244,7 @@ _tree = _branch = None
 
 TREE_MAX_NODES = 256               # drafted nodes of a segment
 TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
+TREE_TC5_HEAD_DIMS = (64, 128, 256)
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
 TREE_MAX_SPLITS = 64
 TREE_SCRATCH_BYTES = 256 << 20
@@ -2321,33 +2322,37 @@ def _tree_lengths(batch, page_size: int, blocks: int):
     return held
 
 
-# What a CTA costs beside its key tiles, and what the merge of split keys costs, in key tiles of the kernel: the tcgen05 kernel's tiles take half a
-# microsecond each, those of the kernel for any type and head size 1.6 (bfloat16) and 4 (float32).  Measured in tree steps of 1 to 64
-# requests behind 500 to 8,000 tokens; one tree of 8 nodes behind 500: 10.3 us unsplit, 11.8 split in four.
-TREE_COSTS = {"tcgen05": (12.0, 8.0), "bfloat16": (3.0, 2.5), "float32": (1.5, 1.0)}
+# By kernel: what a CTA costs beside its key tiles, and what the merge of split keys costs, in key tiles; how long a tile takes (us).  The partial
+# results are written and read at TREE_HBM bytes a us besides.  Measured in tree steps of 1 to 64 requests behind 500 to 8,000 tokens;
+# one tree of 8 nodes behind 500: 10.3 us unsplit, 11.8 split in four.
+TREE_COSTS = {"tcgen05": (12.0, 8.0, 0.55), "bfloat16": (3.0, 2.5, 1.6), "float32": (1.5, 1.0, 4.0)}
+TREE_HBM = 5.5e6
 TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64)
 
 
 def tree_shares(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int, kind: str):
     """(splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; (1, 0): no split.  Of shares that
-    cut the longest walk into a number of TREE_PARTS, the one whose launch is done first: rounds of CTAs times a CTA's cost, and the merge."""
+    cut the longest walk into a number of TREE_PARTS, the one whose launch is done first."""
     tiles = [(e - 1) // TREE_KEY_TILE - (max(0, e - k - window + 1) if window else 0) // TREE_KEY_TILE + 1 for k, e in zip(nodes, ends)]
     blocks = [-(-k * rows_per_node // cta_rows) * kv_heads for k in nodes]
     slots, longest = num_sms() * ctas_per_sm, max(tiles)
-    fixed, merge = TREE_COSTS[kind]
+    fixed, merge, tile_us = TREE_COSTS[kind]
+    total = sum([b * t for b, t in zip(blocks, tiles)])
+    part_bytes = rows * (head_dim + 2) * 4
 
-    def done(ctas, share):                             # rounds count in parts: a last one that is not full is still a round for those in it
-        return max(1.0, -(-ctas // slots) - 0.3 if ctas > slots else 1.0) * (share + fixed)
+    def done(ctas, top):                               # one round: the longest CTA; more: the load, and half of an average CTA behind it
+        if ctas <= slots:
+            return top + fixed
+        return max(top + fixed, (total + ctas * fixed) / slots + 0.5 * (total / ctas + fixed))
 
     best, best_done = (1, 0), done(sum(blocks), longest)
-    most = min(TREE_MAX_SPLITS, TREE_SCRATCH_BYTES // max(1, rows * (head_dim + 2) * 4))
     for parts in TREE_PARTS:
         share = -(-longest // parts)
         splits = -(-longest // share)
-        if splits > most or splits == 1:
+        if splits == 1 or splits > TREE_MAX_SPLITS or splits * part_bytes > TREE_SCRATCH_BYTES:
             break
         ctas = sum([b * -(-t // share) for b, t in zip(blocks, tiles)])
-        d = done(ctas, share) + merge * (1.0 + 0.03 * splits)
+        d = done(ctas, share) + merge + 2 * splits * part_bytes / TREE_HBM / tile_us
         if d < best_done:
             best, best_done = (splits, share), d
         if ctas > 2 * slots:
@@ -2394,7 +2399,7 @@ def _tree_plan(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_head
     if block_table.dim() != 2:
         raise KernelError("block_table: int32 [segments, blocks]")
     n, rows, longest, _, _ = _tree_lengths(batch, page_size, block_table.shape[1])
-    if not (num_heads % num_kv_heads == 0 and 0 < head_dim <= 256):
+    if not (num_kv_heads > 0 and num_heads % num_kv_heads == 0 and 0 < head_dim <= 256):
         raise KernelError("query heads: a multiple of the kv heads; head size: up to 256")
     if not (qkv.dim() == 2 and qkv.shape[0] == rows and qkv.shape[1] >= num_heads * head_dim):
         raise KernelError("qkv: a row per node, of the query heads at least")
@@ -2416,8 +2421,8 @@ def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_head
     _, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
     group = num_heads // num_kv_heads
     tiles = 0                                          # the tensor cores take up to two tiles of TREE_TILE_ROWS rows a CTA
-    if kind and dtype == torch.bfloat16 and head_dim in TC5_ATTENTION_HEAD_DIMS:
-        tiles = 1 if longest * group <= TREE_TILE_ROWS else 2
+    if kind and dtype == torch.bfloat16 and head_dim in TREE_TC5_HEAD_DIMS:
+        tiles = 1 if longest * group <= TREE_TILE_ROWS or head_dim == 256 else 2
     return (tiles,) + tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim, tiles * TREE_TILE_ROWS or 32,
                                   1 if tiles or head_dim > 128 else 2, "tcgen05" if tiles else "float32" if dtype == torch.float32 else "bfloat16")
 

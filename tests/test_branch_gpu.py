@@ -113,6 +113,14 @@ SHAPES = [  # heads, kv heads, head size, page, cached, nodes, kind
     (6, 3, 48, 8, [77, 12], [9, 20], "random"),
     (4, 1, 256, 16, [33, 200], [5, 11], "random"),
     (2, 1, 16, 5, [31], [6], "chain"),
+    (8, 2, 256, 16, [300, 64, 2], [70, 33, 8], "random"),
+    (8, 2, 128, 32, [300, 64, 2], [20, 3, 8], "random"),
+    (8, 2, 128, 128, [300, 64, 2], [12, 3, 8], "random"),
+    (8, 2, 64, 24, [300, 64, 2], [12, 3, 40], "random"),
+    (12, 2, 128, 16, [700, 1], [16, 5], "random"),
+    (2, 1, 8, 4, [100], [9], "random"),
+    (2, 1, 6, 4, [100], [9], "random"),
+    (4, 2, 200, 16, [100], [30], "random"),
 ]
 
 
@@ -126,7 +134,7 @@ def test_tree_attention(shape, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("options", [dict(window=1), dict(window=3), dict(window=70), dict(window=5000), dict(softcap=2.0), dict(sink=True),
                                      dict(window=100, softcap=5.0, sink=True)], ids=str)
-@pytest.mark.parametrize("D", [64, 128, 32])
+@pytest.mark.parametrize("D", [64, 128, 256, 32])
 def test_tree_attention_options(D, options, dtype):
     a = Attention(5, dtype, 8, 2, D, 16, [200, 0, 65, 1500], [20, 9, 1, 40], kind="random", pad=16, **options)
     a.check(a.run())
@@ -144,7 +152,7 @@ def test_tree_attention_shares(splits, share, heads, nodes, dtype, monkeypatch):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-@pytest.mark.parametrize("heads,D", [(4, 128), (16, 64), (4, 48)])
+@pytest.mark.parametrize("heads,D", [(4, 128), (16, 64), (4, 48), (4, 256)])
 def test_what_a_node_does_not_see_does_not_reach_it(heads, D, value, dtype):
     """One node's value (and, in another run, its key) is no number: only its descendants may show it."""
     for name in ("v", "k"):
