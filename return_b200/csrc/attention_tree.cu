@@ -6,7 +6,8 @@
 // window both must lie less than `window` positions back: j > c + depth(i) - window, depth(i) - depth(a) < window.
 //   s = scale q.k   (softcap > 0: softcap tanh(s / softcap))
 //   out = sum_j exp(s_j - m) v_j / (sum_j exp(s_j - m) + exp(sink[h] - m))
-// A block that the table marks as gone (-1) reads as keys and values of zero; a row that sees no key gets zeros.
+// A block that the table marks as gone (-1), or whose page the pool does not have, reads as keys and values of zero; a row that sees no key
+// gets zeros.
 //
 // Which ancestors a node has is not read from a mask: a thread walks up its parents once (the list of a segment, at most
 // TREE_MAX_NODES, is in shared memory) and keeps the bits.  A parent that is not below its child ends the walk, so a list that is no
@@ -43,6 +44,12 @@ struct Segment {
         n_split = share > 0 ? min(max_split, max(1, (tiles + share - 1) / share)) : 1;
     }
 };
+
+// A block table's entry: the page, -1 where there is none.
+__device__ __forceinline__ int page_at(const int* entry, int pages) {
+    const int page = *entry;
+    return (unsigned)page < (unsigned)pages ? page : -1;
+}
 
 // x / G and x % G for the rows of a CTA: a quotient by the reciprocal, put right where it is one off.
 struct ByGroup {
@@ -134,7 +141,7 @@ __device__ __forceinline__ void mma_parts(float (&big)[4], float (&rest)[4], con
     mma16(rest, am, b0.h, b1.h);
 }
 // Whether the products cannot take a value.
-__device__ __forceinline__ bool is_odd(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x77800000u; }        // |x| >= 2^112, or no number
+__device__ __forceinline__ bool is_odd(float x) { return (__float_as_uint(x) & 0x7fffffffu) >= 0x73800000u; }        // |x| >= 2^104 (times 2^16, 64 of them are still numbers), or no number
 __device__ __forceinline__ bool is_odd(bf16 x) { return (__bfloat16_as_ushort(x) & 0x7f80u) == 0x7f80u; }
 
 template <typename TA, int DP> struct MmaShape {
@@ -150,7 +157,7 @@ template <typename TA, int DP>
 __global__ void __launch_bounds__(MTHREADS, DP <= 128 ? 2 : 1)
 tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, const TA* __restrict__ vpool,
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
-                const int* __restrict__ block_table, int bt_stride, int page_size, TA* __restrict__ out,
+                const int* __restrict__ block_table, int bt_stride, int page_size, int pages, TA* __restrict__ out,
                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, int D, float scale, int window,
                 float softcap, const float* __restrict__ sink, int share, int vec) {
     typedef MmaShape<TA, DP> S;
@@ -182,7 +189,7 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
     // Where a tile's rows lie in a pool, -1: no key of this CTA's, or a block marked as gone.
     auto locate = [&](int jt) {
         if (tid < KEY_TILE) {
-            const int j = jt * KEY_TILE + tid, page = j >= sg.lo && j <= sg.hi ? bt[j / page_size] : -1;
+            const int j = jt * KEY_TILE + tid, page = j >= sg.lo && j <= sg.hi ? page_at(bt + j / page_size, pages) : -1;
             where[jt & 1][tid] = page < 0 ? -1 : (((long long)page * Hkv + kvh) * page_size + j % page_size) * D;
         }
     };
@@ -585,7 +592,7 @@ template <int D, bool STREAMS, bool CAP>
 __global__ void __launch_bounds__(Shape<D, STREAMS>::THREADS, 1)
 tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpool, const bf16* __restrict__ vpool,
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
-                const int* __restrict__ block_table, int bt_stride, int page_size, bf16* __restrict__ out,
+                const int* __restrict__ block_table, int bt_stride, int page_size, int pages, bf16* __restrict__ out,
                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, float scale, int window,
                 float softcap, const float* __restrict__ sink, int share, int* __restrict__ status, int by_tma,
                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -646,7 +653,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     for (int i = tid; i < sg.n; i += S::THREADS) parent[i] = tree_parent[sg.q_begin + i];
     const int box = min(pg.page_size, KN), pi = lane / S::DS, slab = lane % S::DS;       // a loader's lane by TMA: page of the tile, slab
     auto in_sight = [&](int jt) { const int j = jt * KN + pi * box; return pi * box < KN && j + box > sg.lo && j <= sg.hi; };
-    auto ask_page = [&](int jt) { return in_sight(jt) ? bt_row[pg.block(jt * KN + pi * box)] : -1; };
+    auto ask_page = [&](int jt) { return in_sight(jt) ? page_at(bt_row + pg.block(jt * KN + pi * box), pages) : -1; };
     int next = warp >= W_LOAD && by_tma ? ask_page(jt_begin) : -1;
     if (warp == W_ISSUE) tmem_alloc(smem_u32(tmem_slot), S::TMEM_COLS);
     if (tid < S::N_BARS) {
@@ -915,7 +922,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int j = jt * KN + u * 32 + lane;
-                    page[u] = j >= sg.lo && j <= sg.hi ? bt_row[pg.block(j)] : -1;
+                    page[u] = j >= sg.lo && j <= sg.hi ? page_at(bt_row + pg.block(j), pages) : -1;
                 }
             };
             auto announce = [&](int t) {                      // tile t has landed
@@ -1013,7 +1020,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     const int j_base = (jt_begin + t) * KN;
                     if (whole(j_base)) continue;
                     for (unsigned long long vis = visible(j_base); vis != 0ull; vis &= vis - 1ull) {
-                        const int j = j_base + __ffsll((long long)vis) - 1, page = bt_row[pg.block(j)];
+                        const int j = j_base + __ffsll((long long)vis) - 1, page = page_at(bt_row + pg.block(j), pages);
                         if (page < 0) continue;
                         const size_t key = (((size_t)page * Hkv + kvh) * pg.page_size + pg.row(j)) * D;
                         unsigned any = 0u;
@@ -1169,7 +1176,7 @@ int mma_launch(const TreeCall& a) {
     const int vec = a.D * sizeof(TA) % 16 == 0 && (((uintptr_t)a.kpool | (uintptr_t)a.vpool) & 15) == 0;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + MROWS - 1) / MROWS * a.Hkv, a.segments, a.splits);
     const int e = rb_launch_pdl(tree_mma_kernel<TA, DP>, grid, dim3(MTHREADS), SMEM, a.st, (const TA*)a.q, a.ld, (const TA*)a.kpool,
-                                (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, (TA*)a.out, a.scratch,
+                                (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (TA*)a.out, a.scratch,
                                 a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, vec);
     return e ? e : merge<TA>(a);
 }
@@ -1198,7 +1205,7 @@ int tc5_kernel_launch(const TreeCall& a) {
         return (int)cudaErrorInvalidValue;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
     const int e = rb_launch_pdl(tree_tc5_kernel<D, STREAMS, CAP>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
-                                (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, (bf16*)a.out, a.scratch,
+                                (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (bf16*)a.out, a.scratch,
                                 a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
 }

@@ -2322,42 +2322,55 @@ def _tree_lengths(batch, page_size: int, blocks: int):
     return held
 
 
-# By kernel: what a CTA costs beside its key tiles, and what the merge of split keys costs, in key tiles; how long a tile takes (us).  The partial
-# results are written and read at TREE_HBM bytes a us besides.  Measured in tree steps of 1 to 64 requests behind 500 to 8,000 tokens;
-# one tree of 8 nodes behind 500: 10.3 us unsplit, 11.8 split in four.
-TREE_COSTS = {"tcgen05": (12.0, 8.0, 0.55), "bfloat16": (3.0, 2.5, 1.6), "float32": (1.5, 1.0, 4.0)}
+# What a launch costs, by kernel, in us: a CTA beside its key tiles (heads of 128; 60 % of it whatever the head size), a key tile as a + b times
+# the head size / 128, the merge of split keys as a + b times the splits, which part of a CTA's time the last ones stand alone where there
+# are more than fit at once, and by how much a tile is slower where two CTAs share an SM.  Partial results are written and read, and keys
+# and values read, at TREE_HBM bytes a us.  Fitted to 620 launches (1 to 16 requests behind 60 to 8,000 tokens, trees of 4 to 32 nodes, heads of 64
+# to 256, each split in up to 12 ways): on average the choice is 1 % slower than the best of them, at worst 15.
+TREE_COSTS = {"tcgen05": (7.1, 0.38, 0.49, 2.6, 0.064, 0.33, 0.0), "bfloat16": (4.4, 0.70, 1.61, 2.9, 0.057, 0.27, 0.41),
+              "float32": (3.1, 1.32, 4.26, 2.9, 0.113, 0.25, 0.47)}
 TREE_HBM = 5.5e6
-TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64)
+TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20, 24, 32, 48, 64)
 
 
-def tree_shares(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int, kind: str):
-    """(splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; (1, 0): no split.  Of shares that
-    cut the longest walk into a number of TREE_PARTS, the one whose launch is done first."""
+def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int, kind: str):
+    """(us, splits, share): a segment's keys go to one CTA for every ``share`` key tiles, ``splits`` at most; splits 1, share 0: no split.  Of
+    shares that cut the longest walk into a number of TREE_PARTS, the one whose launch is done first, and when."""
     tiles = [(e - 1) // TREE_KEY_TILE - (max(0, e - k - window + 1) if window else 0) // TREE_KEY_TILE + 1 for k, e in zip(nodes, ends)]
     blocks = [-(-k * rows_per_node // cta_rows) * kv_heads for k in nodes]
-    slots, longest = num_sms() * ctas_per_sm, max(tiles)
-    fixed, merge, tile_us = TREE_COSTS[kind]
+    sms, longest = num_sms(), max(tiles)
+    fixed, tile, tile_dim, merge, merge_split, alone, shared = TREE_COSTS[kind]
+    fixed, tile = fixed * (0.6 + 0.4 * head_dim / 128), tile + tile_dim * head_dim / 128
+    slots = sms * ctas_per_sm if ctas_per_sm > 1 else 0.93 * sms             # a launch that takes every SM waits for the last one's CTAs
     total = sum([b * t for b, t in zip(blocks, tiles)])
-    part_bytes = rows * (head_dim + 2) * 4
+    part_us = 2 * rows * (head_dim + 2) * 4 / TREE_HBM
+    least = sum(tiles) * TREE_KEY_TILE * kv_heads * head_dim * (8 if kind == "float32" else 4) / TREE_HBM + 0.5 * fixed
 
-    def done(ctas, top):                               # one round: the longest CTA; more: the load, and half of an average CTA behind it
-        if ctas <= slots:
-            return top + fixed
-        return max(top + fixed, (total + ctas * fixed) / slots + 0.5 * (total / ctas + fixed))
+    def done(ctas, top):                               # one round: the longest CTA; more: the load, and a part of an average CTA behind it
+        each = tile * (1 + shared) if ctas_per_sm > 1 and ctas > sms else tile
+        longest_cta = fixed + top * each
+        if ctas > slots:
+            longest_cta = max(longest_cta, (total * each + ctas * fixed) / slots + alone * (total / ctas * each + fixed))
+        return max(longest_cta, least)
 
-    best, best_done = (1, 0), done(sum(blocks), longest)
+    best = done(sum(blocks), longest), 1, 0
     for parts in TREE_PARTS:
         share = -(-longest // parts)
         splits = -(-longest // share)
-        if splits == 1 or splits > TREE_MAX_SPLITS or splits * part_bytes > TREE_SCRATCH_BYTES:
+        if splits == 1 or splits > TREE_MAX_SPLITS or splits * rows * (head_dim + 2) * 4 > TREE_SCRATCH_BYTES:
             break
         ctas = sum([b * -(-t // share) for b, t in zip(blocks, tiles)])
-        d = done(ctas, share) + merge + 2 * splits * part_bytes / TREE_HBM / tile_us
-        if d < best_done:
-            best, best_done = (splits, share), d
+        us = done(ctas, share) + merge + splits * (merge_split + part_us)
+        if us < best[0]:
+            best = us, splits, share
         if ctas > 2 * slots:
             break
     return best
+
+
+def tree_shares(*step):
+    """(splits, share) of ``tree_cost``."""
+    return tree_cost(*step)[1:]
 
 
 def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window=None,
@@ -2366,7 +2379,8 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     index in the segment of the node before it, below i, -1 for the root) has its key and value in slot ``seg_pos0 + i`` already and
     stands at position ``seg_pos0 + depth(i)``; it sees the segment's cached keys, its ancestors and itself, with a window those
     less than ``window`` positions back.  ``qkv``: rows that begin with the rotated queries (row stride any).  ``softcap``,
-    ``sink``: as in ``paged_attention``.  A segment has up to TREE_MAX_NODES nodes."""
+    ``sink``: as in ``paged_attention``.  A segment has up to TREE_MAX_NODES nodes.  A block that the table marks as gone (-1), or whose
+    page the pool does not have, reads as zeros."""
     key = (qkv.shape, k_pool.shape, v_pool.shape, out.shape, block_table.shape, qkv.dtype, page_size, num_heads, num_kv_heads, head_dim, window,
            scale, softcap, sink is None)
     plan = batch.scratch.get(key)                      # the step's layers are alike: what follows from shapes is looked at once
@@ -2420,11 +2434,19 @@ def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_head
     """(query tiles of the tensor cores' kernel or 0, splits, share) of a step's launches."""
     _, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
     group = num_heads // num_kv_heads
-    tiles = 0                                          # the tensor cores take up to two tiles of TREE_TILE_ROWS rows a CTA
-    if kind and dtype == torch.bfloat16 and head_dim in TREE_TC5_HEAD_DIMS:
-        tiles = 1 if longest * group <= TREE_TILE_ROWS or head_dim == 256 else 2
-    return (tiles,) + tree_shares(nodes, ends, window, group, num_kv_heads, rows * num_heads, head_dim, tiles * TREE_TILE_ROWS or 32,
-                                  1 if tiles or head_dim > 128 else 2, "tcgen05" if tiles else "float32" if dtype == torch.float32 else "bfloat16")
+    step = (nodes, ends, window, group, num_kv_heads, rows * num_heads)
+    # Any type and head size (rounded up to a power of two): tiles of 32 rows.
+    padded = next(d for d in (32, 64, 128, 256) if d >= head_dim)
+    any_kind = step + (padded, 32, 1 if padded > 128 else 2, "float32" if dtype == torch.float32 else "bfloat16")
+    if not (kind and dtype == torch.bfloat16 and head_dim in TREE_TC5_HEAD_DIMS):
+        return (0,) + tree_shares(*any_kind)
+    # The tensor cores' fifth generation, up to two tiles of TREE_TILE_ROWS rows a CTA, has more to set up: 16 query and 8 key heads of 128, a
+    # tree of 8 nodes behind 500 tokens 10.5 us against 9.5, four behind 2,000 18.4 against 21.2.
+    tiles = 1 if longest * group <= TREE_TILE_ROWS or head_dim == 256 else 2
+    own_kind = step + (head_dim, tiles * TREE_TILE_ROWS, 1, "tcgen05")
+    if tree_cost(*any_kind)[0] < tree_cost(*own_kind)[0]:
+        return (0,) + tree_shares(*any_kind)
+    return (tiles,) + tree_shares(*own_kind)
 
 
 def _pool_shape(pool):

@@ -150,6 +150,41 @@ def test_tree_attention_shares(splits, share, heads, nodes, dtype, monkeypatch):
     a.check(a.run())
 
 
+@pytest.fixture(params=["tcgen05", "bfloat16"])
+def kernel(request, monkeypatch):
+    """One of the two kernels that a bfloat16 step may run on, whatever it costs."""
+    monkeypatch.setitem(ops.TREE_COSTS, request.param, (0.0,) * 7)
+    launch = ops._tree_launch
+
+    def watched(*a):
+        got = launch(*a)
+        assert (got[0] > 0) == (request.param == "tcgen05")
+        return got
+
+    monkeypatch.setattr(ops, "_tree_launch", watched)
+
+
+@pytest.mark.parametrize("shape", [x for x in SHAPES if x[2] in ops.TREE_TC5_HEAD_DIMS], ids=lambda s: "-".join(map(str, s[:4])))
+def test_tree_attention_on_either_kernel(shape, kernel):
+    a = Attention(3, torch.bfloat16, *shape[:4], list(shape[4]), list(shape[5]), kind=shape[6])
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("options", [dict(window=3), dict(window=70), dict(softcap=2.0), dict(window=100, softcap=5.0, sink=True)], ids=str)
+@pytest.mark.parametrize("splits,share", [(1, 0), (7, 4)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tree_attention_options_on_either_kernel(D, options, splits, share, kernel, monkeypatch):
+    monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
+    a = Attention(5, torch.bfloat16, 8, 2, D, 16, [200, 0, 65, 1500], [20, 9, 1, 40], pad=16, **options)
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("heads,D", [(4, 128), (16, 64), (4, 256)])
+def test_what_a_node_does_not_see_does_not_reach_it_on_either_kernel(heads, D, value, kernel):
+    test_what_a_node_does_not_see_does_not_reach_it(heads, D, value, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("heads,D", [(4, 128), (16, 64), (4, 48), (4, 256)])
@@ -176,6 +211,30 @@ def test_what_a_node_does_not_see_does_not_reach_it(heads, D, value, dtype):
             else:
                 assert torch.equal(got[t], clean[t]), t
         del old
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("D", [128, 48])
+def test_blocks_that_are_gone_read_as_zeros(D, page, dtype):
+    """A table's -1, and a page that the pool does not have."""
+    a = Attention(17, dtype, 8, 2, D, page, [150, 20], [9, 3])
+    for t, block in ((0, 1), (0, 4), (1, 0)):
+        a.k[a.tables[t][block]] = a.v[a.tables[t][block]] = 0.0
+    a.check(a.run())
+    want = a.run()
+    pages = a.k.shape[0]
+    a.block_table[0, 1], a.block_table[0, 4], a.block_table[1, 0] = -1, pages, 2 ** 31 - 1
+    assert torch.equal(a.run(), want)
+
+
+def test_float32_values_near_the_end_of_the_type():
+    """The products' parts are scaled up; values that the scale would take beyond the type are added by themselves."""
+    a = Attention(19, torch.float32, 8, 2, 64, 16, [150, 20], [9, 3])
+    held = torch.isfinite(a.v)
+    for exponent in (100, 103, 104, 105, 111, 118):
+        a.v[held] = torch.sign(a.v[held]) * 2.0 ** exponent
+        a.check(a.run())
 
 
 def test_tree_attention_takes_what_the_documentation_allows():
