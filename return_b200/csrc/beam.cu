@@ -338,10 +338,10 @@ constexpr int HELD = 4;
 __global__ void __launch_bounds__(MERGE_THREADS)
 beam_merge_kernel(const float* __restrict__ scores, const float* __restrict__ part_ms, const Key* __restrict__ cand, int beams, int V, int parts,
                   int keep, float* __restrict__ scores_out, int* __restrict__ beams_out, int* __restrict__ tokens_out) {
-    constexpr int T = MERGE_THREADS, WARPS = T / 32, NOWHERE = 0x7fffffff;
+    constexpr int T = MERGE_THREADS, WARPS = T / 32;
     __shared__ double s_shift[BEAM_MAX_BEAMS];                // score - lse; NaN: the row counts as -inf
-    __shared__ double s_v[COLLECT], s_bv[WARPS];
-    __shared__ int s_at[COLLECT], s_n, s_bi[WARPS];
+    __shared__ double s_v[COLLECT];
+    __shared__ int s_at[COLLECT], s_n, s_count[2];
     __shared__ __align__(16) float s_list[T];
     __shared__ float s_pass;
     pdl_wait();
@@ -358,7 +358,7 @@ beam_merge_kernel(const float* __restrict__ scores, const float* __restrict__ pa
     Key first[HELD];                                          // asked for before the rows' sums are worked out
 #pragma unroll
     for (int u = 0; u < HELD; ++u) first[u] = tid + u * T < total ? mine[tid + u * T] : NONE;
-    if (tid == 0) { s_n = 0; s_pass = -INFINITY; }
+    if (tid == 0) { s_n = 0; s_pass = -INFINITY; s_count[0] = s_count[1] = 0; }
     for (int b = warp; b < beams; b += WARPS) {
         const float2* ms = reinterpret_cast<const float2*>(part_ms) + (size_t)(req * beams + b) * parts;
         const float score = scores[req * beams + b];
@@ -422,51 +422,68 @@ beam_merge_kernel(const float* __restrict__ scores, const float* __restrict__ pa
             if (at >= 0) f(v, at);
         }
     };
-    each([&](double v, int at) {
-        if (v >= pass) {
-            const int n = atomicAdd(&s_n, 1);
-            if (n < COLLECT) { s_v[n] = v; s_at[n] = at; }
-        }
-    });
-    __syncthreads();
-    const int n = s_n;
-    auto put = [&](int rank, double v, int at) {
-        const size_t to = (size_t)req * keep + rank;
-        scores_out[to] = (float)v;
-        beams_out[to] = at / V;
-        tokens_out[to] = at % V;
+    auto gather = [&](auto passes) {
+        each([&](double v, int at) {
+            if (passes(v, at)) {
+                const int n = atomicAdd(&s_n, 1);
+                if (n < COLLECT) { s_v[n] = v; s_at[n] = at; }
+            }
+        });
+        __syncthreads();
+        return s_n;
     };
-    if (n <= COLLECT) {
-        for (int i = tid; i < n; i += T) {
-            const double v = s_v[i];
-            const int at = s_at[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += before(s_v[j], s_at[j], v, at) ? 1 : 0;
-            if (rank < keep) put(rank, v, at);
+    int n = gather([&](double v, int) { return v >= pass; });
+    if (n > COLLECT) {
+        // Too many: the bar is put between them by halving, by their totals as integers of the same order, and where as many are equal, by their
+        // places.  `keep` pass `low` and do not pass `high`; of those whose total is the bar, last_at is the last place that passes.
+        auto order = [](double v) {
+            const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+            return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+        };
+        auto passes = [&](double v, int at, unsigned long long bar, int to) {
+            const unsigned long long o = order(v);
+            return o > bar || (o == bar && at <= to);
+        };
+        int round = 0;
+        auto count = [&](unsigned long long bar, int to) {
+            int passing = 0;
+            each([&](double v, int at) { passing += passes(v, at, bar, to) ? 1 : 0; });
+            passing = __reduce_add_sync(0xffffffffu, passing);
+            if (lane == 0) atomicAdd(&s_count[round], passing);
+            __syncthreads();
+            passing = s_count[round];
+            round ^= 1;
+            __syncthreads();
+            if (tid == 0) s_count[round ^ 1] = 0;             // added to again behind the next call's barriers
+            return passing;
+        };
+        unsigned long long low = order(pass), high = order((double)INFINITY) + 1;
+        int last_at = beams * V - 1;
+        bool fits = false;
+        while (!fits && high - low > 1) {
+            const unsigned long long mid = low + (high - low) / 2;
+            const int passing = count(mid, last_at);
+            if (passing >= keep) { low = mid; fits = passing <= COLLECT; } else high = mid;
         }
-        return;
+        for (int from = -1; !fits && last_at - from > 1;) {
+            const int mid = from + (last_at - from) / 2, passing = count(low, mid);
+            if (passing >= keep) { last_at = mid; fits = passing <= COLLECT; } else from = mid;
+        }
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        n = min(gather([&](double v, int at) { return passes(v, at, low, last_at); }), COLLECT);
     }
-    double last = (double)INFINITY;                           // too many: one by one
-    int last_at = -1;
-    for (int k = 0; k < keep; ++k) {
-        double best = none;
-        int best_at = NOWHERE;
-        auto better = [&](double v, int at) { if (before(v, at, best, best_at)) { best = v; best_at = at; } };
-        each([&](double v, int at) { if (before(last, last_at, v, at)) better(v, at); });
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(0xffffffffu, best, o);
-            const int at = __shfl_xor_sync(0xffffffffu, best_at, o);
-            better(v, at);
+    for (int i = tid; i < n; i += T) {
+        const double v = s_v[i];
+        const int at = s_at[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += before(s_v[j], s_at[j], v, at) ? 1 : 0;
+        if (rank < keep) {
+            const size_t to = (size_t)req * keep + rank;
+            scores_out[to] = (float)v;
+            beams_out[to] = at / V;
+            tokens_out[to] = at % V;
         }
-        if (lane == 0) { s_bv[warp] = best; s_bi[warp] = best_at; }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) better(s_bv[w], s_bi[w]);
-        __syncthreads();
-        if (tid == 0) put(k, best, best_at);
-        last = best;
-        last_at = best_at;
     }
 }
 
