@@ -498,9 +498,9 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 //   else           up to 256 rows: a query tile of 128 rows a group, both go through every key tile.
 // Per key tile and group:
 //   S = Q K^T      tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a group;
-//   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into shared memory.  The reference maximum moves only
+//   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into S's own columns.  The reference maximum moves only
 //                  when the true one has outrun it by 2^8, so O is rescaled in tensor memory a few times at most;
-//   O += P V       tcgen05.mma, M = 128, N = head size, V as it lies in the cache.
+//   O += P V       tcgen05.mma, M = 128, N = head size, P from tensor memory, V as it lies in the cache.
 // Warps: four of rows a group (those without rows have nothing to do, and nobody waits for them), for each group one that issues S and one that issues
 // P V (an issuing thread pays some 230 cycles a wait and 60 to 90 an instruction, so two threads share that), one that gathers K and one
 // that gathers V into the 128-byte swizzle, through rings of STAGES tiles: page by page with TMA where pages are 8, 16, 32 or a multiple of 64
@@ -520,18 +520,18 @@ template <int N> struct Width { static constexpr int value = N; };
 template <int D, bool STREAMS> struct Shape {
     static constexpr int GROUPS = D == 256 ? 1 : 2, NQ = STREAMS ? 1 : GROUPS;       // groups of row warps; query tiles
     static constexpr int DS = D / 64;         // 64-wide slabs of the head size
-    static constexpr unsigned Q_BYTES = DS * QM * 128, K_BYTES = DS * KN * 128, P_BYTES = QM * 128;
-    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (STREAMS ? 4 : 3) : (STREAMS ? 8 : 6);
+    static constexpr unsigned Q_BYTES = DS * QM * 128, K_BYTES = DS * KN * 128;
+    static constexpr int STAGES = D == 256 ? 2 : D == 128 ? (STREAMS ? 6 : 5) : (STREAMS ? 8 : 6);
     static constexpr int LAG = STAGES >= 4 ? 2 : 1;           // a tile is announced when this many later ones have been asked for
     static constexpr int W_ISSUE = 4 * GROUPS, W_LOAD = 6 * GROUPS, THREADS = 32 * (W_LOAD + 2);      // the first warps of the other roles
     static constexpr unsigned TMEM_COLS = 512, O_COL = GROUPS * 2 * KN;
     static constexpr int B_K_FULL = 0, B_V_FULL = STAGES, B_K_EMPTY = 2 * STAGES, B_V_EMPTY = 3 * STAGES, B_S = 4 * STAGES,
                          B_P = B_S + 2 * GROUPS, B_PV = B_P + 2 * GROUPS, B_Q = B_PV + 2 * GROUPS, B_V_LAND = B_Q + GROUPS, N_BARS = B_V_LAND + STAGES;
     static constexpr unsigned TAIL = N_BARS * 8 + 16 + TREE_MAX_NODES * 4;
-    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + 2 * GROUPS * P_BYTES + TAIL;
+    static constexpr unsigned SMEM_USED = NQ * Q_BYTES + 2 * STAGES * K_BYTES + TAIL;
     static constexpr unsigned SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024;       // one CTA an SM: it takes all of the tensor memory
     static_assert(SMEM <= 227 * 1024 && O_COL + GROUPS * D <= TMEM_COLS && STAGES > LAG, "a CTA's memories");
-    static_assert(2 * STAGES * K_BYTES + 2 * GROUPS * P_BYTES >= GROUPS * QM * D * 4, "room for the outputs behind Q");
+    static_assert(2 * STAGES * K_BYTES >= GROUPS * QM * D * 4, "room for the outputs behind Q");
     static_assert(!STREAMS || GROUPS == 1 || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
 };
 
@@ -539,6 +539,23 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+// D += A B^T with A in tensor memory: a lane a row, two neighbouring values of k a column.
+__device__ __forceinline__ void mma_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b_desc, unsigned idesc, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((unsigned)accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(unsigned taddr, const unsigned (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
     unsigned long long v;
@@ -607,8 +624,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     unsigned char* sQ = tc5_smem;                             // [query tile]
     unsigned char* sK = sQ + NQ * S::Q_BYTES;                 // [stage]
     unsigned char* sV = sK + STAGES * S::K_BYTES;             // [stage]
-    unsigned char* sP = sV + STAGES * S::K_BYTES;             // [group][buffer]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sP + 2 * GROUPS * S::P_BYTES);
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(sV + STAGES * S::K_BYTES);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + S::N_BARS);
     volatile int* odd_values = reinterpret_cast<int*>(tmem_slot + 1);
     int* parent = reinterpret_cast<int*>(tmem_slot + 4);
@@ -696,11 +712,6 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 
     if (has_rows) {
         // ================================================================== one row per thread, W keys of a tile
-        unsigned char* myPs = sP + grp * 2 * S::P_BYTES;
-        if (STREAMS && copies > 1) {                          // the other copies' keys: P stays zero there
-            for (int c = 0; c < 16; ++c)
-                *reinterpret_cast<uint4*>(myPs + (c >> 3) * S::P_BYTES + sw128_offset(r, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
-        }
         const int depth = tree_line(parent, node_head.x, window, line);
         lo_r = window > 0 ? max(0, sg.c + depth - window + 1) : 0;
         if (!STREAMS || grp == 0) {
@@ -784,26 +795,38 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     }
                     tmem_st_wait();
                 }
-                unsigned char* myP = myPs + buf * S::P_BYTES;
                 const unsigned long long scale2 = pack2(scale_eff, scale_eff), shift2 = pack2(-mu, -mu);
                 unsigned long long sum2[4] = {};
+                unsigned w[W / 2];
 #pragma unroll
                 for (int c = 0; c < W / 8; ++c) {
-                    unsigned w[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         float x0, x1;
                         unpack2(fma2(pack2(__uint_as_float(a[8 * c + 2 * k]), __uint_as_float(a[8 * c + 2 * k + 1])), scale2, shift2), x0, x1);
                         const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                         sum2[k] = add2(sum2[k], pack2(p0, p1));
-                        w[k] = pack_bf16(p0, p1);
+                        w[4 * c + k] = pack_bf16(p0, p1);
                     }
-                    *reinterpret_cast<uint4*>(myP + sw128_offset(r, (col >> 3) + c)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                // P(i) takes the first half of S(i)'s columns; the other copies' keys are zero there
+                const unsigned p_addr = lane_addr + (grp * 2 + buf) * KN;
+                if constexpr (W == 64) {
+                    tmem_st32(p_addr, w);
+                } else if constexpr (W == 32) {
+                    const unsigned none[16] = {};
+                    tmem_st16(p_addr + copy * 16, w);
+                    tmem_st16(p_addr + (copy ^ 1) * 16, none);
+                } else {
+                    const unsigned none[8] = {};
+                    tmem_st8(p_addr + copy * 8, w);
+#pragma unroll
+                    for (int c = 1; c < 4; ++c) tmem_st8(p_addr + (copy ^ c) * 8, none);
+                }
+                tmem_st_wait();
                 float sum_lo, sum_hi;
                 unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_lo, sum_hi);
                 l_run = l_run * alpha + (sum_lo + sum_hi);
-                fence_proxy_async();
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(S::B_P + grp * 2 + buf));       // S(i) is read, O is rescaled, P(i) is written
@@ -836,7 +859,6 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             }
         } else {                                              // P V
             const unsigned idesc = instr_desc_bf16(QM, D, true);
-            const unsigned long long dP = smem_desc_sw128(smem_u32(sP) + grp * 2 * S::P_BYTES, 0);
             const unsigned long long dV = smem_desc_sw128_mn(smem_u32(sV), KN * 128, 1024u);
             const unsigned d_o = tmem + S::O_COL + grp * D;
             for (int i = 0; i < n_mine; ++i) {
@@ -844,10 +866,11 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 ok = mbar_wait(bar(S::B_V_FULL + st), (t / STAGES) & 1) && ok;
                 ok = mbar_wait(bar(S::B_P + grp * 2 + (i & 1)), (i >> 1) & 1) && ok;
                 fence_after_sync();
-                const unsigned long long v_tile = dV + (unsigned long long)(st * (S::K_BYTES >> 4)), p_tile = dP + (unsigned long long)((i & 1) * (S::P_BYTES >> 4));
+                const unsigned long long v_tile = dV + (unsigned long long)(st * (S::K_BYTES >> 4));
+                const unsigned p_tile = tmem + (grp * 2 + (i & 1)) * KN;
 #pragma unroll
-                for (int k16 = 0; k16 < KN / 16; ++k16)       // 16 keys: 32 bytes along P's rows, 2048 bytes down V's
-                    mma_ss(d_o, p_tile + (unsigned long long)(k16 * 2), v_tile + (unsigned long long)(k16 * 128), idesc, i > 0 || k16 > 0);
+                for (int k16 = 0; k16 < KN / 16; ++k16)       // 16 keys: eight columns of P, 2048 bytes down V
+                    mma_ts(d_o, p_tile + k16 * 8, v_tile + (unsigned long long)(k16 * 128), idesc, i > 0 || k16 > 0);
                 mma_commit(bar(S::B_PV + grp * 2 + (i & 1)));
                 mma_commit(bar(S::B_V_EMPTY + st));
             }
@@ -969,7 +992,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             for (int t = max(0, n_tiles - S::LAG); t < n_tiles; ++t) announce(t);
         }
     }
-    // The rows leave through shared memory, where K, V and P lay: each (group, copy) its outputs in float32, brought to the row's common maximum,
+    // The rows leave through shared memory, where K and V lay: each (group, copy) its outputs in float32, brought to the row's common maximum,
     // a row of D by 16-byte pieces, piece p of row x at p ^ (x % 8).
     float2* stats = reinterpret_cast<float2*>(sQ);            // [group][tile row]: maximum and sum
     float* row_inv = reinterpret_cast<float*>(stats + GROUPS * QM);
