@@ -588,6 +588,15 @@ __device__ __forceinline__ void cp16u(unsigned smem_addr, const void* gmem, bool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_addr), "l"(gmem), "r"(bytes));
 }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+// Waits for the loads from tensor memory, and ties their registers to it.
+__device__ __forceinline__ void tmem_ld_wait32(unsigned (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :: "memory");
+}
 // tanh(x) = 1 - 2 / (e^(2x) + 1) with the hardware's 2^x and quotient: an absolute error of a few 1e-7.
 __device__ __forceinline__ float fast_tanh(float x) { return 1.0f - __fdividef(2.0f, fast_exp2(x * (2.0f * LOG2E)) + 1.0f); }
 // The halves of a word of two bfloat16 that are no finite numbers, as bits 15 and 31: an exponent of ones plus one carries into them.
@@ -720,6 +729,31 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
         }
+        // capped scores: a polynomial where all of the warp's are well below the cap
+        auto cap = [&](auto& a) {
+            constexpr int N = sizeof(a) / sizeof(a[0]);
+                                const float k = scale / softcap;
+                                float far = 0.f;
+            #pragma unroll
+                                for (int e = 0; e < N; e += 2) far = max3(far, fabsf(__uint_as_float(a[e])), fabsf(__uint_as_float(a[e + 1])));
+                                if (!__any_sync(0xffffffffu, !(far * k <= TANH_POLY_MAX))) {
+                                    const unsigned long long k2 = pack2(k, k);
+            #pragma unroll
+                                    for (int e = 0; e < N; e += 2) {
+                                        const unsigned long long x = mul2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), k2), u = mul2(x, x);
+                                        unsigned long long t = fma2(u, pack2(TANH_P4, TANH_P4), pack2(TANH_P3, TANH_P3));
+                                        t = fma2(u, t, pack2(TANH_P2, TANH_P2));
+                                        t = fma2(u, t, pack2(TANH_P1, TANH_P1));
+                                        float t0, t1;
+                                        unpack2(mul2(x, fma2(u, t, pack2(TANH_P0, TANH_P0))), t0, t1);
+                                        a[e] = __float_as_uint(t0);
+                                        a[e + 1] = __float_as_uint(t1);
+                                    }
+                                } else {
+            #pragma unroll
+                                    for (int e = 0; e < N; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+                                }
+        };
         auto walk = [&](auto width) {
             constexpr int W = decltype(width)::value;
             const int col = W == 64 ? 0 : copy * W;           // of a tile's keys
@@ -727,88 +761,115 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 const int j_base = (jt_begin + tile_no(grp, i)) * KN, buf = i & 1;
                 ok = mbar_wait(bar(S::B_S + grp * 2 + buf), (i >> 1) & 1) && ok;
                 fence_after_sync();
-                unsigned a[W];
                 const unsigned from = lane_addr + (grp * 2 + buf) * KN + col;
-                if constexpr (W == 16) {
-                    tmem_ld16(from, a);
-                } else {
+                const unsigned long long scale2 = pack2(scale_eff, scale_eff);
+                unsigned w[W / 2];
+                float tile_sum = 0.f;
+                bool done = false;
+                if (whole(j_base)) {
+                    // The reference rarely moves: the exponentials are made with the last one while the maximum is looked for, and thrown away if it has
+                    // been outrun.
+                    const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+                    const unsigned long long shift2 = pack2(-mu, -mu);
+                    constexpr int H = W < 32 ? W : 32;
+                    unsigned half[W / H][H];
+                    unsigned long long sum2[2] = {};
+                    float top[2] = {-INFINITY, -INFINITY};
+                    if constexpr (W == 16) {
+                        tmem_ld16(from, half[0]);
+                        tmem_ld_wait();
+                    } else {
+                        tmem_ld32(from, half[0]);
+                        tmem_ld_wait32(half[0]);
+                        if constexpr (W == 64) tmem_ld32(from + 32, half[1]);
+                    }
 #pragma unroll
-                    for (int c = 0; c < W; c += 32) tmem_ld32(from + c, reinterpret_cast<unsigned(&)[32]>(a[c]));
-                }
-                tmem_ld_wait();
-                if (CAP) {                                    // a polynomial where all of the warp's scores are well below the cap
-                    const float k = scale / softcap;
-                    float far = 0.f;
+                    for (int q = 0; q < W / H; ++q) {
+                        if constexpr (W == 64)
+                            if (q == 1) tmem_ld_wait32(half[1]);
+                        if (CAP) cap(half[q]);
 #pragma unroll
-                    for (int e = 0; e < W; e += 2) far = max3(far, fabsf(__uint_as_float(a[e])), fabsf(__uint_as_float(a[e + 1])));
-                    if (!__any_sync(0xffffffffu, !(far * k <= TANH_POLY_MAX))) {
-                        const unsigned long long k2 = pack2(k, k);
-#pragma unroll
-                        for (int e = 0; e < W; e += 2) {
-                            const unsigned long long x = mul2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), k2), u = mul2(x, x);
-                            unsigned long long t = fma2(u, pack2(TANH_P4, TANH_P4), pack2(TANH_P3, TANH_P3));
-                            t = fma2(u, t, pack2(TANH_P2, TANH_P2));
-                            t = fma2(u, t, pack2(TANH_P1, TANH_P1));
-                            float t0, t1;
-                            unpack2(mul2(x, fma2(u, t, pack2(TANH_P0, TANH_P0))), t0, t1);
-                            a[e] = __float_as_uint(t0);
-                            a[e + 1] = __float_as_uint(t1);
+                        for (int e = 0; e < H; e += 2) {
+                            const float s0 = __uint_as_float(half[q][e]), s1 = __uint_as_float(half[q][e + 1]);
+                            const unsigned long long x = fma2(pack2(s0, s1), scale2, shift2);
+                            float x0, x1;
+                            unpack2(x, x0, x1);
+                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                            top[(e >> 1) & 1] = max3(top[(e >> 1) & 1], s0, s1);
+                            sum2[(e >> 1) & 1] = add2(sum2[(e >> 1) & 1], pack2(p0, p1));
+                            w[q * (H / 2) + (e >> 1)] = pack_bf16(p0, p1);
                         }
+                    }
+                    done = !__any_sync(0xffffffffu, fmaxf(top[0], top[1]) * scale_eff > m_ref + RESCALE_STEP);
+                    float sum_lo, sum_hi;
+                    unpack2(add2(sum2[0], sum2[1]), sum_lo, sum_hi);
+                    tile_sum = sum_lo + sum_hi;
+                }
+                if (!done) {
+                    unsigned a[W];
+                    if constexpr (W == 16) {
+                        tmem_ld16(from, a);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < W; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+                        for (int c = 0; c < W; c += 32) tmem_ld32(from + c, reinterpret_cast<unsigned(&)[32]>(a[c]));
                     }
-                }
-                if (!whole(j_base)) {
-                    const unsigned long long vis = visible(j_base) >> col;
-                    const unsigned vis_lo = (unsigned)vis, vis_hi = (unsigned)(vis >> 32);
+                    tmem_ld_wait();
+                    if (CAP) cap(a);
+                    if (!whole(j_base)) {
+                        const unsigned long long vis = visible(j_base) >> col;
+                        const unsigned vis_lo = (unsigned)vis, vis_hi = (unsigned)(vis >> 32);
 #pragma unroll
-                    for (int e = 0; e < W; ++e)
-                        if (!((e < 32 ? vis_lo : vis_hi) & (1u << (e & 31)))) a[e] = 0xff800000u;
-                }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int e = 0; e < W; ++e)
+                            if (!((e < 32 ? vis_lo : vis_hi) & (1u << (e & 31)))) a[e] = 0xff800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < W; e += 8)
+                    for (int e = 0; e < W; e += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(a[e + 2 * k]), __uint_as_float(a[e + 2 * k + 1]));
-                const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale_eff;     // the scale is positive
-                float alpha = 1.f;
-                bool moved = false;
-                if (mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx != -INFINITY)) {
-                    alpha = fast_exp2(m_ref - mx);            // 0 on the first move
-                    m_ref = mx;
-                    moved = true;
-                }
-                const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-                // P(i) goes into the buffer that P V(i - 2) read: that was done when S(i) was issued.  O is touched only when P V(i - 1) is done.
-                if (i > 0 && __any_sync(0xffffffffu, moved)) {
-                    ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
-                    fence_after_sync();
+                        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], __uint_as_float(a[e + 2 * k]), __uint_as_float(a[e + 2 * k + 1]));
+                    const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale_eff;     // the scale is positive
+                    float alpha = 1.f;
+                    bool moved = false;
+                    if (mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx != -INFINITY)) {
+                        alpha = fast_exp2(m_ref - mx);            // 0 on the first move
+                        m_ref = mx;
+                        moved = true;
+                    }
+                    const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+                    // P(i) goes into the buffer that P V(i - 2) read: that was done when S(i) was issued.  O is touched only when P V(i - 1) is done.
+                    if (i > 0 && __any_sync(0xffffffffu, moved)) {
+                        ok = mbar_wait(bar(S::B_PV + grp * 2 + (buf ^ 1)), ((i - 1) >> 1) & 1) && ok;
+                        fence_after_sync();
 #pragma unroll 1
-                    for (int c0 = 0; c0 < D; c0 += 32) {
-                        unsigned o[32];
-                        tmem_ld32(o_addr + c0, o);
-                        tmem_ld_wait();
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            unsigned o[32];
+                            tmem_ld32(o_addr + c0, o);
+                            tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(o_addr + c0, o);
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st32(o_addr + c0, o);
+                        }
+                        tmem_st_wait();
                     }
-                    tmem_st_wait();
-                }
-                const unsigned long long scale2 = pack2(scale_eff, scale_eff), shift2 = pack2(-mu, -mu);
-                unsigned long long sum2[4] = {};
-                unsigned w[W / 2];
+                    const unsigned long long shift2 = pack2(-mu, -mu);
+                    unsigned long long sum2[4] = {};
 #pragma unroll
-                for (int c = 0; c < W / 8; ++c) {
+                    for (int c = 0; c < W / 8; ++c) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float x0, x1;
-                        unpack2(fma2(pack2(__uint_as_float(a[8 * c + 2 * k]), __uint_as_float(a[8 * c + 2 * k + 1])), scale2, shift2), x0, x1);
-                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                        sum2[k] = add2(sum2[k], pack2(p0, p1));
-                        w[4 * c + k] = pack_bf16(p0, p1);
+                        for (int k = 0; k < 4; ++k) {
+                            float x0, x1;
+                            unpack2(fma2(pack2(__uint_as_float(a[8 * c + 2 * k]), __uint_as_float(a[8 * c + 2 * k + 1])), scale2, shift2), x0, x1);
+                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                            sum2[k] = add2(sum2[k], pack2(p0, p1));
+                            w[4 * c + k] = pack_bf16(p0, p1);
+                        }
                     }
+                    float sum_lo, sum_hi;
+                    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_lo, sum_hi);
+                    tile_sum = sum_lo + sum_hi;
+                    l_run *= alpha;
                 }
+                l_run += tile_sum;
                 // P(i) takes the first half of S(i)'s columns; the other copies' keys are zero there
                 const unsigned p_addr = lane_addr + (grp * 2 + buf) * KN;
                 if constexpr (W == 64) {
@@ -824,9 +885,6 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     for (int c = 1; c < 4; ++c) tmem_st8(p_addr + (copy ^ c) * 8, none);
                 }
                 tmem_st_wait();
-                float sum_lo, sum_hi;
-                unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), sum_lo, sum_hi);
-                l_run = l_run * alpha + (sum_lo + sum_hi);
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(S::B_P + grp * 2 + buf));       // S(i) is read, O is rescaled, P(i) is written
