@@ -275,12 +275,6 @@ class CacheManager:
             out.append(fork)
         return out
 
-    def rename(self, rid, new) -> None:
-        """The request goes on under another name."""
-        if new in self._req:
-            raise KeyError(f"request {new!r} is already live")
-        self._req[new] = self._req.pop(rid)
-
     def truncate(self, rid, length: int) -> None:
         """Takes the last tokens of a request back: its length becomes ``length`` (not more than it is) and the
         pages behind it return to their pools.  What lies in the kept pages beyond ``length`` is overwritten by
