@@ -15,8 +15,9 @@
 //
 // Rows are (node, query head) pairs that share a key/value head, G = Hq / Hkv heads a node: row r is node r / G, head r % G.  The
 // keys of a segment are split over CTAs, one for every `share` key tiles (0: one CTA walks them all); each leaves its unnormalised
-// output, maximum and sum in float32, and tree_merge_kernel joins them in the order of the shares.  So the result depends
-// on `share`, which the host works out from the step's lengths, and on nothing else of the launch.
+// output, maximum and sum in float32, and they are joined in the order of the shares: up to JOIN_MAX shares can be a cluster and join them
+// through shared memory, others leave them in memory for tree_merge_kernel.  So the result depends on `share`, which the host works
+// out from the step's lengths, and on nothing else of the launch.
 #include "tc5.cuh"
 #include "tma.cuh"
 
@@ -29,6 +30,19 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KEY_TILE = 64;                  // the unit of `share`
+
+// Up to so many shares of a segment's keys can be a cluster, whose CTAs join their outputs through each other's shared memory.
+constexpr int JOIN_MAX = 8;
+__device__ __forceinline__ float4 peer_float4(unsigned at) {
+    float4 f;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(at));
+    return f;
+}
+__device__ __forceinline__ float2 peer_float2(unsigned at) {
+    float2 f;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(at));
+    return f;
+}
 
 // What a CTA knows about its segment.
 struct Segment {
@@ -159,7 +173,7 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
                 const int* __restrict__ block_table, int bt_stride, int page_size, int pages, TA* __restrict__ out,
                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, int D, float scale, int window,
-                float softcap, const float* __restrict__ sink, int share, int vec) {
+                float softcap, const float* __restrict__ sink, int share, int joined, int vec) {
     typedef MmaShape<TA, DP> S;
     constexpr bool F32 = S::F32;
     constexpr int PER16 = 16 / sizeof(TA);                             // elements of a 16-byte piece
@@ -175,13 +189,18 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
     __shared__ long long where[2][KEY_TILE];
     __shared__ int lows[MROWS];                                        // a row's first key
     __shared__ unsigned odd_keys[2];                                   // a tile's keys whose values the products cannot take
-    __shared__ float s_alpha[MROWS], s_m[MROWS], s_l[MROWS];
+    __shared__ float s_alpha[MROWS];
+    __shared__ float2 s_ml[MROWS];                                     // maximum (in units of log2) and sum
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int seg = blockIdx.y, kvh = blockIdx.x % Hkv, row0 = blockIdx.x / Hkv * MROWS, sp = blockIdx.z, G = Hq / Hkv;
     const Segment sg(cu_q, seg_pos0, seg, window, share, gridDim.z);
     const int rows = min(MROWS, sg.n * G - row0);
-    if (rows <= 0 || sp >= sg.n_split) return;
+    if (rows <= 0) return;                                             // all shares of a block of rows alike
+    if (sp >= sg.n_split) {
+        if (joined) { tc5::cluster_sync_all(); tc5::cluster_sync_all(); }
+        return;
+    }
     const int* bt = block_table + (size_t)seg * bt_stride;
     const int t0 = share > 0 ? sp * share : 0, t1 = share > 0 && sp + 1 < sg.n_split ? t0 + share : sg.tiles;      // this CTA's tiles
     auto q_row = [&](int r) { return q + (size_t)(sg.q_begin + (row0 + r) / G) * ld + (size_t)(kvh * G + (row0 + r) % G) * D; };
@@ -454,9 +473,55 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
         }
     }
     pdl_trigger_late();
-    if ((lane & 7) == 0) {
-        s_m[4 * warp + (lane >> 3)] = m;
-        s_l[4 * warp + (lane >> 3)] = l;
+    if ((lane & 7) == 0) s_ml[4 * warp + (lane >> 3)] = make_float2(m * LOG2E, l);
+    if (joined && sg.n_split > 1) {
+        // Every share's outputs, maxima and sums lie where its keys lay; each takes a part of the (row, four columns) pairs and goes through the
+        // shares in their order.
+        constexpr int OP = DP + 4;
+        static_assert(MROWS * OP * 4 <= S::K_BYTES, "room for the outputs");
+        float* os = reinterpret_cast<float*>(mma_smem);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+                *reinterpret_cast<float2*>(os + (rt + g + 8 * hh) * OP + part * (DP / 4) + 8 * n + 2 * t4) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
+        tc5::cluster_sync_all();
+        for (int i = sp * MTHREADS + tid; i < rows * (DP / 4); i += sg.n_split * MTHREADS) {
+            const int r = i / (DP / 4), d = 4 * (i % (DP / 4)), row = row0 + r, h = kvh * G + row % G;
+            if (d >= D) continue;
+            float2 ml[JOIN_MAX];
+            float4 f[JOIN_MAX];
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u) {
+                ml[u] = make_float2(-INFINITY, 0.f);
+                if (u < sg.n_split) {
+                    ml[u] = peer_float2(tc5::map_to_cta(smem_addr(s_ml + r), u));
+                    f[u] = peer_float4(tc5::map_to_cta(smem_addr(os + r * OP + d), u));
+                    top = fmaxf(top, ml[u].x);
+                }
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u)
+                if (ml[u].y != 0.f) {                                  // a share without keys for this row left nothing
+                    const float w = exp2f(ml[u].x - ref);
+                    total = fmaf(ml[u].y, w, total);
+                    sum.x = fmaf(f[u].x, w, sum.x); sum.y = fmaf(f[u].y, w, sum.y);
+                    sum.z = fmaf(f[u].z, w, sum.z); sum.w = fmaf(f[u].w, w, sum.w);
+                }
+            if (sink != nullptr) total += exp2f(sink[h] * LOG2E - ref);
+            const float inv = total == 0.f ? 0.f : 1.0f / total;
+            TA* to = out + ((size_t)(sg.q_begin + row / G) * Hq + h) * D + d;
+            const float v[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < D) to[e] = from_f32<TA>(v[e]);
+        }
+        __syncwarp();
+        tc5::cluster_sync_all();                                       // nobody leaves before its outputs have been read
+        return;
     }
     __syncthreads();
 #pragma unroll
@@ -465,14 +530,12 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
         if (r >= rows) continue;
         const int h = kvh * G + row % G;
         const size_t at = (size_t)(sg.q_begin + row / G) * Hq + h, slot = (size_t)sp * total_rows * Hq + at;
-        float total = s_l[r];
+        const float2 ml = s_ml[r];
+        float total = ml.y;
         if (sg.n_split > 1) {
-            if (part == 0 && t4 == 0) {
-                part_ml[2 * slot] = s_m[r] * LOG2E;                    // in units of log2, as the merge takes it
-                part_ml[2 * slot + 1] = total;
-            }
+            if (part == 0 && t4 == 0) *reinterpret_cast<float2*>(part_ml + 2 * slot) = ml;
         } else if (sink != nullptr) {
-            total += s_m[r] == -INFINITY ? 1.f : expf(sink[h] - s_m[r]);
+            total += ml.x == -INFINITY ? 1.f : exp2f(sink[h] * LOG2E - ml.x);
         }
         const float inv = total == 0.f ? 0.f : 1.0f / total;
 #pragma unroll
@@ -485,6 +548,8 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
                 else out[at * D + d] = from_f32<TA>(o[n][2 * hh + e] * inv);
             }
     }
+    __syncwarp();
+    if (joined) { tc5::cluster_sync_all(); tc5::cluster_sync_all(); }  // beside shares that have nothing
 }
 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
@@ -620,7 +685,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
                 const int* __restrict__ block_table, int bt_stride, int page_size, int pages, bf16* __restrict__ out,
                 float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, float scale, int window,
-                float softcap, const float* __restrict__ sink, int share, int* __restrict__ status, int by_tma,
+                float softcap, const float* __restrict__ sink, int share, int joined, int* __restrict__ status, int by_tma,
                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     typedef Shape<D, STREAMS> S;
     constexpr int STAGES = S::STAGES, NQ = S::NQ, GROUPS = S::GROUPS, W_ISSUE = S::W_ISSUE, W_LOAD = S::W_LOAD;
@@ -643,7 +708,11 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const int seg = blockIdx.y, kvh = blockIdx.x % Hkv, row0 = blockIdx.x / Hkv * (NQ * QM), split = blockIdx.z, G = Hq / Hkv;
     const Segment sg(cu_q, seg_pos0, seg, window, share, gridDim.z);
     const int rows = min(NQ * QM, sg.n * G - row0);
-    if (rows <= 0 || split >= sg.n_split) return;
+    if (rows <= 0) return;                                    // all shares of a block of rows alike
+    if (split >= sg.n_split) {
+        if (joined) { cluster_sync_all(); cluster_sync_all(); }
+        return;
+    }
     const int t0 = share > 0 ? split * share : 0, t1 = share > 0 && split + 1 < sg.n_split ? t0 + share : sg.tiles;
     const int jt_begin = sg.jt0 + t0, n_tiles = t1 - t0;      // one tile at least
     const int* bt_row = block_table + (size_t)seg * bt_stride;
@@ -1054,6 +1123,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     // a row of D by 16-byte pieces, piece p of row x at p ^ (x % 8).
     float2* stats = reinterpret_cast<float2*>(sQ);            // [group][tile row]: maximum and sum
     float* row_inv = reinterpret_cast<float*>(stats + GROUPS * QM);
+    float2* row_ml = reinterpret_cast<float2*>(row_inv + NQ * QM);      // what a cluster joins
     pdl_trigger_late();
     fence_before_sync();
     __syncthreads();                                          // no product reads shared memory any more
@@ -1081,7 +1151,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         }
         if (row_valid && (!STREAMS || (grp == 0 && copy == 0))) {
             const size_t at = token * Hq + h;
-            if (sg.n_split > 1) *reinterpret_cast<float2*>(part_ml + 2 * ((size_t)split * total_rows * Hq + at)) = make_float2(m_ref, l_run);
+            if (sg.n_split > 1) *(joined ? row_ml + in_cta : reinterpret_cast<float2*>(part_ml + 2 * ((size_t)split * total_rows * Hq + at))) = make_float2(m_ref, l_run);
             else if (sink != nullptr) l_run += exp2f(sink[h] * LOG2E - mu);
             row_inv[in_cta] = l_run == 0.f ? 0.f : 1.f / l_run;
         }
@@ -1133,21 +1203,63 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     // a row's partial outputs added, whole lines written: a thread four columns
     const bool parted = sg.n_split > 1;
     const int slots = STREAMS ? groups * copies : 1;
+    auto place = [&](int x, int piece) { return (unsigned)(x * (D * 4) + ((piece ^ (x & 7)) << 4)); };
 #pragma unroll 2
     for (int i = tid; i < rows * (D / 4); i += S::THREADS) {
         const int x = i / (D / 4), piece = i % (D / 4);
-        const int2 nh = by_group(row0 + x);
-        const size_t at = (size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; c < slots; ++c) {
-            const int at_row = STREAMS ? c * copy_rows + x : x;      // copies of a group lie side by side, groups QM apart
-            const float4 f = *reinterpret_cast<const float4*>(sK + (size_t)at_row * (D * 4) + ((piece ^ (at_row & 7)) << 4));
+        for (int c = 0; c < slots; ++c) {                     // copies of a group lie side by side, groups QM apart
+            const float4 f = *reinterpret_cast<const float4*>(sK + place(STREAMS ? c * copy_rows + x : x, piece));
             sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
         }
+        if (parted && joined) {
+            *reinterpret_cast<float4*>(sK + place(x, piece)) = sum;
+            continue;
+        }
+        const int2 nh = by_group(row0 + x);
+        const size_t at = (size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y;
         const float inv = row_inv[x];
         if (parted) *reinterpret_cast<float4*>(part_o + ((size_t)split * total_rows * Hq + at) * D + 4 * piece) = sum;
         else *reinterpret_cast<uint2*>(out + at * D + 4 * piece) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
     }
+    if (!joined) return;
+    __syncwarp();
+    cluster_sync_all();
+    if (parted) {                                             // each share takes a part of the pairs and goes through the shares in their order
+        for (int i = split * S::THREADS + tid; i < rows * (D / 4); i += sg.n_split * S::THREADS) {
+            const int x = i / (D / 4), piece = i % (D / 4);
+            const unsigned at_ml = smem_u32(row_ml + x), at_sum = smem_u32(sK + place(x, piece));
+            float2 ml[JOIN_MAX];
+            float4 f[JOIN_MAX];
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u) {
+                ml[u] = make_float2(-INFINITY, 0.f);
+                if (u < sg.n_split) {
+                    ml[u] = peer_float2(map_to_cta(at_ml, u));
+                    f[u] = peer_float4(map_to_cta(at_sum, u));
+                    top = fmaxf(top, ml[u].x);
+                }
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u)
+                if (ml[u].y != 0.f) {                         // a share without keys for this row left nothing
+                    const float w = exp2f(ml[u].x - ref);
+                    total = fmaf(ml[u].y, w, total);
+                    sum.x = fmaf(f[u].x, w, sum.x); sum.y = fmaf(f[u].y, w, sum.y);
+                    sum.z = fmaf(f[u].z, w, sum.z); sum.w = fmaf(f[u].w, w, sum.w);
+                }
+            const int2 nh = by_group(row0 + x);
+            if (sink != nullptr) total += exp2f(sink[kvh * G + nh.y] * LOG2E - ref);
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            *reinterpret_cast<uint2*>(out + ((size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y) * D + 4 * piece) =
+                make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();                                       // nobody leaves before its outputs have been read
 }
 
 // out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).  All
@@ -1234,15 +1346,36 @@ struct TreeCall {
     float softcap;
     const float* sink;
     int splits, share;
+    bool joined;
     float* scratch;
     int* status;
     cudaStream_t st;
-    float* part_ml() const { return splits > 1 ? scratch + (size_t)splits * total_rows * Hq * D : nullptr; }
+    float* part_ml() const { return scratch != nullptr ? scratch + (size_t)splits * total_rows * Hq * D : nullptr; }
 };
+
+// A launch whose shares of a block of rows are a cluster, if they join their outputs themselves.
+template <typename... KArgs, typename... Args>
+int launch(const TreeCall& a, void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, Args... args) {
+    if (!a.joined) return rb_launch_pdl(kernel, grid, dim3(threads), smem, a.st, args...);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = a.st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = (unsigned)a.splits;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = RB_PDL_MODE == 3 ? 1 : 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
 
 template <typename TA>
 int merge(const TreeCall& a) {
-    if (a.splits <= 1) return 0;
+    if (a.splits <= 1 || a.joined) return 0;
     dim3 grid((a.max_nodes * a.Hq + 7) / 8, a.segments);
     return rb_launch_pdl(a.D % 4 == 0 && a.D <= 128 ? tree_merge_kernel<TA, 4> : tree_merge_kernel<TA, 1>, grid, dim3(256), 0, a.st, a.scratch, a.part_ml(), a.cu_q, a.seg_pos0, a.total_rows, a.Hq, a.D,
                          a.window, a.share, a.splits, (TA*)a.out, a.sink);
@@ -1256,9 +1389,9 @@ int mma_launch(const TreeCall& a) {
     if (rc) return rc;
     const int vec = a.D * sizeof(TA) % 16 == 0 && (((uintptr_t)a.kpool | (uintptr_t)a.vpool) & 15) == 0;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + MROWS - 1) / MROWS * a.Hkv, a.segments, a.splits);
-    const int e = rb_launch_pdl(tree_mma_kernel<TA, DP>, grid, dim3(MTHREADS), SMEM, a.st, (const TA*)a.q, a.ld, (const TA*)a.kpool,
+    const int e = launch(a, tree_mma_kernel<TA, DP>, grid, MTHREADS, SMEM, (const TA*)a.q, a.ld, (const TA*)a.kpool,
                                 (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (TA*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, vec);
+                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, vec);
     return e ? e : merge<TA>(a);
 }
 template <typename TA>
@@ -1285,9 +1418,9 @@ int tc5_kernel_launch(const TreeCall& a) {
     if (by_tma && !(tma::make_map_bf16(&kmap, a.kpool, (int)pool_rows, D, D, box) && tma::make_map_bf16(&vmap, a.vpool, (int)pool_rows, D, D, box)))
         return (int)cudaErrorInvalidValue;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
-    const int e = rb_launch_pdl(tree_tc5_kernel<D, STREAMS, CAP>, grid, dim3(S::THREADS), S::SMEM, a.st, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
+    const int e = launch(a, tree_tc5_kernel<D, STREAMS, CAP>, grid, S::THREADS, S::SMEM, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
                                 (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (bf16*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, a.status, by_tma, kmap, vmap);
+                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
 }
 
@@ -1299,21 +1432,23 @@ int tc5_launch(const TreeCall& a) {
 }  // namespace
 
 RB_EXPORT int rb_tree_max_nodes() { return TREE_MAX_NODES; }
+RB_EXPORT int rb_tree_join_max() { return JOIN_MAX; }
 
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys
-// go to one CTA for every `share` key tiles of 64, `splits` at most; scratch then holds splits * total_rows * Hq * (D + 2) floats.
+// go to one CTA for every `share` key tiles of 64, `splits` at most, which are a cluster and join their outputs if `joined` (JOIN_MAX at most); else scratch holds
+// splits * total_rows * Hq * (D + 2) floats.
 // query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, or 256 with one; pools and
 // queries on 16-byte boundaries, ld a multiple of 8).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
                                 const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
                                 int segments, int max_nodes, int total_rows, int Hq, int Hkv, int D, float scale, int window,
-                                float softcap, const float* sink, int splits, int share, void* scratch, int query_tiles, int* status,
+                                float softcap, const float* sink, int splits, int share, int joined, void* scratch, int query_tiles, int* status,
                                 cudaStream_t st) {
     if (segments <= 0 || max_nodes <= 0) return 0;
     if (segments > 65535 || max_nodes > TREE_MAX_NODES || D <= 0 || D > TREE_MAX_D || Hkv <= 0 || Hq % Hkv || page_size <= 0) return (int)cudaErrorInvalidValue;
-    if (splits < 1 || splits > TREE_MAX_SPLITS || (splits > 1 && (share <= 0 || scratch == nullptr))) return (int)cudaErrorInvalidValue;
+    if (splits < 1 || splits > TREE_MAX_SPLITS || (splits > 1 && (share <= 0 || (joined ? splits > JOIN_MAX : scratch == nullptr)))) return (int)cudaErrorInvalidValue;
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
-                  D, pages, scale, window, softcap, sink, splits, share, (float*)scratch, status, st};
+                  D, pages, scale, window, softcap, sink, splits, share, joined && splits > 1, (float*)scratch, status, st};
     if (query_tiles > 0) {
         if (act_dtype != RB_BF16 || (D != 64 && D != 128 && D != 256) || query_tiles > (D == 256 ? 1 : 2) || status == nullptr) return (int)cudaErrorInvalidValue;
         if ((((uintptr_t)q | (uintptr_t)kpool | (uintptr_t)vpool | (uintptr_t)out) & 15) || ld % 8) return (int)cudaErrorInvalidValue;

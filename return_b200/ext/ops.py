@@ -2246,7 +2246,7 @@ TREE_MAX_NODES = 256               # drafted nodes of a segment
 TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
 TREE_TC5_HEAD_DIMS = (64, 128, 256)
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
-TREE_MAX_SPLITS = 64
+TREE_MAX_SPLITS, TREE_JOIN_MAX = 64, 8      # of a segment's keys; so many can join their outputs without a launch of their own
 TREE_SCRATCH_BYTES = 256 << 20
 
 
@@ -2256,7 +2256,7 @@ def tree_lib() -> ctypes.CDLL:
     if _tree is None:
         lib = build.load("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE})
         P, I, F = c_void_p, c_int, c_float
-        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, P, I, P, P]
+        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, I, P, I, P, P]
         lib.rb_tree_attention.restype = c_int
         _tree = build.native_calls(lib)
     return _tree
@@ -2323,14 +2323,23 @@ def _tree_lengths(batch, page_size: int, blocks: int):
 
 
 # What a launch costs, by kernel, in us: a CTA beside its key tiles (heads of 128; 60 % of it whatever the head size), a key tile as a + b times
-# the head size / 128, the merge of split keys as a + b times the splits, which part of a CTA's time the last ones stand alone where there
+# the head size / 128, the launch that merges split keys as a + b times the splits, which part of a CTA's time the last ones stand alone where there
 # are more than fit at once, and by how much a tile is slower where two CTAs share an SM.  Partial results are written and read, and keys
 # and values read, at TREE_HBM bytes a us.  Fitted to 620 launches (1 to 16 requests behind 60 to 8,000 tokens, trees of 4 to 32 nodes, heads of 64
 # to 256, each split in up to 12 ways): on average the choice is 1 % slower than the best of them, at worst 15.
 TREE_COSTS = {"tcgen05": (7.1, 0.38, 0.49, 2.6, 0.064, 0.33, 0.0), "bfloat16": (4.4, 0.70, 1.61, 2.9, 0.057, 0.27, 0.41),
               "float32": (3.1, 1.32, 4.26, 2.9, 0.113, 0.25, 0.47)}
+TREE_JOIN = {"tcgen05": (1.4, 0.1), "bfloat16": (2.3, 0.075), "float32": (2.2, 0.14)}        # shares that join as clusters: a + b times the splits
 TREE_HBM = 5.5e6
 TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20, 24, 32, 48, 64)
+
+
+def _tree_joins(splits: int, ctas: int, ctas_per_sm: int) -> bool:
+    """Whether the shares of a block of rows are a cluster that joins its outputs itself.  Clusters do not fill the device (24 rows of 6 CTAs, one to
+    an SM: 27 us for 24), and where two CTAs fit an SM they are put there, though others stand idle (24 of 6: 29.7 us, 23.8 by a merge
+    launch; 8 of 8, 11.4 and 12.4)."""
+    sms = num_sms()
+    return 1 < splits <= TREE_JOIN_MAX and ctas <= 0.87 * sms * ctas_per_sm and not (ctas_per_sm > 1 and sms / 2 < ctas <= sms)
 
 
 def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int, ctas_per_sm: int, kind: str):
@@ -2340,7 +2349,10 @@ def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int,
     blocks = [-(-k * rows_per_node // cta_rows) * kv_heads for k in nodes]
     sms, longest = num_sms(), max(tiles)
     fixed, tile, tile_dim, merge, merge_split, alone, shared = TREE_COSTS[kind]
+    join, join_split = TREE_JOIN[kind]
     fixed, tile = fixed * (0.6 + 0.4 * head_dim / 128), tile + tile_dim * head_dim / 128
+    if cta_rows > TREE_TILE_ROWS:
+        tile *= 1.25                                   # two row tiles a key tile: both groups of warps go through all of them
     slots = sms * ctas_per_sm if ctas_per_sm > 1 else 0.93 * sms             # a launch that takes every SM waits for the last one's CTAs
     total = sum([b * t for b, t in zip(blocks, tiles)])
     part_us = 2 * rows * (head_dim + 2) * 4 / TREE_HBM
@@ -2360,7 +2372,10 @@ def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int,
         if splits == 1 or splits > TREE_MAX_SPLITS or splits * rows * (head_dim + 2) * 4 > TREE_SCRATCH_BYTES:
             break
         ctas = sum([b * -(-t // share) for b, t in zip(blocks, tiles)])
-        us = done(ctas, share) + merge + splits * (merge_split + part_us)
+        if _tree_joins(splits, ctas, ctas_per_sm):
+            us = done(ctas, share) + join + splits * join_split
+        else:
+            us = done(ctas, share) + merge + splits * (merge_split + part_us)
         if us < best[0]:
             best = us, splits, share
         if ctas > 2 * slots:
@@ -2371,6 +2386,15 @@ def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int,
 def tree_shares(*step):
     """(splits, share) of ``tree_cost``."""
     return tree_cost(*step)[1:]
+
+
+def tree_joins(splits: int, share: int, nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int, head_dim: int, cta_rows: int,
+               ctas_per_sm: int, kind: str) -> bool:
+    """``_tree_joins`` of a step's launch."""
+    if splits == 1:
+        return False
+    tiles = [(e - 1) // TREE_KEY_TILE - (max(0, e - k - window + 1) if window else 0) // TREE_KEY_TILE + 1 for k, e in zip(nodes, ends)]
+    return _tree_joins(splits, sum([-(-k * rows_per_node // cta_rows) * kv_heads * -(-t // share) for k, t in zip(nodes, tiles)]), ctas_per_sm)
 
 
 def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window=None,
@@ -2398,14 +2422,15 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     kind = 0 if (q_at | k_at | v_at | out_at) & 15 or ld & 7 else 1          # kernels that move 16 bytes at a time, or any
     if shares[kind] is None:
         shares[kind] = _tree_launch(batch, page_size, block_table, num_heads, num_kv_heads, head_dim, window, dtype, kind)
-    tiles, splits, share = shares[kind]
+    tiles, splits, share, joined = shares[kind]
+    merged = splits > 1 and not joined
     # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
-    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if splits > 1 else None
+    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if merged else None
     _check(tree_lib().rb_tree_attention(q_at, ld, k_at, v_at, batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), batch.tree_parent.data_ptr(),
                                         block_table.data_ptr(), block_table.stride(0), page_size, k_pool.shape[0], out_at, code, n, longest, T,
-                                        num_heads, num_kv_heads, head_dim, scale, window, softcap, _sink_ptr(sink, num_heads), splits, share,
+                                        num_heads, num_kv_heads, head_dim, scale, window, softcap, _sink_ptr(sink, num_heads), splits, share, int(joined),
                                         None if scratch is None else scratch.data_ptr(), tiles, _status_word(qkv.device) if tiles else None,
-                                        _stream()), "tree_attention", 2 if splits > 1 else 1)
+                                        _stream()), "tree_attention", 2 if merged else 1)
 
 
 def _tree_plan(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_heads, num_kv_heads, head_dim, scale, window, sink, softcap):
@@ -2431,7 +2456,7 @@ def _tree_plan(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_head
 
 
 def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_heads: int, head_dim: int, window: int, dtype, kind: int):
-    """(query tiles of the tensor cores' kernel or 0, splits, share) of a step's launches."""
+    """(query tiles of the tensor cores' kernel or 0, splits, share, whether shares join as clusters) of a step's launch."""
     _, rows, longest, nodes, ends = _tree_lengths(batch, page_size, block_table.shape[1])
     group = num_heads // num_kv_heads
     step = (nodes, ends, window, group, num_kv_heads, rows * num_heads)
@@ -2439,14 +2464,16 @@ def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_head
     padded = next(d for d in (32, 64, 128, 256) if d >= head_dim)
     any_kind = step + (padded, 32, 1 if padded > 128 else 2, "float32" if dtype == torch.float32 else "bfloat16")
     if not (kind and dtype == torch.bfloat16 and head_dim in TREE_TC5_HEAD_DIMS):
-        return (0,) + tree_shares(*any_kind)
+        splits, share = tree_shares(*any_kind)
+        return 0, splits, share, tree_joins(splits, share, *any_kind)
     # The tensor cores' fifth generation, up to two tiles of TREE_TILE_ROWS rows a CTA, has more to set up: 16 query and 8 key heads of 128, a
-    # tree of 8 nodes behind 500 tokens 10.5 us against 9.5, four behind 2,000 18.4 against 21.2.
+    # tree of 8 nodes behind 500 tokens 9.6 us against 8.5, four behind 2,000 16.1 against 20.0.
     tiles = 1 if longest * group <= TREE_TILE_ROWS or head_dim == 256 else 2
     own_kind = step + (head_dim, tiles * TREE_TILE_ROWS, 1, "tcgen05")
     if tree_cost(*any_kind)[0] < tree_cost(*own_kind)[0]:
-        return (0,) + tree_shares(*any_kind)
-    return (tiles,) + tree_shares(*own_kind)
+        tiles, own_kind = 0, any_kind
+    splits, share = tree_shares(*own_kind)
+    return tiles, splits, share, tree_joins(splits, share, *own_kind)
 
 
 def _pool_shape(pool):

@@ -158,7 +158,7 @@ def kernel(request, monkeypatch):
 
     def watched(*a):
         got = launch(*a)
-        assert (got[0] > 0) == (request.param == "tcgen05")
+        assert (got[0] > 0) == (request.param == "tcgen05" and a[7] == torch.bfloat16 and a[5] in ops.TREE_TC5_HEAD_DIMS)
         return got
 
     monkeypatch.setattr(ops, "_tree_launch", watched)
@@ -177,6 +177,18 @@ def test_tree_attention_options_on_either_kernel(D, options, splits, share, kern
     monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
     a = Attention(5, torch.bfloat16, 8, 2, D, 16, [200, 0, 65, 1500], [20, 9, 1, 40], pad=16, **options)
     a.check(a.run())
+
+
+@pytest.mark.parametrize("joined", [True, False])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 256), (torch.float32, 128), (torch.float32, 6), (torch.bfloat16, 48)])
+@pytest.mark.parametrize("splits,share", [(2, 9), (3, 6), (8, 3), (8, 2)])
+def test_tree_attention_shares_joined_or_merged(splits, share, D, dtype, joined, kernel, monkeypatch):
+    """Shares that join as clusters, or by a launch of their own; segments of one share, and of none in some clusters' CTAs."""
+    monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
+    monkeypatch.setattr(ops, "tree_joins", lambda *a: joined)
+    for heads, nodes in ((8, [8, 2, 1]), (16, [70, 3, 33])):
+        a = Attention(23, dtype, heads, 2, D, 16, [1000, 3, 250], nodes, window=None if heads == 8 else 300, sink=heads == 8)
+        a.check(a.run())
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
