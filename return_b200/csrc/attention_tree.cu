@@ -111,6 +111,10 @@ __device__ __forceinline__ unsigned line_bits(const unsigned* line, int at) {
 // A product with a value that is no number reaches every row (zero times infinity), and float32's parts cannot hold one, nor one that 2^16 takes
 // beyond the numbers.  Where a float32 score is no finite number it is made again from the operands.  Where an output's sum over a tile is none,
 // such values are set to zero in shared memory, the tile's sums are made again, and the values are added for the rows that see them.
+// What bounds it: the chain keys - scores - softmax - values of a tile, 2.3 us (bfloat16, heads of 128) or 5.5 us (float32, where the splitting of
+// operands and six products are as long as the waits), hence two CTAs an SM and keys shared out down to one tile a CTA.  Measured: one tree of 8
+// nodes behind 500 tokens, 16 query and 8 key heads of 128, bfloat16 8.5 us in eight shares that join as clusters (9.5 with a merge launch, 22.2
+// unsplit); float32, three trees of 13 nodes behind a window of 1,000, 25 us in 16 shares, 95 unsplit.  FFMA from shared memory took 36.
 constexpr int MROWS = 32, MTHREADS = 256;
 constexpr int SP = KEY_TILE + 8;              // floats of a row of scores: eight-byte reads of four rows by four lanes hit all banks
 constexpr float UP = 65536.f, DOWN = 1.f / UP;
@@ -574,6 +578,13 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 // all of its waiters to have passed the current one, so no parity wait can fall two phases behind.
 // A key tile that some row does not see in full is looked through for values that are no numbers before the products take it: they are
 // set to zero there (zero times infinity would reach every row) and added to the rows that see them at the end.
+// What bounds it.  Few rows: HBM, and some 14 us around the walk (tables, tensor memory, first keys, outputs, join): 8 trees of 16 nodes behind 2,040
+// tokens, 32 query and 8 key heads of 128, 25.9 us of which the walk of 69 MB takes 11; 64 trees of 8 nodes 133 us, 4.1 TB/s.  Many rows: the row
+// warps, 1,390 cycles of the 1,830 a key tile of 256 rows takes (exponentials 1,024 of them, were nothing else in their way), while the tensor cores are
+// busy for 45 %: 32 trees of up to 64 nodes behind 2,000 to 8,000 tokens, 64 query and 8 key heads, 321 us, 0.80 PFLOP/s, at the power limit when they
+// follow each other.  Tried there: P through shared memory 345 us; the maximum before the exponentials 335; every fourth or second pair of
+// exponentials as a polynomial on the multiply-add units 335 and 348; key tiles cut into shares for the balance of the SMs costs the
+// traffic of partial results, 24 us at two shares, for 8 % of balance.
 using namespace tc5;
 
 constexpr int QM = 128;                       // rows of a query tile
@@ -1263,7 +1274,8 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 }
 
 // out[row, h] = sum_s O_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over the shares of the keys, in their order: one warp a (node, head).  All
-// maxima and sums are asked for at once (a lane a share), then the shares' rows eight at a time: about two trips to memory.
+// maxima and sums are asked for at once (a lane a share), then the shares' rows eight at a time: about two trips to memory.  Bound by the launch and
+// those trips: 2.9 us behind its producer for 16 shares of 128 rows, 0.06 us a share more.
 // grid: (nodes of the longest tree x Hq / 8, segments).  VEC: values of a row that lie together in a lane.
 template <typename TA, int VEC>
 __global__ void __launch_bounds__(256)

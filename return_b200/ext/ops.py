@@ -2326,7 +2326,7 @@ def _tree_lengths(batch, page_size: int, blocks: int):
 # the head size / 128, the launch that merges split keys as a + b times the splits, which part of a CTA's time the last ones stand alone where there
 # are more than fit at once, and by how much a tile is slower where two CTAs share an SM.  Partial results are written and read, and keys
 # and values read, at TREE_HBM bytes a us.  Fitted to 620 launches (1 to 16 requests behind 60 to 8,000 tokens, trees of 4 to 32 nodes, heads of 64
-# to 256, each split in up to 12 ways): on average the choice is 1 % slower than the best of them, at worst 15.
+# to 256, each split in up to 12 ways): on average the choice is 1 % slower than the best of them, at worst 15.  The joins were fitted to 520 more.
 TREE_COSTS = {"tcgen05": (7.1, 0.38, 0.49, 2.6, 0.064, 0.33, 0.0), "bfloat16": (4.4, 0.70, 1.61, 2.9, 0.057, 0.27, 0.41),
               "float32": (3.1, 1.32, 4.26, 2.9, 0.113, 0.25, 0.47)}
 TREE_JOIN = {"tcgen05": (1.4, 0.1), "bfloat16": (2.3, 0.075), "float32": (2.2, 0.14)}        # shares that join as clusters: a + b times the splits
