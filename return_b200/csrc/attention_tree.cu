@@ -557,7 +557,7 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 }
 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
-// bfloat16, head sizes 64, 128 and 256.  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
+// bfloat16, head sizes up to 256 that are multiples of 8, in shapes for 64, 128 and 256 (what lies behind the head size is zero).  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
 // tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
 //   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn.  With 64 rows or fewer the tile holds them twice, with
 //                  32 four times, and of a key tile each copy's warps take a half or a quarter (their P is zero elsewhere): a row's thread has
@@ -689,15 +689,17 @@ struct Paging {
     __device__ __forceinline__ int row(int j) const { return shift >= 0 ? j & (page_size - 1) : j % page_size; }
 };
 
-// grid: (row blocks x kv heads, segments, splits).  CAP: scores are capped (the plain kernel is spared the registers).
-template <int D, bool STREAMS, bool CAP>
+// grid: (row blocks x kv heads, segments, splits).  CAP: scores are capped.  WHOLE: the head size is D, else head_size, less than D.  (The plain
+// kernels are spared the registers: 32 trees behind 2,000 to 8,000 tokens 328 us, 340 with a head size of its own.)
+template <int D, bool STREAMS, bool CAP, bool WHOLE>
 __global__ void __launch_bounds__(Shape<D, STREAMS>::THREADS, 1)
 tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpool, const bf16* __restrict__ vpool,
                 const int* __restrict__ cu_q, const int* __restrict__ seg_pos0, const int* __restrict__ tree_parent,
                 const int* __restrict__ block_table, int bt_stride, int page_size, int pages, bf16* __restrict__ out,
-                float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, float scale, int window,
+                float* __restrict__ part_o, float* __restrict__ part_ml, int total_rows, int Hq, int Hkv, int head_size, float scale, int window,
                 float softcap, const float* __restrict__ sink, int share, int joined, int* __restrict__ status, int by_tma,
                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    const int head = WHOLE ? D : head_size;
     typedef Shape<D, STREAMS> S;
     constexpr int STAGES = S::STAGES, NQ = S::NQ, GROUPS = S::GROUPS, W_ISSUE = S::W_ISSUE, W_LOAD = S::W_LOAD;
     // The swizzled tiles need 1024-byte alignment: the kernel has no static shared memory, so its window starts at the CTA's base.
@@ -748,9 +750,9 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 #pragma unroll 4
         for (int i = 0; i < 32 / RPI; ++i) {                  // a row's pieces by neighbouring lanes
             const int rt = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + (STREAMS ? rt & (copy_rows - 1) : (warp >> 2) * QM + rt);
-            const bool there = rr - row0 < rows;
+            const bool there = rr - row0 < rows && sub * 8 < head;
             const int2 nh = by_group(rr);
-            const bf16* src = q + (there ? (size_t)(sg.q_begin + nh.x) * ld + (size_t)(kvh * G + nh.y) * D + sub * 8 : 0);
+            const bf16* src = q + (there ? (size_t)(sg.q_begin + nh.x) * ld + (size_t)(kvh * G + nh.y) * head + sub * 8 : 0);
             cp16u(smem_u32(tile + sw128_offset(rt, sub & 7)), src, there);
         }
     }
@@ -1107,7 +1109,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     where[u] = next_page[u] < 0 ? 0ull : reinterpret_cast<unsigned long long>(
-                        pool + (((size_t)next_page[u] * Hkv + kvh) * pg.page_size + pg.row((jt_begin + t) * KN + u * 32 + lane)) * D);
+                        pool + (((size_t)next_page[u] * Hkv + kvh) * pg.page_size + pg.row((jt_begin + t) * KN + u * 32 + lane)) * head);
                 const unsigned slab = (unsigned)(sub >> 3) * (KN * 128), c7 = (unsigned)(sub & 7);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -1115,8 +1117,9 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     for (int i = 0; i < 32 / RPI; ++i) {
                         const int owner = i * RPI + rsel, krow = u * 32 + owner;
                         const unsigned long long w = __shfl_sync(0xffffffffu, where[u], owner);
-                        const bf16* src = w ? reinterpret_cast<const bf16*>(w) + sub * 8 : pool;
-                        cp16u(tile_smem + (krow >> 3) * 1024 + (krow & 7) * 128 + slab + ((c7 ^ (unsigned)(krow & 7)) << 4), src, w != 0ull);
+                        const bool there = w != 0ull && sub * 8 < head;
+                        const bf16* src = there ? reinterpret_cast<const bf16*>(w) + sub * 8 : pool;
+                        cp16u(tile_smem + (krow >> 3) * 1024 + (krow & 7) * 128 + slab + ((c7 ^ (unsigned)(krow & 7)) << 4), src, there);
                     }
                 }
                 asm volatile("cp.async.commit_group;\n" ::);
@@ -1184,19 +1187,20 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
                     for (unsigned long long vis = visible(j_base); vis != 0ull; vis &= vis - 1ull) {
                         const int j = j_base + __ffsll((long long)vis) - 1, page = page_at(bt_row + pg.block(j), pages);
                         if (page < 0) continue;
-                        const size_t key = (((size_t)page * Hkv + kvh) * pg.page_size + pg.row(j)) * D;
+                        const size_t key = (((size_t)page * Hkv + kvh) * pg.page_size + pg.row(j)) * head;
                         unsigned any = 0u;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) any |= odd_halves(*reinterpret_cast<const unsigned*>(vpool + key + c0 + i));
+                        for (int i = 0; i < 32; i += 2)
+                            if (c0 + i < head) any |= odd_halves(*reinterpret_cast<const unsigned*>(vpool + key + c0 + i));
                         if (any == 0u) continue;
                         float s = 0.f;
-                        const bf16* qrow = q + token * ld + (size_t)h * D;
-                        for (int d = 0; d < D; ++d) s = fmaf(__bfloat162float(qrow[d]), __bfloat162float(kpool[key + d]), s);
+                        const bf16* qrow = q + token * ld + (size_t)h * head;
+                        for (int d = 0; d < head; ++d) s = fmaf(__bfloat162float(qrow[d]), __bfloat162float(kpool[key + d]), s);
                         s = CAP ? fast_tanh(s * (scale / softcap)) : s;
                         const float p = fast_exp2(fmaf(s, scale_eff, -mu));
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float v = __bfloat162float(vpool[key + c0 + i]);
+                            const float v = c0 + i < head ? __bfloat162float(vpool[key + c0 + i]) : 0.f;
                             if (!isfinite(v)) o[i] = __float_as_uint(fmaf(p, v, __uint_as_float(o[i])));
                         }
                     }
@@ -1218,6 +1222,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
 #pragma unroll 2
     for (int i = tid; i < rows * (D / 4); i += S::THREADS) {
         const int x = i / (D / 4), piece = i % (D / 4);
+        if (4 * piece >= head) continue;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int c = 0; c < slots; ++c) {                     // copies of a group lie side by side, groups QM apart
             const float4 f = *reinterpret_cast<const float4*>(sK + place(STREAMS ? c * copy_rows + x : x, piece));
@@ -1230,8 +1235,8 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         const int2 nh = by_group(row0 + x);
         const size_t at = (size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y;
         const float inv = row_inv[x];
-        if (parted) *reinterpret_cast<float4*>(part_o + ((size_t)split * total_rows * Hq + at) * D + 4 * piece) = sum;
-        else *reinterpret_cast<uint2*>(out + at * D + 4 * piece) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+        if (parted) *reinterpret_cast<float4*>(part_o + ((size_t)split * total_rows * Hq + at) * head + 4 * piece) = sum;
+        else *reinterpret_cast<uint2*>(out + at * head + 4 * piece) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
     }
     if (!joined) return;
     __syncwarp();
@@ -1239,6 +1244,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     if (parted) {                                             // each share takes a part of the pairs and goes through the shares in their order
         for (int i = split * S::THREADS + tid; i < rows * (D / 4); i += sg.n_split * S::THREADS) {
             const int x = i / (D / 4), piece = i % (D / 4);
+            if (4 * piece >= head) continue;
             const unsigned at_ml = smem_u32(row_ml + x), at_sum = smem_u32(sK + place(x, piece));
             float2 ml[JOIN_MAX];
             float4 f[JOIN_MAX];
@@ -1265,7 +1271,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             const int2 nh = by_group(row0 + x);
             if (sink != nullptr) total += exp2f(sink[kvh * G + nh.y] * LOG2E - ref);
             const float inv = total == 0.f ? 0.f : 1.f / total;
-            *reinterpret_cast<uint2*>(out + ((size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y) * D + 4 * piece) =
+            *reinterpret_cast<uint2*>(out + ((size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y) * head + 4 * piece) =
                 make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
         }
     }
@@ -1413,13 +1419,13 @@ int mma_any(const TreeCall& a) {
     return a.D <= 128 ? mma_launch<TA, 128>(a) : mma_launch<TA, 256>(a);
 }
 
-template <int D, bool STREAMS, bool CAP>
+template <int D, bool STREAMS, bool CAP, bool WHOLE>
 int tc5_kernel_launch(const TreeCall& a) {
     typedef Shape<D, STREAMS> S;
     constexpr int ROWS = S::NQ * QM;
     static PerDevice configured;
     const int rc = configured.once([&](int) {
-        return cudaFuncSetAttribute(tree_tc5_kernel<D, STREAMS, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        return cudaFuncSetAttribute(tree_tc5_kernel<D, STREAMS, CAP, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     });
     if (rc) return rc;
     // pages are whole boxes of whole groups of eight rows, and their rows can be counted in 31 bits
@@ -1427,18 +1433,19 @@ int tc5_kernel_launch(const TreeCall& a) {
     int by_tma = a.page_size % 8 == 0 && (KN % a.page_size == 0 || a.page_size % KN == 0) && pool_rows <= 0x7fffffffll;
     CUtensorMap kmap = {}, vmap = {};
     const int box = a.page_size < KN ? a.page_size : KN;
-    if (by_tma && !(tma::make_map_bf16(&kmap, a.kpool, (int)pool_rows, D, D, box) && tma::make_map_bf16(&vmap, a.vpool, (int)pool_rows, D, D, box)))
+    if (by_tma && !(tma::make_map_bf16(&kmap, a.kpool, (int)pool_rows, a.D, a.D, box) && tma::make_map_bf16(&vmap, a.vpool, (int)pool_rows, a.D, a.D, box)))
         return (int)cudaErrorInvalidValue;
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
-    const int e = launch(a, tree_tc5_kernel<D, STREAMS, CAP>, grid, S::THREADS, S::SMEM, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
+    const int e = launch(a, tree_tc5_kernel<D, STREAMS, CAP, WHOLE>, grid, S::THREADS, S::SMEM, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
                                 (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (bf16*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, a.status, by_tma, kmap, vmap);
+                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
 }
 
 template <int D, bool STREAMS>
 int tc5_launch(const TreeCall& a) {
-    return a.softcap > 0.f ? tc5_kernel_launch<D, STREAMS, true>(a) : tc5_kernel_launch<D, STREAMS, false>(a);
+    if (a.D == D) return a.softcap > 0.f ? tc5_kernel_launch<D, STREAMS, true, true>(a) : tc5_kernel_launch<D, STREAMS, false, true>(a);
+    return a.softcap > 0.f ? tc5_kernel_launch<D, STREAMS, true, false>(a) : tc5_kernel_launch<D, STREAMS, false, false>(a);
 }
 
 }  // namespace
@@ -1449,8 +1456,8 @@ RB_EXPORT int rb_tree_join_max() { return JOIN_MAX; }
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys
 // go to one CTA for every `share` key tiles of 64, `splits` at most, which are a cluster and join their outputs if `joined` (JOIN_MAX at most); else scratch holds
 // splits * total_rows * Hq * (D + 2) floats.
-// query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D 64 or 128, or 256 with one; pools and
-// queries on 16-byte boundaries, ld a multiple of 8).  *status is raised if a wait gave up.
+// query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D and ld multiples
+// of 8, one tile beyond 128; pools, queries and out on 16-byte boundaries).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
                                 const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
                                 int segments, int max_nodes, int total_rows, int Hq, int Hkv, int D, float scale, int window,
@@ -1462,10 +1469,10 @@ RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const 
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
                   D, pages, scale, window, softcap, sink, splits, share, joined && splits > 1, (float*)scratch, status, st};
     if (query_tiles > 0) {
-        if (act_dtype != RB_BF16 || (D != 64 && D != 128 && D != 256) || query_tiles > (D == 256 ? 1 : 2) || status == nullptr) return (int)cudaErrorInvalidValue;
+        if (act_dtype != RB_BF16 || D % 8 || query_tiles > (D > 128 ? 1 : 2) || status == nullptr) return (int)cudaErrorInvalidValue;
         if ((((uintptr_t)q | (uintptr_t)kpool | (uintptr_t)vpool | (uintptr_t)out) & 15) || ld % 8) return (int)cudaErrorInvalidValue;
-        if (D == 256) return tc5_launch<256, true>(a);
-        if (D == 64) return query_tiles == 1 ? tc5_launch<64, true>(a) : tc5_launch<64, false>(a);
+        if (D > 128) return tc5_launch<256, true>(a);
+        if (D <= 64) return query_tiles == 1 ? tc5_launch<64, true>(a) : tc5_launch<64, false>(a);
         return query_tiles == 1 ? tc5_launch<128, true>(a) : tc5_launch<128, false>(a);
     }
     return act_dtype == RB_F32 ? mma_any<float>(a) : mma_any<bf16>(a);

@@ -2244,7 +2244,7 @@ _tree = _branch = None
 
 TREE_MAX_NODES = 256               # drafted nodes of a segment
 TREE_TILE_ROWS = 128               # (node, query head) rows of a tile on the tensor cores
-TREE_TC5_HEAD_DIMS = (64, 128, 256)
+TREE_TC5_HEAD_DIMS = (64, 128, 256)      # shapes of the kernel on them; other head sizes are filled up with zeros
 TREE_KEY_TILE = 64                 # keys of a tile: the unit in which a tree's keys are shared out
 TREE_MAX_SPLITS, TREE_JOIN_MAX = 64, 8      # of a segment's keys; so many can join their outputs without a launch of their own
 TREE_SCRATCH_BYTES = 256 << 20
@@ -2463,13 +2463,14 @@ def _tree_launch(batch, page_size: int, block_table, num_heads: int, num_kv_head
     # Any type and head size (rounded up to a power of two): tiles of 32 rows.
     padded = next(d for d in (32, 64, 128, 256) if d >= head_dim)
     any_kind = step + (padded, 32, 1 if padded > 128 else 2, "float32" if dtype == torch.float32 else "bfloat16")
-    if not (kind and dtype == torch.bfloat16 and head_dim in TREE_TC5_HEAD_DIMS):
+    padded = next((d for d in TREE_TC5_HEAD_DIMS if d >= head_dim), 0)
+    if not (kind and padded and dtype == torch.bfloat16 and head_dim % 8 == 0):
         splits, share = tree_shares(*any_kind)
         return 0, splits, share, tree_joins(splits, share, *any_kind)
     # The tensor cores' fifth generation, up to two tiles of TREE_TILE_ROWS rows a CTA, has more to set up: 16 query and 8 key heads of 128, a
     # tree of 8 nodes behind 500 tokens 9.6 us against 8.5, four behind 2,000 16.1 against 20.0.
-    tiles = 1 if longest * group <= TREE_TILE_ROWS or head_dim == 256 else 2
-    own_kind = step + (head_dim, tiles * TREE_TILE_ROWS, 1, "tcgen05")
+    tiles = 1 if longest * group <= TREE_TILE_ROWS or padded == 256 else 2
+    own_kind = step + (padded, tiles * TREE_TILE_ROWS, 1, "tcgen05")
     if tree_cost(*any_kind)[0] < tree_cost(*own_kind)[0]:
         tiles, own_kind = 0, any_kind
     splits, share = tree_shares(*own_kind)
