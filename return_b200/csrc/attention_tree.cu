@@ -579,7 +579,7 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 // A key tile that some row does not see in full is looked through for values that are no numbers before the products take it: they are
 // set to zero there (zero times infinity would reach every row) and added to the rows that see them at the end.
 // What bounds it.  Few rows: HBM, and some 14 us around the walk (tables, tensor memory, first keys, outputs, join): 8 trees of 16 nodes behind 2,040
-// tokens, 32 query and 8 key heads of 128, 25.9 us of which the walk of 69 MB takes 11; 64 trees of 8 nodes 133 us, 4.1 TB/s.  Many rows: the row
+// tokens, 32 query and 8 key heads of 128, 25.7 us of which the walk of 69 MB takes 11; 64 trees of 8 nodes 133 us, 4.1 TB/s.  Many rows: the row
 // warps, 1,390 cycles of the 1,830 a key tile of 256 rows takes (exponentials 1,024 of them, were nothing else in their way), while the tensor cores are
 // busy for 45 %: 32 trees of up to 64 nodes behind 2,000 to 8,000 tokens, 64 query and 8 key heads, 321 us, 0.80 PFLOP/s, at the power limit when they
 // follow each other.  Tried there: P through shared memory 345 us; the maximum before the exponentials 335; every fourth or second pair of
@@ -745,11 +745,12 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     // Everything that waits for memory is asked for before the barrier: queries, parents, the loaders' first pages.
     constexpr int LPR = D / 8, RPI = 32 / LPR;                // lanes a row of 16-byte pieces, rows an instruction
     const int rsel = lane / LPR, sub = lane % LPR;
-    if (warp < W_ISSUE && (!STREAMS || warp < 4) && (warp & 3) < active_warps(warp >> 2)) {
+    if (warp < W_ISSUE && (warp & 3) < active_warps(warp >> 2)) {
+        constexpr int MINE = STREAMS ? 32 / GROUPS : 32;      // rows a warp asks for: STREAMS' groups share a tile
         unsigned char* tile = sQ + (STREAMS ? 0 : warp >> 2) * S::Q_BYTES + (unsigned)(sub >> 3) * (QM * 128);
 #pragma unroll 4
-        for (int i = 0; i < 32 / RPI; ++i) {                  // a row's pieces by neighbouring lanes
-            const int rt = (warp & 3) * 32 + i * RPI + rsel, rr = row0 + (STREAMS ? rt & (copy_rows - 1) : (warp >> 2) * QM + rt);
+        for (int i = 0; i < MINE / RPI; ++i) {                // a row's pieces by neighbouring lanes
+            const int rt = (warp & 3) * 32 + (STREAMS ? (warp >> 2) * MINE : 0) + i * RPI + rsel, rr = row0 + (STREAMS ? rt & (copy_rows - 1) : (warp >> 2) * QM + rt);
             const bool there = rr - row0 < rows && sub * 8 < head;
             const int2 nh = by_group(rr);
             const bf16* src = q + (there ? (size_t)(sg.q_begin + nh.x) * ld + (size_t)(kvh * G + nh.y) * head + sub * 8 : 0);
@@ -768,7 +769,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         int count = 1;
         if (i >= S::B_K_EMPTY && i < S::B_S) count = !STREAMS && rows > QM ? 2 : 1;           // the groups that read a key tile
         else if (i >= S::B_P && i < S::B_PV) count = max(1, active_warps((i - S::B_P) >> 1));
-        else if (i >= S::B_Q && i < S::B_V_LAND) count = max(1, active_warps(i - S::B_Q));
+        else if (i >= S::B_Q && i < S::B_V_LAND) count = STREAMS ? GROUPS * active_warps(0) : max(1, active_warps(i - S::B_Q));
         mbar_init(bar(i), count);
         mbar_init_fence();
     }
@@ -805,12 +806,10 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         // ================================================================== one row per thread, W keys of a tile
         const int depth = tree_line(parent, node_head.x, window, line);
         lo_r = window > 0 ? max(0, sg.c + depth - window + 1) : 0;
-        if (!STREAMS || grp == 0) {
-            cp_wait<0>();
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
-        }
+        cp_wait<0>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(S::B_Q + qt));
         // capped scores: a polynomial where all of the warp's are well below the cap
         auto cap = [&](auto& a) {
             constexpr int N = sizeof(a) / sizeof(a[0]);
@@ -1242,37 +1241,54 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     __syncwarp();
     cluster_sync_all();
     if (parted) {                                             // each share takes a part of the pairs and goes through the shares in their order
-        for (int i = split * S::THREADS + tid; i < rows * (D / 4); i += sg.n_split * S::THREADS) {
-            const int x = i / (D / 4), piece = i % (D / 4);
-            if (4 * piece >= head) continue;
-            const unsigned at_ml = smem_u32(row_ml + x), at_sum = smem_u32(sK + place(x, piece));
+        float* weight = reinterpret_cast<float*>(row_ml + NQ * QM);       // [share][row]
+        static_assert(GROUPS * QM * 8 + NQ * QM * (4 + 8 + 4 * JOIN_MAX) <= NQ * S::Q_BYTES, "room for the weights in the place of Q");
+        if (tid < rows) {
             float2 ml[JOIN_MAX];
-            float4 f[JOIN_MAX];
-            float top = -INFINITY, total = 0.f;
+            float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < JOIN_MAX; ++u) {
                 ml[u] = make_float2(-INFINITY, 0.f);
-                if (u < sg.n_split) {
-                    ml[u] = peer_float2(map_to_cta(at_ml, u));
-                    f[u] = peer_float4(map_to_cta(at_sum, u));
-                    top = fmaxf(top, ml[u].x);
-                }
+                if (u < sg.n_split) ml[u] = peer_float2(map_to_cta(smem_u32(row_ml + tid), u));
             }
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u) top = fmaxf(top, ml[u].x);
             const float ref = top == -INFINITY ? 0.f : top;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            float total = sink != nullptr ? exp2f(sink[kvh * G + by_group(row0 + tid).y] * LOG2E - ref) : 0.f;
+#pragma unroll
+            for (int u = 0; u < JOIN_MAX; ++u) {
+                ml[u].x = ml[u].y == 0.f ? 0.f : exp2f(ml[u].x - ref);     // a share without keys for this row left nothing
+                total = fmaf(ml[u].y, ml[u].x, total);
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
             for (int u = 0; u < JOIN_MAX; ++u)
-                if (ml[u].y != 0.f) {                         // a share without keys for this row left nothing
-                    const float w = exp2f(ml[u].x - ref);
-                    total = fmaf(ml[u].y, w, total);
-                    sum.x = fmaf(f[u].x, w, sum.x); sum.y = fmaf(f[u].y, w, sum.y);
-                    sum.z = fmaf(f[u].z, w, sum.z); sum.w = fmaf(f[u].w, w, sum.w);
+                if (u < sg.n_split) weight[u * (NQ * QM) + tid] = ml[u].x * inv;
+        }
+        __syncthreads();
+        for (int i = split * S::THREADS + tid; i < rows * (D / 4); i += sg.n_split * S::THREADS) {
+            const int x = i / (D / 4), piece = i % (D / 4);
+            if (4 * piece >= head) continue;
+            const unsigned at_sum = smem_u32(sK + place(x, piece));
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int u0 = 0; u0 < sg.n_split; u0 += 4) {
+                float4 f[4];
+                float w[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    w[u] = u0 + u < sg.n_split ? weight[(u0 + u) * (NQ * QM) + x] : 0.f;
+                    if (u0 + u < sg.n_split) f[u] = peer_float4(map_to_cta(at_sum, u0 + u));
                 }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (w[u] != 0.f) {
+                        sum.x = fmaf(f[u].x, w[u], sum.x); sum.y = fmaf(f[u].y, w[u], sum.y);
+                        sum.z = fmaf(f[u].z, w[u], sum.z); sum.w = fmaf(f[u].w, w[u], sum.w);
+                    }
+            }
             const int2 nh = by_group(row0 + x);
-            if (sink != nullptr) total += exp2f(sink[kvh * G + nh.y] * LOG2E - ref);
-            const float inv = total == 0.f ? 0.f : 1.f / total;
             *reinterpret_cast<uint2*>(out + ((size_t)(sg.q_begin + nh.x) * Hq + kvh * G + nh.y) * head + 4 * piece) =
-                make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+                make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
         }
     }
     __syncwarp();
