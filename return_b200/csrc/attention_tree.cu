@@ -557,8 +557,8 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 }
 
 // ---------------------------------------------------------------------------------------- fifth-generation tensor cores
-// bfloat16, head sizes up to 256 that are multiples of 8, in shapes for 64, 128 and 256 (what lies behind the head size is zero).  A CTA (one an SM) owns rows of one segment and key/value head and walks its share of the keys in
-// tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
+// bfloat16, head sizes up to 256 that are multiples of 8, in shapes for 64, 128 and 256 (what lies behind the head size is zero).  A CTA (one an SM)
+// owns rows of one segment and key/value head and walks its share of the keys in tiles of 64.  Two groups of four warps work side by side, so that one's waits pass while the other computes:
 //   STREAMS        up to 128 rows: one query tile, the groups take the key tiles in turn.  With 64 rows or fewer the tile holds them twice, with
 //                  32 four times, and of a key tile each copy's warps take a half or a quarter (their P is zero elsewhere): a row's thread has
 //                  to sit on the warp of its tensor-memory lane, and this way all four have exponentials to make.  Every copy of either group

@@ -2335,9 +2335,9 @@ TREE_PARTS = (2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 20, 24, 32, 48, 64)
 
 
 def _tree_joins(splits: int, ctas: int, ctas_per_sm: int) -> bool:
-    """Whether the shares of a block of rows are a cluster that joins its outputs itself.  Clusters do not fill the device (24 rows of 6 CTAs, one to
-    an SM: 27 us for 24), and where two CTAs fit an SM they are put there, though others stand idle (24 of 6: 29.7 us, 23.8 by a merge
-    launch; 8 of 8, 11.4 and 12.4)."""
+    """Whether the shares of a block of rows are a cluster that joins its outputs itself.  Clusters do not fill the device (32 blocks of 5 shares,
+    one CTA an SM: 27.9 us, 24.0 by a merge launch), and where two CTAs fit an SM they are put there, though others stand idle (24 blocks
+    of 6: 29.7 us and 23.8; 8 of 8, where it does not matter: 11.4 and 12.4)."""
     sms = num_sms()
     return 1 < splits <= TREE_JOIN_MAX and ctas <= 0.87 * sms * ctas_per_sm and not (ctas_per_sm > 1 and sms / 2 < ctas <= sms)
 
