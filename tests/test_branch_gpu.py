@@ -311,6 +311,36 @@ def test_tree_attention_takes_what_the_documentation_allows():
     ops.check_status(torch.device(DEV))
 
 
+@pytest.mark.parametrize("splits,share", [(2, 8), (5, 3), (8, 2)])
+def test_joined_shares_on_two_streams_and_in_graphs(splits, share, kernel, monkeypatch):
+    """Clusters of two calls, and of two captured graphs, side by side on the device."""
+    monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
+    monkeypatch.setattr(ops, "tree_joins", lambda *a: True)
+    a = Attention(31, torch.bfloat16, 16, 4, 128, 16, [1000, 30, 700, 500, 900, 1000], [8, 5, 1, 8, 8, 8])
+    want = a.run()
+    a.check(want)
+    heads, kv_heads, D, scale = a.args
+    qkv, k, v = (x.to(DEV) for x in (a.qkv, a.k, a.v))
+    call = lambda out: ops.tree_attention(qkv, k, v, a.batch, a.block_table, 16, out, heads, kv_heads, D, scale)  # noqa: E731
+    outs = [torch.empty_like(want) for _ in range(4)]
+    streams, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    for o in outs[2:]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(o)
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for s, o, graph in zip(streams, outs, graphs):
+            with torch.cuda.stream(s):
+                call(o)
+                graph.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert torch.equal(o, want)
+    ops.check_status(torch.device(DEV))
+
+
 # ---------------------------------------------------------------------------------------- commit
 
 def commit_case(seed, layers, heads, D, page, cached, nodes, dtype, latent=False, twice=False):
