@@ -2417,7 +2417,10 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     if not (qkv.stride(1) == 1 and k_pool.is_contiguous() and v_pool.is_contiguous() and out.is_contiguous()
             and block_table.dtype == torch.int32 and block_table.stride(1) == 1):
         raise KernelError("qkv and block_table (int32): unit stride along a row; pools and out: contiguous")
-    _same_device(qkv, k_pool, v_pool, block_table, out, batch.cu_q, batch.seg_pos0, batch.tree_parent, sink)
+    cu_q, seg_pos0, parent, at = batch.cu_q, batch.seg_pos0, batch.tree_parent, qkv.get_device()          # asked here: a call for it costs the host 0.6 us
+    if at < 0 or not (k_pool.get_device() == v_pool.get_device() == block_table.get_device() == out.get_device() == cu_q.get_device() == seg_pos0.get_device()
+            == parent.get_device() == at == _device_index() and (sink is None or sink.get_device() == at)):
+        _same_device(qkv, k_pool, v_pool, block_table, out, cu_q, seg_pos0, parent, sink)
     q_at, k_at, v_at, out_at, ld = qkv.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), qkv.stride(0)
     kind = 0 if (q_at | k_at | v_at | out_at) & 15 or ld & 7 else 1          # kernels that move 16 bytes at a time, or any
     if shares[kind] is None:
@@ -2426,7 +2429,7 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
     merged = splits > 1 and not joined
     # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
     scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if merged else None
-    _check(tree_lib().rb_tree_attention(q_at, ld, k_at, v_at, batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), batch.tree_parent.data_ptr(),
+    _check(tree_lib().rb_tree_attention(q_at, ld, k_at, v_at, cu_q.data_ptr(), seg_pos0.data_ptr(), parent.data_ptr(),
                                         block_table.data_ptr(), block_table.stride(0), page_size, k_pool.shape[0], out_at, code, n, longest, T,
                                         num_heads, num_kv_heads, head_dim, scale, window, softcap, _sink_ptr(sink, num_heads), splits, share, int(joined),
                                         None if scratch is None else scratch.data_ptr(), tiles, _status_word(qkv.device) if tiles else None,
@@ -2495,11 +2498,13 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
     ``caches``: (pool, block_table) of every group of layers; the row of slot ``seg_pos0 + path[i]`` goes to slot ``seg_pos0 + i``.  The
     request then holds ``seg_pos0 + count`` tokens.  Other rows stay as they are; a move from or to a page that the table marks as
     gone is left out."""
-    key = ("tree.commit", sampled.shape, path.shape, count.shape, emitted.shape, *[x for pool, table in caches for x in (pool.shape, pool.dtype, table.shape)])
-    plan = batch.scratch.get(key)                      # what follows from the shapes is looked at once a step
-    if plan is None:
-        plan = batch.scratch[key] = _commit_plan(sampled, batch, caches, path, count, emitted)
-    n, width, shapes = plan
+    looked = [sampled.shape, path.shape, count.shape, emitted.shape]
+    for pool, table in caches:
+        looked += (pool.shape, pool.dtype, table.shape)
+    plan = batch.scratch.get("tree.commit")            # what follows from the shapes is looked at once a step
+    if plan is None or plan[0] != looked:
+        plan = batch.scratch["tree.commit"] = (looked,) + _commit_plan(sampled, batch, caches, path, count, emitted)
+    _, n, width, shapes = plan
     ints = torch.int32
     tokens = batch.tokens
     if not (sampled.dtype == ints and path.dtype == ints and count.dtype == ints and emitted.dtype == ints and tokens.dtype == ints
@@ -2508,14 +2513,19 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
     for pool, table in caches:
         if not (pool.is_contiguous() and table.dtype == ints and table.stride(1) == 1):
             raise KernelError("a pool: contiguous; its block_table: int32, unit stride along a row")
-    _same_device(sampled, tokens, batch.tree_parent, batch.cu_q, batch.seg_pos0, path, count, emitted)
+    parent, cu_q, seg_pos0, at = batch.tree_parent, batch.cu_q, batch.seg_pos0, sampled.get_device()
+    if at < 0 or not (tokens.get_device() == parent.get_device() == cu_q.get_device() == seg_pos0.get_device() == path.get_device() == count.get_device()
+            == emitted.get_device() == at == _device_index()):
+        _same_device(sampled, tokens, parent, cu_q, seg_pos0, path, count, emitted)
+    for pool, table in caches:
+        if not (pool.get_device() == table.get_device() == at):
+            _same_device(pool, table)
     entry, st = branch_lib().rb_tree_commit, _stream()
-    args = (tokens.data_ptr(), batch.tree_parent.data_ptr(), sampled.data_ptr(), batch.cu_q.data_ptr(), batch.seg_pos0.data_ptr(), n)
+    args = (tokens.data_ptr(), parent.data_ptr(), sampled.data_ptr(), cu_q.data_ptr(), seg_pos0.data_ptr(), n)
     outs = (path.data_ptr(), count.data_ptr(), emitted.data_ptr(), width)
     if not shapes:
         _check(entry(*args, None, 0, 1, None, 0, 0, 0, 0, *outs, st), "tree_commit")
     for (pool, table), (planes, pages, heads, page_size, row_bytes) in zip(caches, shapes):
-        _same_device(pool, table)
         _check(entry(*args, table.data_ptr(), table.stride(0), page_size, pool.data_ptr(), planes, pages, heads, row_bytes, *outs, st), "tree_commit")
         outs = (None, None, None, 0)
 
@@ -2635,10 +2645,12 @@ def beam_select(logits, scores, beams: int, scores_out, beams_out, tokens_out) -
     if not (scores.dtype == f32 and scores_out.dtype == f32 and beams_out.dtype == ints and tokens_out.dtype == ints and scores.is_contiguous()
             and scores_out.is_contiguous() and beams_out.is_contiguous() and tokens_out.is_contiguous()):
         raise KernelError("scores and scores_out: contiguous float32; beams_out and tokens_out: contiguous int32")
-    _same_device(logits, scores, scores_out, beams_out, tokens_out)
+    at = logits.get_device()
+    if at < 0 or not (scores.get_device() == scores_out.get_device() == beams_out.get_device() == tokens_out.get_device() == at == _device_index()):
+        _same_device(logits, scores, scores_out, beams_out, tokens_out)
     if requests == 0:
         return
     rows, V = logits.shape
-    scratch = torch.empty(_beam_scratch(rows, V, keep, logits.get_device()), dtype=f32, device=logits.device)
+    scratch = torch.empty(_beam_scratch(rows, V, keep, at), dtype=f32, device=logits.device)
     _check(branch_lib().rb_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), requests, beams, V, keep, scores_out.data_ptr(),
                               beams_out.data_ptr(), tokens_out.data_ptr(), scratch.data_ptr(), _stream()), "beam_select", 2)
