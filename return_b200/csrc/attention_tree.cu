@@ -114,7 +114,7 @@ __device__ __forceinline__ unsigned line_bits(const unsigned* line, int at) {
 // What bounds it: the chain keys - scores - softmax - values of a tile, 2.3 us (bfloat16, heads of 128) or 5.5 us (float32, where the splitting of
 // operands and six products are as long as the waits), hence two CTAs an SM and keys shared out down to one tile a CTA.  Measured: one tree of 8
 // nodes behind 500 tokens, 16 query and 8 key heads of 128, bfloat16 8.5 us in eight shares that join as clusters (9.5 with a merge launch, 22.2
-// unsplit); float32, three trees of 13 nodes behind a window of 1,000, 25 us in 16 shares, 95 unsplit.  FFMA from shared memory took 36.
+// unsplit); float32, three trees of 13 nodes behind a window of 1,000, 25 us in 16 shares, 95 unsplit.  On the CUDA cores those took 71.
 constexpr int MROWS = 32, MTHREADS = 256;
 constexpr int SP = KEY_TILE + 8;              // floats of a row of scores: eight-byte reads of four rows by four lanes hit all banks
 constexpr float UP = 65536.f, DOWN = 1.f / UP;

@@ -16,8 +16,8 @@
 //
 // What bounds it: 128 rows of 151,936, the 16 best of eight beams, 27.8 us, of which the parts take 24 (3.2 TB/s; a stream alone would take 12): a CTA's first
 // tile waits 2.3 us for memory and 4.6 for its selection, later tiles for the logits, the last ranking and sums 2 us, and 256 CTAs fill 108 of 148 SMs
-// twice and the others once.  Four rows of 32,768: 7.7 us, a selection and a merge.  In parts, since a row a CTA leaves too few; by streaming, since
-// a selection in every tile took 36 us.
+// twice and the others once.  Four rows of 32,768: 7.7 us, a selection and a merge.  The first form, without the ring and
+// the rising bound, took 40 and 10.9 us.
 #include "common.cuh"
 
 #define BEAM_MAX_KEEP 128

@@ -60,8 +60,8 @@ struct ByDivisor {
 // grid: (segments, parts of the planes x heads).  Node path[i] moves from slot c + path[i] to slot c + i.  LPR lanes share a row's pieces; a
 // thread keeps to its piece of a (plane, head) and goes through the moves in order, eight loads before their stores.  No store meets a row
 // that is still to be read: path[k] >= k, so a later move's source lies behind every earlier move's destination.
-// Bound by two trips to memory (tables, rows) where little moves: 8 nodes, 28 layers, 3.1 us.  64 requests of which five tokens hold, 36 layers of 8 key heads
-// of 128: 18.4 us in a row of them (14.5 alone), 4.1 TB/s of rows of 256 bytes that lie anywhere; moves one after the other took 31.
+// Bound by two trips to memory (tables, rows) where little moves: 8 nodes, 28 layers, 3.1 us.  64 requests of which six tokens hold, 36 layers of 8 key heads
+// of 128: 18.4 us in a row of them (14.5 alone), 4.1 TB/s of rows of 256 bytes that lie anywhere; the first, simple form took 34.
 // The walk is done by every CTA for itself (a few hundred cycles); the first part writes it down.  What it takes is asked for at once, the
 // part of the block table that the tree lies on with it.
 template <int W>
