@@ -191,7 +191,7 @@ def prepare(case, seed):
             tokens += draft.tolist()
             sampled += target.tolist()
         s["batch"] = _batch(cached, nodes, parents, tokens)
-        s["sampled"], s["width"] = _ints(sampled), max(nodes)
+        s["sampled"] = _ints(sampled)
     if op == "tree_attention":
         D, Hq, Hkv, dt = case["head_dim"], case["heads"], case["kv_heads"], _dtype(case)
         # rows of projections: queries, then the step's keys and values, which are in the cache already
@@ -243,7 +243,7 @@ def _run_own(s):
                            window=case["window"] or None, sink=s["sink"], softcap=case["softcap"] or None)
         return out
     if op == "tree_commit":
-        n, width = case["requests"], s["width"]
+        n, width = case["requests"], max(_lengths(case)[1])
         path, emitted = (torch.empty((n, width), dtype=torch.int32, device=DEVICE) for _ in range(2))
         count = torch.empty((n,), dtype=torch.int32, device=DEVICE)
         ops.tree_commit(s["sampled"], s["batch"], [(s["pool"], s["block_table"])], path, count, emitted)
