@@ -197,6 +197,7 @@ beam_part_kernel(const float* __restrict__ logits, long long ld, int V, int part
         }
         __syncthreads();
         const int now = s_n;
+        __syncthreads();                                      // everyone has the count before shorten() writes the next one
         if (now > COLLECT) {                                  // no room: this tile's best one by one, behind what was held before
             Key last = ~0ull;
             for (int k = 0; k < keep; ++k) {

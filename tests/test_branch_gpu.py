@@ -520,3 +520,17 @@ def test_beam_select_strides_streams_and_graphs():
     torch.cuda.synchronize()
     for o in outs:
         assert all(torch.equal(a.cpu(), b) for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("rows,V,keep", [(296, 4096, 64), (592, 1000, 5), (40, 40000, 128)])
+def test_beam_select_gives_the_same_every_time(rows, V, keep):
+    """A first tile's selection counts what all threads collected: late warps and early ones see one count, run after run."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((rows, V), generator=g)
+    x[::2] = torch.round(x[::2] * 2)                                            # some rows of many equal values
+    s = -torch.rand(rows, generator=g)
+    beams_check(x, s, 4, keep)
+    x, s = x.to(DEV), s.to(DEV)
+    want = beams_run(x, s, 4, keep)
+    for _ in range(200):
+        assert all(torch.equal(a, b) for a, b in zip(beams_run(x, s, 4, keep), want))
