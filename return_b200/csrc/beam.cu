@@ -298,6 +298,7 @@ beam_part_kernel(const float* __restrict__ logits, long long ld, int V, int part
     __syncthreads();
     held = s_n;
     if (held > COLLECT) {                                     // once more, tile by tile
+        asm volatile("cp.async.wait_group 0;\n" ::);          // of tiles behind the part: zeros that may still be on their way to the ring
         __syncthreads();
         if (tid == 0) s_n = 0;
         held = 0;

@@ -534,3 +534,15 @@ def test_beam_select_gives_the_same_every_time(rows, V, keep):
     want = beams_run(x, s, 4, keep)
     for _ in range(200):
         assert all(torch.equal(a, b) for a, b in zip(beams_run(x, s, 4, keep), want))
+
+
+@pytest.mark.parametrize("rows,V,keep", [(600, 2048, 100), (600, 2500, 128), (600, 5000, 7), (600, 3001, 64), (300, 16388, 128), (300, 24576, 128), (300, 40000, 3)])
+def test_beam_select_walks_rising_rows_twice(rows, V, keep):
+    """Rows that rise overflow what is collected and are walked again; nothing of the first walk's tiles may reach the second's."""
+    x = torch.linspace(-30, 0, V).expand(rows, V) + torch.linspace(0, 5, rows)[:, None]
+    s = torch.zeros(rows)
+    beams_check(x, s, 1, keep)
+    x, s = x.to(DEV), s.to(DEV)
+    want = beams_run(x, s, 1, keep)
+    for _ in range(50):
+        assert all(torch.equal(a, b) for a, b in zip(beams_run(x, s, 1, keep), want))
