@@ -1381,10 +1381,9 @@ struct TreeCall {
     const float* sink;
     int splits, share;
     bool joined;
-    float* scratch;
+    float *scratch, *part_ml;
     int* status;
     cudaStream_t st;
-    float* part_ml() const { return scratch != nullptr ? scratch + (size_t)splits * total_rows * Hq * D : nullptr; }
 };
 
 // A launch whose shares of a block of rows are a cluster, if they join their outputs themselves.
@@ -1411,7 +1410,7 @@ template <typename TA>
 int merge(const TreeCall& a) {
     if (a.splits <= 1 || a.joined) return 0;
     dim3 grid((a.max_nodes * a.Hq + 7) / 8, a.segments);
-    return rb_launch_pdl(a.D % 4 == 0 && a.D <= 128 ? tree_merge_kernel<TA, 4> : tree_merge_kernel<TA, 1>, grid, dim3(256), 0, a.st, a.scratch, a.part_ml(), a.cu_q, a.seg_pos0, a.total_rows, a.Hq, a.D,
+    return rb_launch_pdl(a.D % 4 == 0 && a.D <= 128 ? tree_merge_kernel<TA, 4> : tree_merge_kernel<TA, 1>, grid, dim3(256), 0, a.st, a.scratch, a.part_ml, a.cu_q, a.seg_pos0, a.total_rows, a.Hq, a.D,
                          a.window, a.share, a.splits, (TA*)a.out, a.sink);
 }
 
@@ -1425,7 +1424,7 @@ int mma_launch(const TreeCall& a) {
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + MROWS - 1) / MROWS * a.Hkv, a.segments, a.splits);
     const int e = launch(a, tree_mma_kernel<TA, DP>, grid, MTHREADS, SMEM, (const TA*)a.q, a.ld, (const TA*)a.kpool,
                                 (const TA*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (TA*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, vec);
+                                a.part_ml, a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, vec);
     return e ? e : merge<TA>(a);
 }
 template <typename TA>
@@ -1454,7 +1453,7 @@ int tc5_kernel_launch(const TreeCall& a) {
     dim3 grid((a.max_nodes * (a.Hq / a.Hkv) + ROWS - 1) / ROWS * a.Hkv, a.segments, a.splits);
     const int e = launch(a, tree_tc5_kernel<D, STREAMS, CAP, WHOLE>, grid, S::THREADS, S::SMEM, (const bf16*)a.q, a.ld, (const bf16*)a.kpool,
                                 (const bf16*)a.vpool, a.cu_q, a.seg_pos0, a.parent, a.block_table, a.bt_stride, a.page_size, a.pages, (bf16*)a.out, a.scratch,
-                                a.part_ml(), a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, a.status, by_tma, kmap, vmap);
+                                a.part_ml, a.total_rows, a.Hq, a.Hkv, a.D, a.scale, a.window, a.softcap, a.sink, a.splits > 1 ? a.share : 0, (int)a.joined, a.status, by_tma, kmap, vmap);
     return e ? e : merge<bf16>(a);
 }
 
@@ -1471,19 +1470,21 @@ RB_EXPORT int rb_tree_join_max() { return JOIN_MAX; }
 
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys
 // go to one CTA for every `share` key tiles of 64, `splits` at most, which are a cluster and join their outputs if `joined` (JOIN_MAX at most); else scratch holds
-// splits * total_rows * Hq * (D + 2) floats.
+// splits * total_rows * Hq * D floats for their outputs, on a 16-byte boundary, and scratch_ml splits * total_rows * Hq pairs of a maximum and a sum, on one of 8.
 // query_tiles: 0 the kernel for any type and head size; 1 or 2 the tcgen05 kernel with so many tiles of 128 rows a CTA (bfloat16, D and ld multiples
 // of 8, one tile beyond 128; pools, queries and out on 16-byte boundaries).  *status is raised if a wait gave up.
 RB_EXPORT int rb_tree_attention(const void* q, int ld, const void* kpool, const void* vpool, const int* cu_q, const int* seg_pos0,
                                 const int* parent, const int* block_table, int bt_stride, int page_size, int pages, void* out, int act_dtype,
                                 int segments, int max_nodes, int total_rows, int Hq, int Hkv, int D, float scale, int window,
-                                float softcap, const float* sink, int splits, int share, int joined, void* scratch, int query_tiles, int* status,
+                                float softcap, const float* sink, int splits, int share, int joined, void* scratch, void* scratch_ml, int query_tiles, int* status,
                                 cudaStream_t st) {
     if (segments <= 0 || max_nodes <= 0) return 0;
     if (segments > 65535 || max_nodes > TREE_MAX_NODES || D <= 0 || D > TREE_MAX_D || Hkv <= 0 || Hq % Hkv || page_size <= 0) return (int)cudaErrorInvalidValue;
-    if (splits < 1 || splits > TREE_MAX_SPLITS || (splits > 1 && (share <= 0 || (joined ? splits > JOIN_MAX : scratch == nullptr)))) return (int)cudaErrorInvalidValue;
+    if (splits < 1 || splits > TREE_MAX_SPLITS || (splits > 1 && (share <= 0 || (joined ? splits > JOIN_MAX : scratch == nullptr || scratch_ml == nullptr))))
+        return (int)cudaErrorInvalidValue;
+    if (((uintptr_t)scratch & 15) || ((uintptr_t)scratch_ml & 7)) return (int)cudaErrorInvalidValue;
     TreeCall a = {q, kpool, vpool, ld, cu_q, seg_pos0, parent, block_table, bt_stride, page_size, out, segments, max_nodes, total_rows, Hq, Hkv,
-                  D, pages, scale, window, softcap, sink, splits, share, joined && splits > 1, (float*)scratch, status, st};
+                  D, pages, scale, window, softcap, sink, splits, share, joined && splits > 1, (float*)scratch, (float*)scratch_ml, status, st};
     if (query_tiles > 0) {
         if (act_dtype != RB_BF16 || D % 8 || query_tiles > (D > 128 ? 1 : 2) || status == nullptr) return (int)cudaErrorInvalidValue;
         if ((((uintptr_t)q | (uintptr_t)kpool | (uintptr_t)vpool | (uintptr_t)out) & 15) || ld % 8) return (int)cudaErrorInvalidValue;

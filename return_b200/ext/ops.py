@@ -2256,7 +2256,7 @@ def tree_lib() -> ctypes.CDLL:
     if _tree is None:
         lib = build.load("return_tree", _TREE_SOURCES, {"RB_PDL_MODE": PDL_MODE})
         P, I, F = c_void_p, c_int, c_float
-        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, I, P, I, P, P]
+        lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, I, P, P, I, P, P]
         lib.rb_tree_attention.restype = c_int
         _tree = build.native_calls(lib)
     return _tree
@@ -2383,6 +2383,13 @@ def tree_cost(nodes, ends, window, rows_per_node: int, kv_heads: int, rows: int,
     return best
 
 
+def tree_scratch(splits: int, rows: int, head_dim: int):
+    """(floats, where the pairs begin) of the scratch in which shares of the keys leave ``rows`` partial outputs each: first the outputs, then a
+    (maximum, sum) a row, which are moved eight bytes at a time and so begin on a 16-byte boundary whatever the outputs' number."""
+    pairs = -(-splits * rows * head_dim // 4) * 4
+    return pairs + 2 * splits * rows, pairs
+
+
 def tree_shares(*step):
     """(splits, share) of ``tree_cost``."""
     return tree_cost(*step)[1:]
@@ -2427,12 +2434,16 @@ def tree_attention(qkv, k_pool, v_pool, batch, block_table, page_size, out, num_
         shares[kind] = _tree_launch(batch, page_size, block_table, num_heads, num_kv_heads, head_dim, window, dtype, kind)
     tiles, splits, share, joined = shares[kind]
     merged = splits > 1 and not joined
-    # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
-    scratch = torch.empty(splits * T * num_heads * (head_dim + 2), dtype=torch.float32, device=qkv.device) if merged else None
+    scratch_at = pairs_at = None
+    if merged:                                         # a buffer of this call's: two streams, or two captured graphs, may run the same step's tables at once
+        floats, pairs = tree_scratch(splits, T * num_heads, head_dim)
+        scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
+        scratch_at = scratch.data_ptr()
+        pairs_at = scratch_at + 4 * pairs
     _check(tree_lib().rb_tree_attention(q_at, ld, k_at, v_at, cu_q.data_ptr(), seg_pos0.data_ptr(), parent.data_ptr(),
                                         block_table.data_ptr(), block_table.stride(0), page_size, k_pool.shape[0], out_at, code, n, longest, T,
                                         num_heads, num_kv_heads, head_dim, scale, window, softcap, _sink_ptr(sink, num_heads), splits, share, int(joined),
-                                        None if scratch is None else scratch.data_ptr(), tiles, _status_word(qkv.device) if tiles else None,
+                                        scratch_at, pairs_at, tiles, _status_word(qkv.device) if tiles else None,
                                         _stream()), "tree_attention", 2 if merged else 1)
 
 

@@ -120,6 +120,15 @@ def test_tree_shares_cover_the_keys(monkeypatch, kind):
             assert share >= 1 and splits * share >= max(tiles) > (splits - 1) * share
 
 
+def test_scratch_of_shares_that_a_launch_merges():
+    """Odd head sizes, heads, nodes and splits: pairs begin where eight bytes can be moved, behind all outputs, and fit."""
+    for splits in range(2, ops.TREE_MAX_SPLITS + 1):
+        for rows in (1, 2, 3, 7, 35):
+            for head_dim in (1, 3, 5, 6, 33, 128, 255):
+                floats, pairs = ops.tree_scratch(splits, rows, head_dim)
+                assert pairs % 4 == 0 and splits * rows * head_dim <= pairs < splits * rows * head_dim + 4 and floats == pairs + 2 * splits * rows
+
+
 # ---------------------------------------------------------------------------------------- drafted trees on the host
 
 def test_batch_of_drafted_trees():

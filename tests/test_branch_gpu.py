@@ -200,6 +200,22 @@ def test_tree_attention_shares_joined_or_merged(splits, share, D, dtype, joined,
         a.check(a.run())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,D,nodes", [(1, 1, 5, [1]), (3, 1, 33, [5]), (3, 3, 7, [1, 3, 1]), (1, 1, 255, [3])])
+@pytest.mark.parametrize("splits,share", [(3, 4), (11, 1), (5, 3)])
+def test_tree_attention_odd_sizes_merged(splits, share, heads, kv_heads, D, nodes, dtype, monkeypatch):
+    """An odd number of floats lies in front of the shares' maxima and sums."""
+    monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
+    monkeypatch.setattr(ops, "tree_joins", lambda *a: False)
+    a = Attention(37, dtype, heads, kv_heads, D, 16, [700, 3, 65][:len(nodes)], nodes)
+    a.check(a.run())
+
+
+def test_tree_attention_of_one_row_of_an_odd_size():
+    a = Attention(41, torch.float32, 1, 1, 5, 16, [700], [1])
+    a.check(a.run())
+
+
 @pytest.mark.parametrize("falling", [False, True])
 @pytest.mark.parametrize("splits,share", [(1, 0), (4, 5)])
 @pytest.mark.parametrize("softcap", [None, 60.0])
