@@ -131,7 +131,7 @@ class BeamSearch:
                 budget -= n
             logits = r.step(entries)
             for k, i in enumerate(ends):
-                rows[i] = logits[k:k + 1]
+                rows[i] = logits[k:k + 1].clone()             # a captured step's logits are the graph's own: the next one writes over them
         return torch.cat(rows)
 
     def _select(self, live: List[_Search], logits: torch.Tensor, beams: int):

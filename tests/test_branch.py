@@ -251,3 +251,33 @@ def test_draft_settings_refuse():
     for bad in (-1, ops.TREE_MAX_NODES):
         with pytest.raises(ValueError, match="draft_tokens"):
             EngineConfig(draft_tokens=bad)
+
+
+@pytest.mark.parametrize("chunk,lengths", [(1, [1, 1]), (1, [3, 1, 2]), (2, [1, 1, 1, 1, 1]), (4, [5, 1, 1, 6])])
+def test_prompts_of_a_beam_search_keep_their_logits(chunk, lengths):
+    """A step of single tokens hands out the captured graph's own logits, which the next one writes over."""
+    from return_b200.engine.beams import BeamSearch
+
+    class Runner:
+        vocab_size, max_positions = 7, 100
+        config = types.SimpleNamespace(max_reside=8, prefill_chunk=chunk)
+        static = torch.zeros((8, 7))
+
+        def add_request(self, rid):
+            pass
+
+        def reserve(self, rid, tokens, want):
+            return tokens, want
+
+        def step(self, entries):
+            ends = [tokens[-1] for tokens, want in entries if want]
+            out = self.static if all(len(tokens) == 1 for tokens, _ in entries) else torch.zeros_like(self.static)
+            out.fill_(-1)
+            for i, t in enumerate(ends):
+                out[i] = t
+            return out[:len(ends)]
+
+    search = BeamSearch(Runner(), 1, 4)
+    from return_b200.engine.beams import _Search
+    group = [_Search(i, [0] * (n - 1) + [10 + i]) for i, n in enumerate(lengths)]
+    assert search._prompts(group)[:, 0].tolist() == [10 + i for i in range(len(lengths))]

@@ -233,6 +233,19 @@ def test_beam_search_equals_plain(tmp_path, case, beams, penalty, graph):
         assert eng.runner.manager.num_requests == 0
 
 
+@pytest.mark.parametrize("chunk,lengths", [(1, (3, 1)), (2, (1, 1, 1, 1, 1)), (4, (5, 1, 2, 6))])
+def test_beam_search_of_prompts_in_single_tokens(tmp_path, chunk, lengths):
+    """Prompts that end in captured steps of single tokens, several steps after each other."""
+    d = helpers.make_model_dir(tmp_path, "A")
+    prompts = [helpers.random_ids(256, n, 60 + i) for i, n in enumerate(lengths)]
+    eng = engine_of(d, max_reside=10, prefill_chunk=chunk, use_cuda_graph=True)
+    for _ in range(2):                             # graphs captured, and replayed
+        for prompt, results in zip(prompts, eng.beam_search(prompts, beams=2, max_new_tokens=3)):
+            want = plain_beams(lambda ids: helpers.plain_logits(d, ids), prompt, 2, 3, 1.0, None)
+            assert [r.output_ids for r in results] == [t for t, _, _ in want]
+            assert all(abs(r.score - s) < 1e-3 for r, (_, s, _) in zip(results, want))
+
+
 @pytest.mark.parametrize("kind", ["window", "states"])
 def test_beams_hold_what_their_tokens_say(tmp_path, kind):
     """A long search over pages, windows and states that part ways again and again: every result's score is that of its tokens run afresh."""
