@@ -12,7 +12,9 @@
 // random logits.  Where what is collected overflows (rising logits) the part is walked once more, with a selection in every tile, and
 // where a tile's own overflows (equal logits), its best are taken one by one.
 // beam_merge_kernel: a CTA a request puts the rows' sums together and takes the best of all parts' lists.  Totals are
-// compared in 64 bits, so that logits which differ keep their order however far down the scores are; one rounding at the store.
+// compared in 64 bits, a logit less its row's maximum first, so that logits which differ keep their order whatever their size and however far down the
+// scores are; one rounding at the store.  (Beside a score beyond some -2^50, a finite mask's, 64 bits do not tell words apart either: which of them are
+// taken is then the lists' and the places' order.)  Sums of exponentials are float32, each term off by 2^-21 at most relative to it, whatever the logits' size.
 //
 // What bounds it: 128 rows of 151,936, the 16 best of eight beams, 27.8 us, of which the parts take 24 (3.2 TB/s; a stream alone would take 12): a CTA's first
 // tile waits 2.3 us for memory and 4.6 for its selection, later tiles for the logits, the last ranking and sums 2 us, and 256 CTAs fill 108 of 148 SMs
@@ -41,9 +43,9 @@ __device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
     return v;
 }
 __device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
     unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
@@ -252,18 +254,19 @@ beam_part_kernel(const float* __restrict__ logits, long long ld, int V, int part
         stage = stage + 1 == RING ? 0 : stage + 1;
         float x[E], four[E / 4];
         const float mine = take(from, base, x, four);
-        const float m = fmaxf(top, mine), ref = m == -INFINITY ? 0.f : m, shift = -ref * LOG2E;
+        const float m = fmaxf(top, mine), ref = m == -INFINITY ? 0.f : m;
         unsigned long long tile = pack2(0.f, 0.f);            // a sum of few terms at a time keeps its rounding small
-        const unsigned long long unit2 = pack2(LOG2E, LOG2E), shift2 = pack2(shift, shift);
+        // the maximum is taken off before the scale: a product of it would be off by what counts where logits are large, and infinite at the lowest
+        const unsigned long long unit2 = pack2(LOG2E, LOG2E), back2 = pack2(-ref, -ref);
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             float y0, y1;
-            unpack2(fma2(pack2(x[e], x[e + 1]), unit2, shift2), y0, y1);
+            unpack2(mul2(add2(pack2(x[e], x[e + 1]), back2), unit2), y0, y1);
             tile = add2(tile, pack2(fast_exp2(y0), fast_exp2(y1)));
         }
         float even, uneven;
         unpack2(tile, even, uneven);
-        sum = sum * fast_exp2(fmaf(top, LOG2E, shift)) + (even + uneven);       // 2^-inf before the first number
+        sum = sum * fast_exp2((top - ref) * LOG2E) + (even + uneven);       // 2^-inf before the first number
         top = m;
         odd = odd || m == INFINITY;
         if (base == first) {
@@ -346,7 +349,8 @@ __global__ void __launch_bounds__(MERGE_THREADS)
 beam_merge_kernel(const float* __restrict__ scores, const float* __restrict__ part_ms, const Key* __restrict__ cand, int beams, int V, int parts,
                   int keep, float* __restrict__ scores_out, int* __restrict__ beams_out, int* __restrict__ tokens_out) {
     constexpr int T = MERGE_THREADS, WARPS = T / 32;
-    __shared__ double s_shift[BEAM_MAX_BEAMS];                // score - lse; NaN: the row counts as -inf
+    // a row's maximum, which is taken off its logits first (they are of one size, the score is not), and score - log(sum); NaN: the row counts as -inf
+    __shared__ double s_top[BEAM_MAX_BEAMS], s_shift[BEAM_MAX_BEAMS];
     __shared__ double s_v[COLLECT];
     __shared__ int s_at[COLLECT], s_n, s_count[2];
     __shared__ __align__(16) float s_list[T];
@@ -379,15 +383,17 @@ beam_merge_kernel(const float* __restrict__ scores, const float* __restrict__ pa
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0)
-            s_shift[b] = top != -INFINITY && isfinite(score) ? (double)score - ((double)top + log(sum)) : __longlong_as_double(0x7ff8000000000000ll);
+        if (lane == 0) {
+            s_top[b] = (double)top;
+            s_shift[b] = top != -INFINITY && isfinite(score) ? (double)score - log(sum) : __longlong_as_double(0x7ff8000000000000ll);
+        }
     }
     __syncthreads();
     // candidate i of the request: its total and its place (b, v) in the order of ties, -1 where there is none; a dead row offers its first words
     auto candidate = [&](int i, Key key, double& v, int& at) {
         const int b = i / per_row, k = i - b * per_row;
         const double shift = s_shift[b];
-        v = (double)value_of(key) + shift;
+        v = ((double)value_of(key) - s_top[b]) + shift;
         at = key == NONE ? -1 : b * V + place_of(key);
         if (isnan(shift)) {
             v = none;

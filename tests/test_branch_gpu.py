@@ -562,3 +562,52 @@ def test_beam_select_walks_rising_rows_twice(rows, V, keep):
     want = beams_run(x, s, 1, keep)
     for _ in range(50):
         assert all(torch.equal(a, b) for a, b in zip(beams_run(x, s, 1, keep), want))
+
+
+LOWEST = [torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min, -1e38, -1e30, -1e20, -1e10, -65504.0]
+
+
+def masked_rows(rows, V, value, seed):
+    """Most words masked, in long runs and one by one, and whole rows of the mask."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, V), generator=g) * 3
+    x[torch.rand((rows, V), generator=g) < 0.5] = value
+    x[:, V // 5:V - V // 5] = value
+    x[3] = value
+    return x, -torch.rand(rows, generator=g)
+
+
+def shifted_rows(rows, V, shift):
+    g = torch.Generator().manual_seed(V)
+    return torch.randn((rows, V), generator=g) * 3 + shift, -30 * torch.rand(rows, generator=g)
+
+
+def certain_rows(rows, V, top):
+    """One word takes nearly everything."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((rows, V), generator=g)
+    x[torch.arange(rows), torch.randint(0, V, (rows,), generator=g)] = top + torch.rand(rows, generator=g)
+    return x, -torch.rand(rows, generator=g)
+
+
+@pytest.mark.parametrize("value", LOWEST, ids=str)
+@pytest.mark.parametrize("V", [100, 2048, 40000, 151936])
+def test_beam_select_masks_of_finite_values(V, value):
+    x, s = masked_rows(6, V, value, V)
+    beams_check(x, s, 3, 7)
+    beams_check(x[3:4], s[3:4], 1, 20)                                          # nothing but the mask
+
+
+@pytest.mark.parametrize("shift", [100.0, -100.0, 1000.0, -1000.0, 10000.0, -10000.0])
+@pytest.mark.parametrize("V", [1000, 32771, 151936])
+def test_beam_select_of_shifted_rows(V, shift):
+    """A constant added to a row changes nothing, but for what it rounds off the logits."""
+    x, s = shifted_rows(8, V, shift)
+    beams_check(x, s, 4, 8)
+
+
+@pytest.mark.parametrize("top", [20.0, 40.0, 57.0, 100.0, 1003.0, 10007.0, 1e30])
+@pytest.mark.parametrize("V", [1000, 40000])
+def test_beam_select_of_words_that_are_certain(V, top):
+    x, s = certain_rows(6, V, top)
+    beams_check(x, s, 3, 3)
