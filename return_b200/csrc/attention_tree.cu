@@ -1170,6 +1170,18 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         }
         const bool odd = *odd_values != 0 && row_valid && (!STREAMS || (grp == 0 && copy == 0));
         unsigned char* slot = sK + (size_t)(grp * QM + r) * (D * 4);
+        // where key j lies in the pools, -1: on no page; and its probability beside mu, from the operands
+        auto key_at = [&](int j) {
+            const int page = page_at(bt_row + pg.block(j), pages);
+            return page < 0 ? -1ll : (((long long)page * Hkv + kvh) * pg.page_size + pg.row(j)) * head;
+        };
+        auto probability = [&](long long key) {
+            float s = 0.f;
+            const bf16* qrow = q + token * ld + (size_t)h * head;
+            for (int d = 0; d < head; ++d) s = fmaf(__bfloat162float(qrow[d]), __bfloat162float(kpool[key + d]), s);
+            s = CAP ? fast_tanh(s * (scale / softcap)) : s;
+            return fast_exp2(fmaf(s, scale_eff, -mu));
+        };
 #pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
             unsigned o[32];
@@ -1178,25 +1190,50 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mine);
+            auto any_odd = [&](long long key) {               // among these columns of a value
+                unsigned any = 0u;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2)
+                    if (c0 + i < head) any |= odd_halves(*reinterpret_cast<const unsigned*>(vpool + key + c0 + i));
+                return any != 0u;
+            };
+            if (STREAMS && copies > 1 && row_valid) {
+                // A value that is no number in a tile that is seen in full is multiplied by zero in the copies whose key it is not: there such columns
+                // become zero, and in the copy whose key it is what the definition gives.
+                float none = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) none = fmaf(__uint_as_float(o[i]), 0.f, none);
+                if (!(none == 0.f)) {
+                    unsigned found = 0u;
+                    for (int t = 0; t < n_mine; ++t) {
+                        const int j_base = (jt_begin + tile_no(grp, t)) * KN;
+                        if (!whole(j_base)) continue;
+                        for (int j = 0; j < KN; ++j) {
+                            const long long key = key_at(j_base + j);
+                            if (key < 0 || !any_odd(key)) continue;
+                            const bool own = j / (KN / copies) == copy;
+                            const float p = own ? probability(key) : 0.f;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float v = c0 + i < head ? __bfloat162float(vpool[key + c0 + i]) : 0.f;
+                                if (isfinite(v)) continue;
+                                if (!(found >> i & 1u)) o[i] = 0u;
+                                found |= 1u << i;
+                                if (own) o[i] = __float_as_uint(fmaf(p, v, __uint_as_float(o[i])));
+                            }
+                        }
+                    }
+                }
+            }
             if (odd) {
                 // what the products left out: values that are no numbers, where this row sees their keys
                 for (int t = 0; t < n_tiles; ++t) {
                     const int j_base = (jt_begin + t) * KN;
                     if (whole(j_base)) continue;
                     for (unsigned long long vis = visible(j_base); vis != 0ull; vis &= vis - 1ull) {
-                        const int j = j_base + __ffsll((long long)vis) - 1, page = page_at(bt_row + pg.block(j), pages);
-                        if (page < 0) continue;
-                        const size_t key = (((size_t)page * Hkv + kvh) * pg.page_size + pg.row(j)) * head;
-                        unsigned any = 0u;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            if (c0 + i < head) any |= odd_halves(*reinterpret_cast<const unsigned*>(vpool + key + c0 + i));
-                        if (any == 0u) continue;
-                        float s = 0.f;
-                        const bf16* qrow = q + token * ld + (size_t)h * head;
-                        for (int d = 0; d < head; ++d) s = fmaf(__bfloat162float(qrow[d]), __bfloat162float(kpool[key + d]), s);
-                        s = CAP ? fast_tanh(s * (scale / softcap)) : s;
-                        const float p = fast_exp2(fmaf(s, scale_eff, -mu));
+                        const long long key = key_at(j_base + __ffsll((long long)vis) - 1);
+                        if (key < 0 || !any_odd(key)) continue;
+                        const float p = probability(key);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const float v = c0 + i < head ? __bfloat162float(vpool[key + c0 + i]) : 0.f;

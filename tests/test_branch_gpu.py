@@ -266,6 +266,28 @@ def test_what_a_node_does_not_see_does_not_reach_it(heads, D, value, dtype):
         del old
 
 
+@pytest.mark.parametrize("splits,share,joined", [(1, 0, False), (3, 8, True), (5, 4, False)])
+@pytest.mark.parametrize("heads,D", [(4, 128), (8, 128), (16, 128), (4, 64), (8, 64), (4, 256), (8, 256), (8, 104), (4, 48)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_values_that_every_node_sees(heads, D, dtype, splits, share, joined, kernel, monkeypatch):
+    """In tiles seen in full, of 16, 32 and 64 rows a tile and more: what the definition gives, and every other column as it was."""
+    monkeypatch.setattr(ops, "tree_shares", lambda *a: (splits, share))
+    monkeypatch.setattr(ops, "tree_joins", lambda *a: joined)
+    inf = float("inf")
+    for nodes, softcap in (([8, 2, 1], None), ([16, 3, 33], 30.0)):
+        a = Attention(43, dtype, heads, 2, D, 16, [1200, 3, 250], nodes, softcap=softcap)
+        for t, j, column, value in ((0, 100, 0, inf), (0, 127, 7, -inf), (0, 700, 33, inf), (0, 130, 33, inf), (0, 64, 40, inf), (0, 900, 40, -inf),
+                                    (0, 0, D - 1, inf), (0, 511, 20, float("nan")), (2, 5, 2, inf), (2, 64, 3, -inf), (2, 200, 3, inf)):
+            a.v[a.tables[t][j // 16], :, j % 16, column] = value
+        want, size = a.want()
+        got = a.run().double().cpu().reshape(want.shape)
+        odd = ~torch.isfinite(want)
+        assert odd[:, :, :].any(-1).all(-1).tolist() == [True] * nodes[0] + [False] * nodes[1] + [True] * nodes[2]
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+        off = (got - want).abs() - a.bound(want, size)
+        assert off[~odd].max() <= 0
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("page", [16, 24])
 @pytest.mark.parametrize("D", [128, 48])
