@@ -4,7 +4,9 @@ The reference samples one continuation a request.  Here a prompt's ``beams`` bes
 request of the cache manager, all beams of all prompts decode in one step (through the captured graphs), one kernel selects the best
 continuations of every prompt over its beams and the vocabulary (``ops.beam_select``), and a beam that is carried on more than once is
 forked: its full pages are shared, the rows of its partly filled last page and its per-request states are copied
-(``ModelRunner.fork_requests``).  The beam carried on first keeps its pages and its slot.
+(``ModelRunner.fork_requests``).  The beam carried on first keeps its pages and its slot.  Where the pages do not suffice for all prompts
+that search at once, the last one gives back what it holds and starts again behind the others; one that does not fit alone raises
+``KVCapacityError``.
 
 A continuation that ends with ``eos_token_id`` leaves the beams with the score (sum of its log-probabilities) / length ** length_penalty
 if it is among the ``beams`` best of its step; the search of a prompt ends when ``beams`` have left and none that goes on has a higher
@@ -13,7 +15,7 @@ score than the lowest of them, or at ``max_new_tokens``.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -38,12 +40,15 @@ class _Search:
 
     def __init__(self, index: int, prompt: Sequence[int]):
         self.index, self.prompt = index, list(prompt)
+        self.serial = 0
+        self.begin()
+
+    def begin(self) -> None:
         self.names: List[tuple] = []
         self.tokens: List[List[int]] = []
         self.scores: List[float] = []
         self.parents: List[int] = []             # which beam of the step before each one goes on from
         self.left: List[BeamResult] = []
-        self.serial = 0
 
     def name(self) -> tuple:
         self.serial += 1
@@ -62,6 +67,7 @@ class BeamSearch:
         if V < self.keep or not (eos_token_id is None or 0 <= eos_token_id < V):
             raise ValueError(f"a vocabulary of {V} for {beams} beams, eos_token_id={eos_token_id}")
         self.runner, self.beams, self.max_new, self.penalty, self.eos = runner, beams, max_new_tokens, length_penalty, eos_token_id
+        self._put_off: List[_Search] = []        # those of the prompts at hand that found no pages beside the others
 
     # ------------------------------------------------------------------ all prompts
     def run(self, prompts: Sequence[Sequence[int]]) -> List[List[BeamResult]]:
@@ -72,67 +78,108 @@ class BeamSearch:
             if len(p) + self.max_new - 1 > r.max_positions:
                 raise KVCapacityError(f"a prompt of {len(p)} tokens and {self.max_new} new ones exceed the engine's sequence limit {r.max_positions}")
         searches = [_Search(i, p) for i, p in enumerate(prompts)]
-        at_once = r.config.max_reside // self.beams
-        for i in range(0, len(searches), at_once):            # as many prompts at a time as have slots for all their beams
-            group = searches[i:i + at_once]
+        at_once, waiting = r.config.max_reside // self.beams, list(searches)
+        while waiting:                                        # as many prompts at a time as have slots for all their beams
+            group, waiting = waiting[:at_once], waiting[at_once:]
+            self._put_off = []
             try:
                 with torch.cuda.device(r.env.device):
                     self._run_group(group)
             finally:
                 for s in group:
-                    for name in s.names:
-                        r.free_request(name)
-                    s.names = []
+                    self._give_back(s)
+            if self._put_off:
+                at_once = max(1, len(group) - len(self._put_off))
+                waiting = self._put_off[::-1] + waiting
         return [sorted(s.left, key=lambda h: -h.score)[:self.beams] for s in searches]
 
+    def _give_back(self, s: _Search) -> None:
+        for name in s.names:
+            self.runner.free_request(name)
+        s.names = []
+
+    def _put_off_last(self, live: List[_Search]) -> None:
+        s = live.pop()
+        self._give_back(s)
+        s.begin()
+        self._put_off.append(s)
+
     def _run_group(self, group: List[_Search]) -> None:
-        logits = self._prompts(group)
-        for s in group:
+        live = list(group)
+        logits = self._prompts(live)
+        for s in live:
             s.tokens, s.scores = [[]], [0.0]
-        live = group
         while True:
             picked = self._select(live, logits, len(live[0].names))
             for s, candidates in zip(live, picked):
                 self._advance(s, candidates)
             for s in live:                                    # a search that is over gives back what its beams hold
                 if not s.tokens:
-                    for name in s.names:
-                        self.runner.free_request(name)
-                    s.names = []
+                    self._give_back(s)
             live = [s for s in live if s.tokens]
             if not live:
                 return
             self._fork(live)
-            entries = [StepEntry(name, tokens[-1:], [0], self.runner.manager.append(name, 1))
-                       for s in live for name, tokens in zip(s.names, s.tokens)]
-            logits = self.runner.step(entries)
+            logits = self.runner.step(self._next_tokens(live))
 
     # ------------------------------------------------------------------ the pieces of a step
-    def _prompts(self, group: List[_Search]) -> torch.Tensor:
-        """Runs the prompts, portions of several in one step; the logits behind each prompt's last token, [prompts, vocab]."""
+    def _prompts(self, live: List[_Search]) -> torch.Tensor:
+        """Runs the prompts, portions of several in one step; the logits behind each prompt's last token, [prompts, vocab].  Prompts that
+        find no pages leave ``live``."""
         r = self.runner
-        rows: List[Optional[torch.Tensor]] = [None] * len(group)
-        done = [0] * len(group)
-        for s in group:
+        rows: Dict[int, torch.Tensor] = {}
+        done = {s.index: 0 for s in live}
+        for s in live:
             name = s.name()
             r.add_request(name)
             s.names = [name]
-        while any(d < len(s.prompt) for d, s in zip(done, group)):
+        while any(done[s.index] < len(s.prompt) for s in live):
             budget, entries, ends = r.config.prefill_chunk, [], []
-            for i, s in enumerate(group):
-                n = min(budget, len(s.prompt) - done[i])
+            for s in list(live):
+                at = done[s.index]
+                n = min(budget, len(s.prompt) - at)
                 if n <= 0:
                     continue
-                last = done[i] + n == len(s.prompt)
-                entries.append(r.reserve(s.names[0], s.prompt[done[i]:done[i] + n], [n - 1] if last else []))
+                last = at + n == len(s.prompt)
+                try:
+                    entries.append(r.reserve(s.names[0], s.prompt[at:at + n], [n - 1] if last else []))
+                except KVCapacityError:
+                    if s is live[0]:
+                        raise
+                    while s in live:                          # those behind it hold no pages yet
+                        self._put_off_last(live)
+                    break
                 if last:
-                    ends.append(i)
-                done[i] += n
+                    ends.append(s.index)
+                done[s.index] += n
                 budget -= n
+            if not entries:
+                continue
             logits = r.step(entries)
             for k, i in enumerate(ends):
                 rows[i] = logits[k:k + 1].clone()             # a captured step's logits are the graph's own: the next one writes over them
-        return torch.cat(rows)
+        return torch.cat([rows[s.index] for s in live])
+
+    def _next_tokens(self, live: List[_Search]) -> List[StepEntry]:
+        """An entry for every beam's last token."""
+        out: List[List[StepEntry]] = []
+        for s in list(live):
+            if s not in live:                                 # put off for one before it
+                break
+            entries: List[StepEntry] = []
+            while len(entries) < len(s.names):
+                name, tokens = s.names[len(entries)], s.tokens[len(entries)]
+                try:
+                    entries.append(StepEntry(name, tokens[-1:], [0], self.runner.manager.append(name, 1)))
+                except KVCapacityError:
+                    if len(live) == 1:
+                        raise
+                    self._put_off_last(live)
+                    if s not in live:
+                        break
+            else:
+                out.append(entries)
+        return [e for entries in out for e in entries]
 
     def _select(self, live: List[_Search], logits: torch.Tensor, beams: int):
         """For each search its best continuations, best first: (score, beam, token)."""
@@ -171,29 +218,32 @@ class BeamSearch:
     def _fork(self, live: List[_Search]) -> None:
         """Requests for the new beams: one that is carried on first keeps its request, one that is not gives back what it holds, all
         others are copies."""
-        pairs, free = [], []
+        names: List[List[tuple]] = []
+        copies: List[List[tuple]] = []
         for s in live:
-            names: List[Optional[tuple]] = []
+            names.append([])
+            copies.append([])
             going = set()
             for p in s.parents:
                 if p in going:
-                    name = s.name()
-                    pairs.append((s.names[p], name))
-                    names.append(name)
+                    names[-1].append(s.name())
+                    copies[-1].append((s.names[p], names[-1][-1]))
                 else:
                     going.add(p)
-                    names.append(s.names[p])
-            free += [name for p, name in enumerate(s.names) if p not in going]
-            s.names = names
-        for name in free:
-            self.runner.free_request(name)
-        done = False
-        try:
-            if pairs:
-                self.runner.fork_requests(pairs)
-            done = True
-        finally:
-            if not done:                                      # no pages for the copies: they were never made
-                missing = {dst for _, dst in pairs}
-                for s in live:
-                    s.names = [n for n in s.names if n not in missing]
+                    names[-1].append(s.names[p])
+            for p, name in enumerate(s.names):
+                if p not in going:
+                    self.runner.free_request(name)
+            s.names = [name for p, name in enumerate(s.names) if p in going]
+        while any(copies):
+            try:
+                self.runner.fork_requests([pair for pairs in copies for pair in pairs])
+                break
+            except KVCapacityError:                           # nothing was copied
+                if len(live) == 1:
+                    raise
+                self._put_off_last(live)
+                names.pop()
+                copies.pop()
+        for s, now in zip(live, names):
+            s.names = now

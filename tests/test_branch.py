@@ -281,3 +281,85 @@ def test_prompts_of_a_beam_search_keep_their_logits(chunk, lengths):
     from return_b200.engine.beams import _Search
     group = [_Search(i, [0] * (n - 1) + [10 + i]) for i, n in enumerate(lengths)]
     assert search._prompts(group)[:, 0].tolist() == [10 + i for i in range(len(lengths))]
+
+
+class BeamRunner:
+    """A runner on the host: a real cache manager, logits that follow from a request's tokens alone."""
+
+    def __init__(self, pages, max_reside=8, chunk=16, page=4, window=None):
+        from return_b200.cache.manager import CacheManager, GroupSpec
+        self.manager = CacheManager([GroupSpec("full", page, pages)] + ([GroupSpec("win", page, pages, window=window)] if window else []), max_reside)
+        self.vocab_size, self.max_positions = 11, 200
+        self.config = types.SimpleNamespace(max_reside=max_reside, prefill_chunk=chunk)
+        self.env = types.SimpleNamespace(device="cpu")
+        self.tokens, self.steps = {}, 0
+
+    def add_request(self, rid):
+        self.manager.add(rid)
+        self.tokens[rid] = []
+
+    def free_request(self, rid):
+        self.manager.free(rid)
+        del self.tokens[rid]
+
+    def reserve(self, rid, tokens, want):
+        from return_b200.engine.batch import StepEntry
+        return StepEntry(rid, tokens, want, self.manager.append(rid, len(tokens)))
+
+    def fork_requests(self, pairs):
+        self.manager.fork_all(pairs)
+        for src, dst in pairs:
+            self.tokens[dst] = list(self.tokens[src])
+
+    def step(self, entries):
+        self.manager.check()
+        self.steps += 1
+        out = []
+        for e in entries:
+            known = self.tokens[e.rid]
+            assert e.start == len(known) and self.manager.length(e.rid) == len(known) + len(e.tokens)
+            known += e.tokens
+            if e.want:
+                seed = 7
+                for t in known:
+                    seed = (seed * 31 + t + 1) % 1000003
+                out.append(torch.randn(self.vocab_size, generator=torch.Generator().manual_seed(seed)))
+        return torch.stack(out) if out else torch.empty((0, self.vocab_size))
+
+
+def host_beams(runner, prompts, monkeypatch, beams=3, new=9, eos=None):
+    import contextlib
+    from plain import branch_plain
+    from return_b200.engine.beams import BeamSearch
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    search = BeamSearch(runner, beams, new, 1.0, eos)
+    monkeypatch.setattr(search, "_select", lambda live, logits, n: branch_plain.beam_select(
+        logits, torch.tensor([x for s in live for x in s.scores]), n, min(search.keep, n * logits.shape[1])))
+    return [[(r.output_ids, r.score, r.finish_reason) for r in results] for results in search.run(prompts)]
+
+
+@pytest.mark.parametrize("window", [None, 6])
+@pytest.mark.parametrize("eos", [None, 5])
+def test_beam_search_puts_prompts_off_that_find_no_pages(monkeypatch, eos, window):
+    """Down to a pool that holds the beams of one prompt alone, the results are those of a pool that holds all; below it the search raises."""
+    from return_b200.cache.manager import KVCapacityError
+    rs = np.random.RandomState(4)
+    prompts = [[int(x) for x in rs.randint(0, 11, n)] for n in (13, 30, 2, 1, 22, 17, 9)]
+    most = BeamRunner(500, window=window)
+    want = host_beams(most, prompts, monkeypatch, eos=eos)
+    refused, steps = 0, []
+    for pages in range(8, 60):
+        runner = BeamRunner(pages, window=window)
+        try:
+            assert host_beams(runner, prompts, monkeypatch, eos=eos) == want
+            assert not refused or pages > refused
+            steps.append(runner.steps)
+        except KVCapacityError:
+            assert not steps, "a larger pool holds what a smaller one held"
+            refused = pages
+        runner.manager.check()
+        assert runner.manager.num_requests == 0 and not runner.tokens
+    assert 8 <= refused < 20 and max(steps) > min(steps) == most.steps
+    # a prompt that does not fit alone
+    with pytest.raises(KVCapacityError):
+        host_beams(BeamRunner(refused, window=window), prompts, monkeypatch, eos=eos)

@@ -271,6 +271,21 @@ def test_beams_hold_what_their_tokens_say(tmp_path, kind):
     assert eng.generate(prompts, max_new_tokens=3, temperature=0.0)[0].num_tokens == 3
 
 
+def test_beam_search_where_pages_run_short(tmp_path):
+    """Prompts that find no pages beside the others wait; the results are those of a pool that holds all."""
+    d = helpers.make_model_dir(tmp_path, "A")
+    prompts = [helpers.random_ids(256, n, 70 + n) for n in (40, 25, 60, 5)]
+    ask = dict(beams=2, max_new_tokens=20)
+    want = engine_of(d, page_size=8).beam_search(prompts, **ask)
+    for pool in (136, 176, 240):
+        eng = engine_of(d, page_size=8, max_token=pool)
+        got = eng.beam_search(prompts, **ask)
+        assert [[r.output_ids for r in x] for x in got] == [[r.output_ids for r in x] for x in want]
+        assert all(abs(a.score - b.score) < 1e-3 for x, y in zip(got, want) for a, b in zip(x, y))
+        eng.runner.manager.check()
+        assert eng.runner.manager.num_requests == 0 and eng.stats()["page_used"] == 0
+
+
 def test_beam_search_refuses_and_gives_back(tmp_path):
     from return_b200.cache.manager import KVCapacityError
     from return_b200.engine.request import Request
