@@ -24,6 +24,7 @@
 
 #define BEAM_MAX_KEEP 128
 #define BEAM_MAX_BEAMS 64
+#define BEAM_MAX_WORDS (1 << 29)              // of a row: twice a row's length and a few tiles stay within an int
 
 namespace {
 
@@ -533,7 +534,7 @@ RB_EXPORT int rb_beam_select(const float* logits, long long ld, const float* sco
     if (requests <= 0) return 0;
     const int rows = requests * beams;
     if (beams < 1 || beams > BEAM_MAX_BEAMS || keep < 1 || keep > BEAM_MAX_KEEP || V < 1 || rows > 65535) return (int)cudaErrorInvalidValue;
-    if ((long long)beams * V > 0x7ffffffell || keep > (long long)beams * V || ((uintptr_t)scratch & 15)) return (int)cudaErrorInvalidValue;
+    if (V > BEAM_MAX_WORDS || (long long)beams * V > 0x7ffffffell || keep > (long long)beams * V || ((uintptr_t)scratch & 15)) return (int)cudaErrorInvalidValue;
     const Cut cut(rows, V);
     float* ms = (float*)scratch;
     Key* cand = (Key*)(ms + 2ll * rows * cut.parts);

@@ -2616,7 +2616,7 @@ def copy_slots(table: SlotTable, src, dst) -> None:
                table.launches)
 
 
-BEAM_MAX_KEEP, BEAM_MAX_BEAMS = 128, 64
+BEAM_MAX_KEEP, BEAM_MAX_BEAMS, BEAM_MAX_WORDS = 128, 64, 1 << 29
 
 
 @functools.lru_cache(maxsize=256)
@@ -2629,8 +2629,8 @@ def _beam_plan(logits, scores, beams: int, scores_out, beams_out, tokens_out):
         raise KernelError(f"logits: a row per request and beam, up to {BEAM_MAX_BEAMS} beams")
     if not 1 <= keep <= min(BEAM_MAX_KEEP, beams * V):
         raise KernelError(f"{keep} continuations asked for: 1 to {BEAM_MAX_KEEP}, and no more than there are")
-    if rows > 65535 or beams * V >= 2 ** 31 - 1:
-        raise KernelError("at most 65,535 rows, and beams * V within 31 bits")
+    if rows > 65535 or V > BEAM_MAX_WORDS or beams * V >= 2 ** 31 - 1:
+        raise KernelError("at most 65,535 rows of 2^29 words, and beams * V within 31 bits")
     if math.prod(scores) != rows:
         raise KernelError("scores: float32, one per row of logits")
     for name, shape in (("beams_out", beams_out), ("tokens_out", tokens_out)):
@@ -2645,7 +2645,7 @@ def _beam_scratch(rows: int, V: int, keep: int, device: int) -> int:
 
 
 def beam_select(logits, scores, beams: int, scores_out, beams_out, tokens_out) -> None:
-    """The ``scores_out.shape[1]`` best continuations of every request, best first.  ``logits`` float32 [requests * beams, V];
+    """The ``scores_out.shape[1]`` best continuations of every request, best first.  ``logits`` float32 [requests * beams, V], V up to 2^29;
     ``scores`` float32 [requests * beams], the beams' sums of log-probabilities.  A continuation (b, v) has the total
     scores[b] + log_softmax(logits[b])[v]; ties go to the lowest (b, v).  A total that is no number, and every one of a beam whose
     score is not finite, counts as -inf.  Out: totals (float32), beams and tokens (int32), [requests, keep] each."""

@@ -104,6 +104,12 @@ def test_beam_select_refuses():
     refuse("65,535", ops.beam_select, **{**args(rows=65538, requests=21846, V=1, keep=1)})
 
 
+def test_beam_select_refuses_rows_that_its_counters_do_not_hold():
+    for rows, V, beams in ((1, 2 ** 29 + 1, 1), (1, 2 ** 31 - 2, 1), (4, 2 ** 29, 4)):
+        out = torch.zeros((rows // beams, 1))
+        refuse("29 words", ops.beam_select, torch.zeros((1, 1)).expand(rows, V), torch.zeros(rows), beams, out, out.int(), out.int())
+
+
 @pytest.mark.parametrize("kind", sorted(ops.TREE_COSTS))
 def test_tree_shares_cover_the_keys(monkeypatch, kind):
     """Every share is within the launch's splits, and the shares cover the longest walk; a full launch of long CTAs, and a short one, are not split."""
