@@ -2509,21 +2509,15 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
     ``caches``: (pool, block_table) of every group of layers; the row of slot ``seg_pos0 + path[i]`` goes to slot ``seg_pos0 + i``.  The
     request then holds ``seg_pos0 + count`` tokens.  Other rows stay as they are; a move from or to a page that the table marks as
     gone is left out."""
-    looked = [sampled.shape, path.shape, count.shape, emitted.shape]
-    for pool, table in caches:
-        looked += (pool.shape, pool.dtype, table.shape)
-    plan = batch.scratch.get("tree.commit")            # what follows from the shapes is looked at once a step
-    if plan is None or plan[0] != looked:
-        plan = batch.scratch["tree.commit"] = (looked,) + _commit_plan(sampled, batch, caches, path, count, emitted)
-    _, n, width, shapes = plan
+    n, width, shapes = _commit_shapes(sampled, batch, caches, path, count, emitted)
     ints = torch.int32
     tokens = batch.tokens
     if not (sampled.dtype == ints and path.dtype == ints and count.dtype == ints and emitted.dtype == ints and tokens.dtype == ints
             and sampled.is_contiguous() and path.is_contiguous() and count.is_contiguous() and emitted.is_contiguous() and tokens.is_contiguous()):
         raise KernelError("sampled, tokens, path, count and emitted: contiguous int32")
     for pool, table in caches:
-        if not (pool.is_contiguous() and table.dtype == ints and table.stride(1) == 1):
-            raise KernelError("a pool: contiguous; its block_table: int32, unit stride along a row")
+        if table.dtype != ints or table.stride(1) != 1:
+            raise KernelError("block_table: int32, unit stride along a row")
     parent, cu_q, seg_pos0, at = batch.tree_parent, batch.cu_q, batch.seg_pos0, sampled.get_device()
     if at < 0 or not (tokens.get_device() == parent.get_device() == cu_q.get_device() == seg_pos0.get_device() == path.get_device() == count.get_device()
             == emitted.get_device() == at == _device_index()):
@@ -2541,8 +2535,8 @@ def tree_commit(sampled, batch, caches, path, count, emitted) -> None:
         outs = (None, None, None, 0)
 
 
-def _commit_plan(sampled, batch, caches, path, count, emitted):
-    """What ``tree_commit`` knows of a step from shapes alone; raises where they do not fit."""
+def _commit_shapes(sampled, batch, caches, path, count, emitted):
+    """(segments, columns of ``path``, ``_pool_shape`` of every cache) of a commit; raises where shapes do not fit."""
     lengths, shapes = None, []
     for pool, table in caches:
         shape = _pool_shape(pool)
