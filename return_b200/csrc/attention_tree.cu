@@ -1503,6 +1503,7 @@ int tc5_launch(const TreeCall& a) {
 }  // namespace
 
 RB_EXPORT int rb_tree_max_nodes() { return TREE_MAX_NODES; }
+RB_EXPORT int rb_tree_max_splits() { return TREE_MAX_SPLITS; }
 RB_EXPORT int rb_tree_join_max() { return JOIN_MAX; }
 
 // q: rotated queries, row stride ld.  max_nodes: the longest segment's nodes (TREE_MAX_NODES at most).  splits > 1: a segment's keys

@@ -526,6 +526,7 @@ struct Cut {
 
 RB_EXPORT int rb_beam_max_keep() { return BEAM_MAX_KEEP; }
 RB_EXPORT int rb_beam_max_beams() { return BEAM_MAX_BEAMS; }
+RB_EXPORT int rb_beam_max_words() { return BEAM_MAX_WORDS; }
 // 4-byte words of scratch: every part's maximum, sum, and list of keys of eight bytes.
 RB_EXPORT long long rb_beam_scratch(int rows, int V, int keep) { return rows * (long long)Cut(rows, V).parts * (2 + 2ll * keep); }
 

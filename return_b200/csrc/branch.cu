@@ -232,6 +232,7 @@ int pairs_per_cta(int first, int pairs, int unit, int per_sm) {
 }  // namespace
 
 RB_EXPORT int rb_slot_tensors() { return SLOT_TENSORS; }
+RB_EXPORT int rb_commit_max_nodes() { return TREE_MAX_NODES; }
 
 // pool null: the walk alone.  path_out null: no walk is written down (a second group's cache of the same step).
 RB_EXPORT int rb_tree_commit(const int* tokens, const int* parent, const int* sampled, const int* cu_q, const int* seg_pos0, int segments,

@@ -2250,6 +2250,14 @@ TREE_MAX_SPLITS, TREE_JOIN_MAX = 64, 8      # of a segment's keys; so many can j
 TREE_SCRATCH_BYTES = 256 << 20
 
 
+def _same_limits(lib, **limits) -> None:
+    """What a library was compiled with and what the checks here go by are one number each."""
+    for name, here in limits.items():
+        there = getattr(lib, name)()
+        if there != here:
+            raise KernelError(f"{name}: {there} in the compiled library, {here} here")
+
+
 def tree_lib() -> ctypes.CDLL:
     """The attention kernels for drafted trees."""
     global _tree
@@ -2258,6 +2266,7 @@ def tree_lib() -> ctypes.CDLL:
         P, I, F = c_void_p, c_int, c_float
         lib.rb_tree_attention.argtypes = [P, I, P, P, P, P, P, P, I, I, I, P, I, I, I, I, I, I, I, F, I, F, P, I, I, I, P, P, I, P, P]
         lib.rb_tree_attention.restype = c_int
+        _same_limits(lib, rb_tree_max_nodes=TREE_MAX_NODES, rb_tree_max_splits=TREE_MAX_SPLITS, rb_tree_join_max=TREE_JOIN_MAX)
         _tree = build.native_calls(lib)
     return _tree
 
@@ -2276,6 +2285,8 @@ def branch_lib() -> ctypes.CDLL:
         lib.rb_beam_scratch.restype = L
         for name in ("rb_tree_commit", "rb_copy_pages", "rb_copy_slots", "rb_beam_select"):
             getattr(lib, name).restype = c_int
+        _same_limits(lib, rb_slot_tensors=SLOT_TENSORS, rb_commit_max_nodes=TREE_MAX_NODES, rb_beam_max_keep=BEAM_MAX_KEEP,
+                     rb_beam_max_beams=BEAM_MAX_BEAMS, rb_beam_max_words=BEAM_MAX_WORDS)
         _branch = build.native_calls(lib)
     return _branch
 

@@ -110,6 +110,12 @@ def test_beam_select_refuses_rows_that_its_counters_do_not_hold():
         refuse("29 words", ops.beam_select, torch.zeros((1, 1)).expand(rows, V), torch.zeros(rows), beams, out, out.int(), out.int())
 
 
+def test_limits_of_a_library_are_those_of_the_checks():
+    lib = types.SimpleNamespace(rb_a=lambda: 3, rb_b=lambda: 4)
+    ops._same_limits(lib, rb_a=3, rb_b=4)
+    refuse("rb_b: 4 in the compiled library, 5 here", ops._same_limits, lib, rb_a=3, rb_b=5)
+
+
 @pytest.mark.parametrize("kind", sorted(ops.TREE_COSTS))
 def test_tree_shares_cover_the_keys(monkeypatch, kind):
     """Every share is within the launch's splits, and the shares cover the longest walk; a full launch of long CTAs, and a short one, are not split."""
