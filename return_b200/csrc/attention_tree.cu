@@ -105,7 +105,7 @@ __device__ __forceinline__ unsigned line_bits(const unsigned* line, int at) {
 // A CTA of eight warps takes 32 rows and walks its keys in tiles of 64.  Scores: a warp 16 rows by 16 keys; softmax: eight lanes a row;
 // outputs: a warp 16 rows by a quarter of the columns, a tile's sum made by itself and added to the running one.  While the
 // scores are made the tile's values arrive, while the outputs are summed the next tile's keys.
-// bfloat16: operands as they are, probabilities rounded to bfloat16.  float32: an operand is split into three bfloat16 parts, which hold its 24
+// bfloat16: operands as they are, probabilities rounded to bfloat16, the values' type (their sum is of the unrounded ones).  float32: an operand is split into three bfloat16 parts, which hold its 24
 // bits, as it is read (queries once), six of the nine products are made (the rest is below 2^-24 of a product), the largest in an accumulator
 // of its own; values are multiplied by 2^16 first, so that small ones keep their bits, and the sums by 2^-16.
 // A product with a value that is no number reaches every row (zero times infinity), and float32's parts cannot hold one, nor one that 2^16 takes
@@ -567,7 +567,9 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 //   else           up to 256 rows: a query tile of 128 rows a group, both go through every key tile.
 // Per key tile and group:
 //   S = Q K^T      tcgen05.mma, M = 128, N = 64, in tensor memory, two buffers a group;
-//   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into S's own columns.  The reference maximum moves only
+//   softmax        a row a thread (its TMEM lane), no shuffles; P rounded to bfloat16 into S's own columns, since the second product's operands are of
+//                  one type (the sum keeps the unrounded ones; against 64 bits outputs are off by up to 0.0023, with P in 32 bits 0.0017, where
+//                  the rounding of the result alone is 0.0020).  The reference maximum moves only
 //                  when the true one has outrun it by 2^8, so O is rescaled in tensor memory a few times at most;
 //   O += P V       tcgen05.mma, M = 128, N = head size, P from tensor memory, V as it lies in the cache.
 // Warps: four of rows a group (those without rows have nothing to do, and nobody waits for them), for each group one that issues S and one that issues
@@ -579,10 +581,10 @@ tree_mma_kernel(const TA* __restrict__ q, int ld, const TA* __restrict__ kpool, 
 // A key tile that some row does not see in full is looked through for values that are no numbers before the products take it: they are
 // set to zero there (zero times infinity would reach every row) and added to the rows that see them at the end.
 // What bounds it.  Few rows: HBM, and some 14 us around the walk (tables, tensor memory, first keys, outputs, join): 8 trees of 16 nodes behind 2,040
-// tokens, 32 query and 8 key heads of 128, 25.7 us of which the walk of 69 MB takes 11; 64 trees of 8 nodes 133 us, 4.1 TB/s.  Many rows: the row
+// tokens, 32 query and 8 key heads of 128, 25.4 us of which the walk of 69 MB takes 11; 64 trees of 8 nodes 133 us, 4.1 TB/s.  Many rows: the row
 // warps, 1,390 cycles of the 1,830 a key tile of 256 rows takes (exponentials 1,024 of them, were nothing else in their way), while the tensor cores are
-// busy for 45 %: 32 trees of up to 64 nodes behind 2,000 to 8,000 tokens, 64 query and 8 key heads, 321 us, 0.80 PFLOP/s, at the power limit when they
-// follow each other.  Tried there: P through shared memory 345 us; the maximum before the exponentials 335; every fourth or second pair of
+// busy for 45 %: 32 trees of up to 64 nodes behind 2,000 to 8,000 tokens, 64 query and 8 key heads, 322 us, 0.80 PFLOP/s, at the power limit when they
+// follow each other (360 us then).  Tried there: P through shared memory 345 us; the maximum before the exponentials 335; every fourth or second pair of
 // exponentials as a polynomial on the multiply-add units 335 and 348; key tiles cut into shares for the balance of the SMs costs the
 // traffic of partial results, 24 us at two shares, for 8 % of balance.
 using namespace tc5;
@@ -690,7 +692,7 @@ struct Paging {
 };
 
 // grid: (row blocks x kv heads, segments, splits).  CAP: scores are capped.  WHOLE: the head size is D, else head_size, less than D.  (The plain
-// kernels are spared the registers: 32 trees behind 2,000 to 8,000 tokens 328 us, 340 with a head size of its own.)
+// kernels are spared the registers: 32 trees behind 2,000 to 8,000 tokens are 4 % slower with a head size of its own.)
 template <int D, bool STREAMS, bool CAP, bool WHOLE>
 __global__ void __launch_bounds__(Shape<D, STREAMS>::THREADS, 1)
 tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpool, const bf16* __restrict__ vpool,
@@ -813,27 +815,27 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
         // capped scores: a polynomial where all of the warp's are well below the cap
         auto cap = [&](auto& a) {
             constexpr int N = sizeof(a) / sizeof(a[0]);
-                                const float k = scale / softcap;
-                                float far = 0.f;
-            #pragma unroll
-                                for (int e = 0; e < N; e += 2) far = max3(far, fabsf(__uint_as_float(a[e])), fabsf(__uint_as_float(a[e + 1])));
-                                if (!__any_sync(0xffffffffu, !(far * k <= TANH_POLY_MAX))) {
-                                    const unsigned long long k2 = pack2(k, k);
-            #pragma unroll
-                                    for (int e = 0; e < N; e += 2) {
-                                        const unsigned long long x = mul2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), k2), u = mul2(x, x);
-                                        unsigned long long t = fma2(u, pack2(TANH_P4, TANH_P4), pack2(TANH_P3, TANH_P3));
-                                        t = fma2(u, t, pack2(TANH_P2, TANH_P2));
-                                        t = fma2(u, t, pack2(TANH_P1, TANH_P1));
-                                        float t0, t1;
-                                        unpack2(mul2(x, fma2(u, t, pack2(TANH_P0, TANH_P0))), t0, t1);
-                                        a[e] = __float_as_uint(t0);
-                                        a[e + 1] = __float_as_uint(t1);
-                                    }
-                                } else {
-            #pragma unroll
-                                    for (int e = 0; e < N; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
-                                }
+            const float k = scale / softcap;
+            float far = 0.f;
+#pragma unroll
+            for (int e = 0; e < N; e += 2) far = max3(far, fabsf(__uint_as_float(a[e])), fabsf(__uint_as_float(a[e + 1])));
+            if (!__any_sync(0xffffffffu, !(far * k <= TANH_POLY_MAX))) {
+                const unsigned long long k2 = pack2(k, k);
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const unsigned long long x = mul2(pack2(__uint_as_float(a[e]), __uint_as_float(a[e + 1])), k2), u = mul2(x, x);
+                    unsigned long long t = fma2(u, pack2(TANH_P4, TANH_P4), pack2(TANH_P3, TANH_P3));
+                    t = fma2(u, t, pack2(TANH_P2, TANH_P2));
+                    t = fma2(u, t, pack2(TANH_P1, TANH_P1));
+                    float t0, t1;
+                    unpack2(mul2(x, fma2(u, t, pack2(TANH_P0, TANH_P0))), t0, t1);
+                    a[e] = __float_as_uint(t0);
+                    a[e + 1] = __float_as_uint(t1);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) a[e] = __float_as_uint(fast_tanh(__uint_as_float(a[e]) * k));
+            }
         };
         auto walk = [&](auto width) {
             constexpr int W = decltype(width)::value;

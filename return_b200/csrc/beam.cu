@@ -14,11 +14,12 @@
 // beam_merge_kernel: a CTA a request puts the rows' sums together and takes the best of all parts' lists.  Totals are
 // compared in 64 bits, a logit less its row's maximum first, so that logits which differ keep their order whatever their size and however far down the
 // scores are; one rounding at the store.  (Beside a score beyond some -2^50, a finite mask's, 64 bits do not tell words apart either: which of them are
-// taken is then the lists' and the places' order.)  Sums of exponentials are float32, each term off by 2^-21 at most relative to it, whatever the logits' size.
+// taken is then the lists' and the places' order.)  Sums of exponentials are float32; a term d below the
+// maximum is off by 2^-22 + d 2^-23 of itself at most, whatever the logits' size.
 //
-// What bounds it: 128 rows of 151,936, the 16 best of eight beams, 27.8 us, of which the parts take 24 (3.2 TB/s; a stream alone would take 12): a CTA's first
+// What bounds it: 128 rows of 151,936, the 16 best of eight beams, 27.4 us, of which the parts take 24 (3.2 TB/s; a stream alone would take 12): a CTA's first
 // tile waits 2.3 us for memory and 4.6 for its selection, later tiles for the logits, the last ranking and sums 2 us, and 256 CTAs fill 108 of 148 SMs
-// twice and the others once.  Four rows of 32,768: 7.7 us, a selection and a merge.  The first form, without the ring and
+// twice and the others once.  Four rows of 32,768: 7.9 us, a selection and a merge.  The first form, without the ring and
 // the rising bound, took 40 and 10.9 us.
 #include "common.cuh"
 

@@ -60,8 +60,8 @@ struct ByDivisor {
 // grid: (segments, parts of the planes x heads).  Node path[i] moves from slot c + path[i] to slot c + i.  LPR lanes share a row's pieces; a
 // thread keeps to its piece of a (plane, head) and goes through the moves in order, eight loads before their stores.  No store meets a row
 // that is still to be read: path[k] >= k, so a later move's source lies behind every earlier move's destination.
-// Bound by two trips to memory (tables, rows) where little moves: 8 nodes, 28 layers, 3.1 us.  64 requests of which six tokens hold, 36 layers of 8 key heads
-// of 128: 18.4 us in a row of them (14.5 alone), 4.1 TB/s of rows of 256 bytes that lie anywhere; the first, simple form took 34.
+// Bound by two trips to memory (tables, rows) where little moves: 8 nodes, 28 layers, 3.5 us.  64 requests of which six tokens hold, 36 layers of 8 key heads
+// of 128, 75 MB read and written: 17.8 us from HBM, 4.2 TB/s of rows of 256 bytes that lie anywhere, and 10.7 where the rows lie in L2.
 // The walk is done by every CTA for itself (a few hundred cycles); the first part writes it down.  What it takes is asked for at once, the
 // part of the block table that the tree lies on with it.
 template <int W>
@@ -166,7 +166,7 @@ __device__ __forceinline__ void copy_bytes(unsigned char* dst, const unsigned ch
 
 // The first rows[i] rows of page src[i] to page dst[i], in every plane and head.  A head's rows of a page lie together, so a (plane, head) is
 // one run of bytes; a warp takes one at a time, eight loads of a lane before their stores.  Bound by HBM: 72 copies over 36 layers of 8 key heads of 128,
-// 178 MB read and written, 34 us, 5.2 TB/s (28 alone); four copies over 28 layers 3.4 us, the launch and a trip to memory.
+// 178 MB read and written, 33 us, 5.4 TB/s; four copies over 28 layers 2.4 us, the launch and a trip to memory.
 // grid: (copies, parts of the planes x heads).
 template <int W>
 __global__ void __launch_bounds__(COPY_THREADS)
@@ -204,7 +204,7 @@ struct SlotTensors {
 constexpr long long SLOT_CHUNK = 32768;       // bytes of a row that a CTA copies
 
 // Row src[i] to row dst[i] of every tensor.  grid: (pieces of the longest row, tensors, copies).  Bound by HBM: 32 copies in eight tensors of 1 MB a row
-// 80 us, the rate of a plain copy; three copies of 0.5 MB 6.6 us.
+// 80 us, the rate of a plain copy; three copies of 0.5 MB 6.3 us, 4.1 where they lie in L2.
 __global__ void __launch_bounds__(COPY_THREADS)
 copy_slots_kernel(const SlotTensors t, const int* __restrict__ src, const int* __restrict__ dst, int slots) {
     const int from = src[blockIdx.z], to = dst[blockIdx.z];

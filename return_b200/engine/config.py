@@ -10,7 +10,8 @@
 ``keep_sessions`` a request that ends keeps its cache for a follow-up request with the same id, until
 ``release`` or until the pages are needed (the reference always keeps, rollout/engine.py:286-306);
 ``draft_tokens`` most tokens that are drafted for a request beside its next one while it decodes, as a tree that one step checks
-(engine/draft.py; 0: none; the reference drafts none).  Models with per-request states take none.
+(engine/draft.py; 0: none; the reference drafts none).  Models with per-request states take none.  Steps for which nothing is found
+then wait for their tokens on the host, as without captured graphs.
 """
 from __future__ import annotations
 
