@@ -633,3 +633,14 @@ def test_beam_select_of_shifted_rows(V, shift):
 def test_beam_select_of_words_that_are_certain(V, top):
     x, s = certain_rows(6, V, top)
     beams_check(x, s, 3, 3)
+
+
+@pytest.mark.parametrize("value", LOWEST, ids=str)
+@pytest.mark.parametrize("V", [100, 9000, 151936])
+def test_beam_select_of_fewer_words_than_are_asked_for(V, value):
+    """Masked words of finite value fill the places behind the others: the lowest ones of the beam that is ahead, or of the first where none is."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((6, V), value)
+    for b in range(6):
+        x[b, torch.randint(0, V, (2,), generator=g)] = torch.randn(2, generator=g)
+    beams_check(x, -torch.rand(6, generator=g), 3, 16)
