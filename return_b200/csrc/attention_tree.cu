@@ -18,6 +18,7 @@
 // output, maximum and sum in float32, and they are joined in the order of the shares: up to JOIN_MAX shares can be a cluster and join them
 // through shared memory, others leave them in memory for tree_merge_kernel.  So the result depends on `share`, which the host works
 // out from the step's lengths, and on nothing else of the launch.
+#include "pairs.cuh"
 #include "tc5.cuh"
 #include "tma.cuh"
 
@@ -64,19 +65,6 @@ __device__ __forceinline__ int page_at(const int* entry, int pages) {
     const int page = *entry;
     return (unsigned)page < (unsigned)pages ? page : -1;
 }
-
-// x / G and x % G for the rows of a CTA: a quotient by the reciprocal, put right where it is one off.
-struct ByGroup {
-    int G;
-    float inv;
-    __device__ __forceinline__ explicit ByGroup(int g) : G(g), inv(1.0f / (float)g) {}
-    __device__ __forceinline__ int2 operator()(int x) const {
-        int q = (int)((float)x * inv), r = x - q * G;
-        if (r < 0) { --q; r += G; }
-        if (r >= G) { ++q; r -= G; }
-        return make_int2(q, r);
-    }
-};
 
 // The node's own line: bit a of `line` for node x itself and its ancestors less than `window` steps up (window <= 0: all); returns
 // the node's depth.  parent: the segment's list in shared memory.
@@ -613,11 +601,6 @@ template <int D, bool STREAMS> struct Shape {
     static_assert(!STREAMS || GROUPS == 1 || STAGES % 2 == 0, "a ring stage belongs to one group, so that its barriers' phases come in turn");
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
 // D += A B^T with A in tensor memory: a lane a row, two neighbouring values of k a column.
 __device__ __forceinline__ void mma_ts(unsigned d_tmem, unsigned a_tmem, unsigned long long b_desc, unsigned idesc, bool accumulate) {
     asm volatile(
@@ -634,32 +617,6 @@ __device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned (&r)[16
 __device__ __forceinline__ void tmem_st8(unsigned taddr, const unsigned (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                  ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
 }
 __device__ __forceinline__ void cp16u(unsigned smem_addr, const void* gmem, bool pred) {
     const int bytes = pred ? 16 : 0;          // 0: nothing is read, the 16 bytes become zero
@@ -732,7 +689,7 @@ tree_tc5_kernel(const bf16* __restrict__ q, int ld, const bf16* __restrict__ kpo
     const int jt_begin = sg.jt0 + t0, n_tiles = t1 - t0;      // one tile at least
     const int* bt_row = block_table + (size_t)seg * bt_stride;
     const Paging pg(page_size);
-    const ByGroup by_group(G);
+    const ByDivisor by_group(G);
     const unsigned bar0 = smem_u32(bars);
     auto bar = [&](int i) { return bar0 + 8u * i; };
     // STREAMS: the query tile holds its rows `copies` times, copy_rows rows each

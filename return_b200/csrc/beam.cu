@@ -21,7 +21,7 @@
 // tile waits 2.3 us for memory and 4.6 for its selection, later tiles for the logits, the last ranking and sums 2 us, and 256 CTAs fill 108 of 148 SMs
 // twice and the others once.  Four rows of 32,768: 7.9 us, a selection and a merge.  The first form, without the ring and
 // the rising bound, took 40 and 10.9 us.
-#include "common.cuh"
+#include "pairs.cuh"
 
 #define BEAM_MAX_KEEP 128
 #define BEAM_MAX_BEAMS 64
@@ -34,32 +34,6 @@ constexpr int COLLECT = 512;
 constexpr int RING = 3;                       // tiles on their way: two of 32 KB for each of two CTAs an SM
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float fast_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ unsigned long long pack2(float lo, float hi) {
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack2(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // A value of a row and its place in one number that grows as the value does, and falls with the place: the order of the selection.  -0 is 0; a
 // NaN is never asked about.  NONE, the lowest, is no value's.

@@ -5,7 +5,7 @@
 // A pool holds all layers of a group: [planes, pages, heads, page_size, row], planes = layers x (keys, values), or layers for a cache of
 // latents (one head).  A row (a token's key of one head) is row_bytes long.  Everything here is moved as bytes, 16 at a time where rows
 // and pools allow it, else two (the smallest element that is cached).
-#include "common.cuh"
+#include "pairs.cuh"
 
 #define TREE_MAX_NODES 256
 #define SLOT_TENSORS 64
@@ -43,19 +43,6 @@ __device__ int walk_tree(const int* token, const int* parent, const int* sampled
 
 constexpr int COMMIT_THREADS = 256;
 constexpr int MOVES_AT_ONCE = 8;
-
-// x / d and x % d of small numbers: a quotient by the reciprocal, put right where it is one off.
-struct ByDivisor {
-    int d;
-    float inv;
-    __device__ __forceinline__ explicit ByDivisor(int n) : d(n), inv(1.0f / (float)n) {}
-    __device__ __forceinline__ int2 operator()(int x) const {
-        int q = (int)((float)x * inv), r = x - q * d;
-        if (r < 0) { --q; r += d; }
-        if (r >= d) { ++q; r -= d; }
-        return make_int2(q, r);
-    }
-};
 
 // grid: (segments, parts of the planes x heads).  Node path[i] moves from slot c + path[i] to slot c + i.  LPR lanes share a row's pieces; a
 // thread keeps to its piece of a (plane, head) and goes through the moves in order, eight loads before their stores.  No store meets a row
